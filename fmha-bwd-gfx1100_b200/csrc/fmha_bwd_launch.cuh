@@ -399,7 +399,7 @@ int enqueue_backward(T* dQ, T* dK, T* dV, const T* Q, const T* K, const T* V, co
 // (kStatusWaitTimeout, kSelfTestSite) in the status slot and the kernel
 // returns normally.
 constexpr int kSelfTestSite = 99;
-__global__ void wait_selftest_kernel(KernelStatus* status, uint64_t timeout_ns) {
+static __global__ void wait_selftest_kernel(KernelStatus* status, uint64_t timeout_ns) {
   __shared__ uint64_t bar;
   __shared__ int abort_flag;
   if (threadIdx.x == 0) {

@@ -107,7 +107,7 @@ __device__ __forceinline__ void note_failure(const WaitCtx& ctx, int where) {
 // points at pinned, device-mapped host memory (or a device array), read by
 // the host after the stream finishes; the first failing CTA's record wins
 // (concurrent writers may interleave; any one record is enough).
-__device__ __noinline__ void publish_failure(int abort_value, KernelStatus* status) {
+static __device__ __noinline__ void publish_failure(int abort_value, KernelStatus* status) {
   if (abort_value == 0) return;
   volatile KernelStatus* st = status;
   if (st->code == 0) {

@@ -24,7 +24,10 @@ sm_100 GPU, calls raise.
 from __future__ import annotations
 
 import ctypes
+import functools
+import math
 import os
+import struct
 
 import torch
 
@@ -47,6 +50,14 @@ LSE_NAMES = {
     torch.bfloat16: "fmha_bwd_full_lse",
     torch.float16: "fmha_bwd_full_fp16_lse",
 }
+
+# attention entries: forward and backward against an encoder's states, and
+# attention behind a shared prefix (argument block fmha_attn_t)
+ATTN_NAMES = {
+    torch.bfloat16: ("fmha_cross_fwd", "fmha_cross_bwd", "fmha_prefix_attn"),
+    torch.float16: ("fmha_cross_fp16_fwd", "fmha_cross_fp16_bwd", "fmha_prefix_fp16_attn"),
+}
+_CROSS_FWD, _CROSS_BWD, _PREFIX = range(3)
 
 ERROR_NAMES = {
     0: "OK",
@@ -101,6 +112,11 @@ def load_library(dtype: torch.dtype = torch.bfloat16) -> ctypes.CDLL:
     getattr(lib, lse).argtypes = (_PTR_ARGS + [ctypes.c_void_p] + _INT_ARGS +
                                   [ctypes.c_float, ctypes.c_void_p])
     getattr(lib, lse).restype = ctypes.c_int
+    for name in ATTN_NAMES[dtype]:
+        getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
+    lib.fmha_attn_workspace.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p]
+    lib.fmha_attn_workspace.restype = ctypes.c_int
     lib.fmha_bwd_last_error.argtypes = []
     lib.fmha_bwd_last_error.restype = ctypes.c_int
     lib.fmha_bwd_last_error_message.argtypes = []
@@ -229,6 +245,201 @@ def fmha_bwd_lse(Q, K, V, O, dO, LSE, scale: float, *, out=None, stream=None,
         if lib.fmha_bwd_poll_device_status() != 0:
             raise FmhaBwdError(6, "fmha_bwd_lse: an in-kernel wait gave up")
     return dQ, dK, dV
+
+
+# ------------------------------------------------- attention: encoder states
+# fmha_attn_t of include/fmha_bwd.h: ten tensors (pointer, batch, head and row
+# stride), LSE, kv_lens, prefix_lens, workspace, its bytes, eight sizes, scale.
+_ATTN = struct.Struct("=40q5q8ifi")
+_NO_TENSOR = (0, 0, 0, 0)
+
+
+def _tensor_arg(t):
+    sb, sh, sr, _ = t.stride()
+    return t.data_ptr(), sb, sh, sr
+
+
+def _check_attn_tensor(name, t, like, shape):
+    if not t.is_cuda or t.device != like.device:
+        raise ValueError(f"{name} must be a CUDA tensor on {like.device}")
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {like.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.stride(3) != 1:
+        raise ValueError(f"{name} must have unit stride along its last axis")
+
+
+def _check_lens(name, t, like, count):
+    if t is None:
+        return 0
+    if not t.is_cuda or t.device != like.device or t.dtype != torch.int32 or not t.is_contiguous() \
+            or t.shape != (count,):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {count} elements on {like.device}")
+    return t.data_ptr()
+
+
+def _check_lse(LSE, Q):
+    if not LSE.is_cuda or LSE.device != Q.device or LSE.dtype != torch.float32 or not LSE.is_contiguous() \
+            or LSE.shape != Q.shape[:3]:
+        raise ValueError(f"LSE must be a contiguous fp32 tensor of shape {tuple(Q.shape[:3])} on {Q.device}")
+
+
+def _check_qkv(Q, K, V, names=("K", "V")):
+    for name, t in zip(("Q", *names), (Q, K, V)):
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [batch, heads, rows, d]")
+    library_path(Q.dtype)  # refuses other dtypes
+    B, Hq, _, d = Q.shape
+    if K.shape[1] == 0 or Hq % K.shape[1] != 0:
+        raise ValueError(f"{Hq} query heads do not divide among {K.shape[1]} kv heads")
+    _check_attn_tensor("Q", Q, Q, Q.shape)
+    _check_attn_tensor(names[0], K, Q, (K.shape[0], K.shape[1], K.shape[2], d))
+    _check_attn_tensor(names[1], V, Q, K.shape)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_workspace_bytes(dtype, op, sizes):
+    lib = load_library(dtype)
+    need = ctypes.c_uint64()
+    rc = lib.fmha_attn_workspace(_ATTN.pack(*_NO_TENSOR * 10, 0, 0, 0, 0, 0, *sizes, 1.0, 0), op, ctypes.byref(need))
+    _raise_if_error(lib, rc)
+    return need.value
+
+
+def _run_attn(op, Q, tensors, make_out, out, LSE, kv_lens, prefix_lens, sizes, scale, stream, sync):
+    """One call of an attention entry on `stream`. `tensors` are the ten of
+    fmha_attn_t, with ... in the place of each output (an LSE that is one comes
+    last among them) and None for those that the entry does not take; outputs and workspace come from torch's allocator,
+    for the stream that the call runs on."""
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, not {scale}")
+    dev = Q.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _run_attn(op, Q, tensors, make_out, out, LSE, kv_lens, prefix_lens, sizes, scale, stream, sync)
+    current = torch.cuda.current_stream()
+    if stream is not None and stream != current:
+        if stream.device != dev:
+            raise ValueError(f"stream is on {stream.device}, the tensors on {dev}")
+        with torch.cuda.stream(stream):
+            res = _run_attn(op, Q, tensors, make_out, out, LSE, kv_lens, prefix_lens, sizes, scale, None, sync)
+        # memory used on a stream other than the one it was allocated for
+        for t in (*tensors, LSE, kv_lens, prefix_lens):
+            if isinstance(t, torch.Tensor):
+                t.record_stream(stream)
+        for t in res:
+            t.record_stream(stream if out is not None else current)
+        return res
+    res = make_out() if out is None else out
+    need = _attn_workspace_bytes(Q.dtype, op, sizes)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    made = iter(res)
+    args = []
+    for t in tensors:
+        args += _NO_TENSOR if t is None else _tensor_arg(next(made) if t is Ellipsis else t)
+    if LSE is Ellipsis:
+        LSE = next(made)
+    lib = load_library(Q.dtype)
+    rc = getattr(lib, ATTN_NAMES[Q.dtype][op])(
+        _ATTN.pack(*args, LSE.data_ptr(), 0 if kv_lens is None else kv_lens.data_ptr(),
+                   0 if prefix_lens is None else prefix_lens.data_ptr(), ws.data_ptr() if need else 0, need, *sizes,
+                   scale, 0), current.cuda_stream)
+    _raise_if_error(lib, rc)
+    if sync:
+        current.synchronize()
+        if lib.fmha_bwd_poll_device_status() != 0:
+            raise FmhaBwdError(6, f"{ATTN_NAMES[Q.dtype][op]}: an in-kernel wait gave up")
+    return tuple(res)
+
+
+def cross_attn_fwd(Q, K, V, kv_lens=None, scale=None, *, out=None, stream=None, sync: bool = True):
+    """Attention to an encoder's states of another length: returns (O, LSE)
+    with O = softmax(scale Q K^T) V over each batch entry's valid keys and LSE
+    the fp32 row log-sum-exp that fmha_bwd_lse and cross_attn_bwd take.
+
+    Q: [B, Hq, M, d]; K, V: [B, Hkv, N, d], Hq a multiple of Hkv (query head h
+    reads kv head h // (Hq // Hkv)). Any strides that are multiples of 8
+    elements with unit stride along d, so the transposed views of [B, rows, H,
+    d] projections need no copy. ``kv_lens``: int32 [B] on the device, the
+    valid rows of K and V (None: all); what lies behind them is never used. A
+    row without valid keys gets O = 0 and LSE = -inf. ``scale`` defaults to
+    1/sqrt(d). M = 1 is the form for single tokens: each K and V is then read
+    once, by as many SMs as it takes.
+
+    ``out`` may supply (O, LSE). Runs on ``stream`` (default: torch's current
+    stream); with ``sync`` the call waits and raises on an in-kernel wait
+    timeout. With sync=False it can be captured into a CUDA graph."""
+    _check_qkv(Q, K, V)
+    B, Hq, M, d = Q.shape
+    if K.shape[0] != B:
+        raise ValueError(f"K has batch {K.shape[0]}, expected {B}")
+    _check_lens("kv_lens", kv_lens, Q, B)
+    if out is not None:
+        _check_attn_tensor("O", out[0], Q, Q.shape)
+        _check_lse(out[1], Q)
+    return _run_attn(
+        _CROSS_FWD, Q, (Q, ..., K, V, None, None, None, None, None, None),
+        lambda: (torch.empty_like(Q), torch.empty(B, Hq, M, dtype=torch.float32, device=Q.device)), out, ..., kv_lens, None,
+        (B, Hq, K.shape[1], M, K.shape[2], d, 0, 0), d ** -0.5 if scale is None else float(scale), stream, sync)
+
+
+def cross_attn_bwd(Q, K, V, O, LSE, dO, kv_lens=None, scale=None, *, out=None, stream=None, sync: bool = True):
+    """Backward of cross_attn_fwd: returns (dQ, dK, dV) from the forward's O
+    and LSE and from dO, with the same kv_lens and scale. dK and dV sum over
+    the query heads of their kv head and are zero at and past kv_lens. There
+    are no atomics: two calls give the same bits. ``out`` may supply (dQ, dK,
+    dV), which are fully overwritten; ``stream`` and ``sync`` as there."""
+    _check_qkv(Q, K, V)
+    B, Hq, M, d = Q.shape
+    if K.shape[0] != B:
+        raise ValueError(f"K has batch {K.shape[0]}, expected {B}")
+    _check_attn_tensor("O", O, Q, Q.shape)
+    _check_attn_tensor("dO", dO, Q, Q.shape)
+    _check_lse(LSE, Q)
+    _check_lens("kv_lens", kv_lens, Q, B)
+    if out is not None:
+        for name, t, like in zip(("dQ", "dK", "dV"), out, (Q, K, V)):
+            _check_attn_tensor(name, t, Q, like.shape)
+    return _run_attn(
+        _CROSS_BWD, Q, (Q, O, K, V, dO, ..., ..., ..., None, None),
+        lambda: (torch.empty_like(Q), torch.empty_like(K), torch.empty_like(V)), out, LSE, kv_lens, None,
+        (B, Hq, K.shape[1], M, K.shape[2], d, 0, 0), d ** -0.5 if scale is None else float(scale), stream, sync)
+
+
+def prefix_attn(Q, Kp, Vp, K, V, prefix_lens=None, kv_lens=None, scale=None, *, out=None, stream=None,
+                sync: bool = True):
+    """Attention of the newest tokens of a batch whose entries share long
+    prefixes: returns (O, LSE) as cross_attn_fwd does.
+
+    Q: [B, Hq, M, d], the M newest tokens of each entry (M = 1 when decoding,
+    more when several drafted tokens are checked at once). Kp, Vp: [P, Hkv,
+    Np, d], shared by B / P consecutive entries each (entry b reads prefix
+    b // (B // P)), of which prefix_lens[p] rows count. K, V: [B, Hkv, N, d],
+    each entry's own cache behind the prefix, of which kv_lens[b] rows count,
+    the M newest tokens' own rows last: row m sees all but the M - 1 - m
+    newest. The softmax runs over both. The prefix is read once for all of
+    its entries. Strides, ``out``, ``stream`` and ``sync`` as cross_attn_fwd."""
+    _check_qkv(Q, K, V)
+    _check_qkv(Q, Kp, Vp, ("Kp", "Vp"))
+    B, Hq, M, d = Q.shape
+    P, Hkv = Kp.shape[:2]
+    if K.shape[0] != B or K.shape[1] != Hkv:
+        raise ValueError(f"K has batch and heads {tuple(K.shape[:2])}, expected {(B, Hkv)}")
+    if P == 0 or B % P != 0:
+        raise ValueError(f"{B} batch entries do not divide among {P} prefixes")
+    _check_lens("prefix_lens", prefix_lens, Q, P)
+    _check_lens("kv_lens", kv_lens, Q, B)
+    if out is not None:
+        _check_attn_tensor("O", out[0], Q, Q.shape)
+        _check_lse(out[1], Q)
+    return _run_attn(
+        _PREFIX, Q, (Q, ..., K, V, None, None, None, None, Kp, Vp),
+        lambda: (torch.empty_like(Q), torch.empty(B, Hq, M, dtype=torch.float32, device=Q.device)), out, ..., kv_lens,
+        prefix_lens, (B, Hq, Hkv, M, K.shape[2], d, P, Kp.shape[2]), d ** -0.5 if scale is None else float(scale),
+        stream, sync)
 
 
 # ---------------------------------------------------------------- stage hooks

@@ -49,6 +49,41 @@ enum {
   FMHA_BWD_ERR_NO_DRIVER = 7
 };
 
+/* One 16-bit tensor [batch][heads][rows][K_dim]: consecutive along K_dim,
+ * strides of the other axes in elements (multiples of 8; the stride of an
+ * axis of size 1 is not looked at). ptr is 16-byte aligned device memory. */
+typedef struct {
+  void* ptr;
+  int64_t batch, head, row;
+} fmha_tensor_t;
+
+/* Arguments of the attention entries fmha_cross_fwd, fmha_cross_bwd and
+ * fmha_prefix_attn (and their fp16 twins). Set unused members to zero.
+ *
+ * q_heads is a multiple of kv_heads; query head h reads kv head
+ * h / (q_heads / kv_heads). Lengths live on the device and are clamped to
+ * [0, rows]; a null length array means that every row counts. What K and V
+ * hold at or past a length is never used, NaN and infinities included. */
+typedef struct {
+  fmha_tensor_t Q, O;           /* [batch][q_heads][M][K_dim] */
+  fmha_tensor_t K, V;           /* [batch][kv_heads][N][K_dim] */
+  fmha_tensor_t dO, dQ;         /* backward: as Q */
+  fmha_tensor_t dK, dV;         /* backward: as K */
+  fmha_tensor_t Kp, Vp;         /* prefix: [prefixes][kv_heads][N_prefix][K_dim] */
+  float* LSE;                   /* [batch][q_heads][M], contiguous */
+  const int* kv_lens;           /* [batch]: valid rows of K and V, or null */
+  const int* prefix_lens;       /* [prefixes], or null */
+  void* workspace;              /* 16-byte aligned device memory of the call, */
+  uint64_t workspace_bytes;     /* at least fmha_attn_workspace() bytes */
+  int batch, q_heads, kv_heads, M, N, K_dim;
+  int prefixes, N_prefix;       /* prefix: batch is a multiple of prefixes */
+  float softmax_scale;          /* positive, finite */
+  int reserved;
+} fmha_attn_t;
+
+/* Operations of fmha_attn_workspace. */
+enum { FMHA_ATTN_CROSS_FWD = 0, FMHA_ATTN_CROSS_BWD = 1, FMHA_ATTN_PREFIX = 2 };
+
 /* ---- libfmha_bwd_bf16.so ------------------------------------------------ */
 
 /* Replaces fmha_bwd_full_py, src/fmha_bwd_kernels.hip:474-477 (bf16).
@@ -133,6 +168,30 @@ int fmha_bwd_full_noalloc(fmha_bf16_t* dQ, fmha_bf16_t* dK, fmha_bf16_t* dV,
                           const fmha_bf16_t* dO, int M, int N, int K_dim,
                           int total_heads, fmha_stream_t stream);
 
+/* Attention of M query rows to an encoder's states of N rows, of which batch
+ * entry b has kv_lens[b]. With S = softmax_scale Q K^T over the valid keys:
+ *   LSE = log sum_n exp(S),   O = sum_n exp(S - LSE) V.
+ * A row without valid keys gets O = 0 and LSE = -inf. M = 1 is the form for
+ * single tokens. No counterpart in the reference, which starts from P.
+ * Stream-ordered; allocates nothing; returns 0 or an error code. */
+int fmha_cross_fwd(const fmha_attn_t* args, fmha_stream_t stream);
+
+/* Its backward, from O and LSE as the forward left them and dO:
+ *   P = exp(S - LSE), D = rowsum(dO * O), dS = P * (dO V^T - D),
+ *   dQ = softmax_scale dS K,  dK = softmax_scale sum dS^T Q,  dV = sum P^T dO
+ * (sums over the query heads of a kv head). dQ, dK and dV are fully
+ * overwritten; rows of dK and dV at or past kv_lens[b] are zero. No atomics:
+ * two calls give the same bits. */
+int fmha_cross_bwd(const fmha_attn_t* args, fmha_stream_t stream);
+
+/* Attention of the M newest tokens of each batch entry to a prefix that
+ * batch / prefixes consecutive entries share (entry b reads prefix
+ * b / (batch / prefixes), its first prefix_lens rows) and to the entry's own
+ * cache K, V behind it (its first kv_lens[b] rows, the M newest tokens
+ * last: row m reads kv_lens[b] - (M - 1 - m) of them), in one softmax. O and
+ * LSE as fmha_cross_fwd. The prefix is read once for all entries. */
+int fmha_prefix_attn(const fmha_attn_t* args, fmha_stream_t stream);
+
 /* Stage hooks (replace the reference's test_* wrappers,
  * src/fmha_bwd_kernels.hip:525-560). Each runs one stage of the backward as
  * its own launch with its 16-bit intermediate in global memory ([H][M][N]
@@ -204,6 +263,12 @@ int fmha_bwd_full_fp16_stream_events(fmha_fp16_t* dQ, fmha_fp16_t* dK,
                                      int M, int N, int K_dim, int total_heads,
                                      fmha_stream_t stream, void* const* events);
 
+/* fp16 attention entries, as fmha_cross_fwd, fmha_cross_bwd and
+ * fmha_prefix_attn. */
+int fmha_cross_fp16_fwd(const fmha_attn_t* args, fmha_stream_t stream);
+int fmha_cross_fp16_bwd(const fmha_attn_t* args, fmha_stream_t stream);
+int fmha_prefix_fp16_attn(const fmha_attn_t* args, fmha_stream_t stream);
+
 /* fp16 stage hooks, as the bf16 ones (src/fmha_bwd_kernels_fp16.hip:284-314,
  * where they have C++ linkage; here they are plain C symbols). */
 void test_dp_kernel_fp16(const fmha_fp16_t* dO, const fmha_fp16_t* V, fmha_fp16_t* dP,
@@ -251,6 +316,11 @@ int fmha_bwd_selftest_wait_timeout(int timeout_ms);
  * call without a partial-sum workspace (never split). Returns FMHA_BWD_OK,
  * or FMHA_BWD_ERR_INVALID_ARGUMENT for a null `out` or negative sizes. */
 int fmha_bwd_work_units(int items, int grid, int len, int allow, int* out);
+
+/* Bytes of workspace that an attention call with these sizes needs (its
+ * pointers are not looked at); 0 means that workspace may be null. `op` is
+ * one of FMHA_ATTN_*. Host-only. Returns FMHA_BWD_OK or an error code. */
+int fmha_attn_workspace(const fmha_attn_t* args, int op, uint64_t* bytes);
 
 /* Upper bound, in milliseconds, on any single in-kernel wait (default 4000,
  * or FMHA_BWD_WAIT_TIMEOUT_MS). A wait that runs out sets the device status
