@@ -1,5 +1,5 @@
 // The fp16 attention entries of libfmha_bwd_fp16.so (include/fmha_bwd.h).
-#include "fmha_attn_simple.cuh"
+#include "fmha_attn_launch.cuh"
 
 #define FMHA_API __attribute__((visibility("default")))
 

@@ -1,0 +1,621 @@
+// Forward of attention on the tensor cores: O and LSE of packed query rows
+// against the keys of one kv head, whole or split along the keys.
+//
+//   S = Q K^T,  p = 2^(S scale log2e - m),  O = sum p V / sum p,
+//   LSE = (m + log2 sum p) ln 2
+//
+// with a running m for each row, in one pass over the keys.
+//
+// Rows. A tile is up to 128 query rows that read the same keys: Mt
+// consecutive tokens of Gt query heads of the kv head's group of St batch
+// entries that share the keys (St > 1 for a shared prefix only), tokens
+// fastest. One tensor-map box of Q brings such a tile in, so a single token
+// of many heads or samples fills a tile just as 128 tokens of one head do.
+//
+// Two tiles per CTA. Each tile has its own softmax warpgroup (thread = row),
+// its own S (128 TMEM columns) and O accumulator (D columns); while one
+// warpgroup computes p of its tile, the tensor core works for the other. p is
+// written as 16-bit over the first 64 columns of S and read from there as the
+// A operand of O += p V. The tensor core runs PV_t(j) and the next S_t(j+1) in
+// the order of issue, so the completion of S_t(j+1) says that PV_t(j) has
+// completed as well: between that and its own signal the warpgroup owns O_t.
+//
+// m moves only when a row's maximum exceeds it by more than 2^8 (its O is then
+// scaled in TMEM by the softmax warpgroup, which owns it): p stays below 2^8
+// (2^14 with fp16's bias below), and most steps rescale nothing.
+//
+// p is rounded to 16 bits (the tensor core's input type) after it went into
+// the fp32 row sum. In fp16 m is lowered by kBias = 6, so that p down to 2^-20
+// of the row's maximum keeps full precision (bf16 has fp32's range).
+#pragma once
+
+#include "fmha_attn.cuh"
+#include "fmha_bwd_lse.cuh"  // ex2_approx, kLog2e
+
+namespace fmha_sm100 {
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+// How query rows fall into tiles (see above).
+struct RowPack {
+  int M, G, S;     // tokens, query heads of a kv head, batch entries that share keys
+  int Mt, Gt, St;  // the box
+  int nm, ng, ns;  // boxes along each
+  int tiles;       // nm * ng * ns
+  // token, head within the group and entry of row r of tile t; false if there is no such row
+  __device__ __forceinline__ bool row(int t, int r, int& m, int& g, int& s) const {
+    const int im = t % nm, u = t / nm;
+    int rm = r, rg = 0, rs = 0;
+    if (Mt < 128) {
+      rm = r % Mt;
+      const int v = r / Mt;
+      rg = v % Gt;
+      rs = v / Gt;
+    }
+    m = im * Mt + rm;
+    g = (u % ng) * Gt + rg;
+    s = (u / ng) * St + rs;
+    return m < M && rg < Gt && g < G && rs < St && s < S;
+  }
+};
+
+inline RowPack pack_rows(int M, int G, int S) {
+  RowPack p;
+  p.M = M;
+  p.G = G;
+  p.S = S;
+  p.Mt = M < 128 ? M : 128;
+  p.Gt = std::min(G, 128 / p.Mt);
+  p.St = std::min(S, 128 / (p.Mt * p.Gt));
+  p.nm = (M + p.Mt - 1) / p.Mt;
+  p.ng = (G + p.Gt - 1) / p.Gt;
+  p.ns = (S + p.St - 1) / p.St;
+  p.tiles = p.nm * p.ng * p.ns;
+  return p;
+}
+
+template <typename T>
+struct FwdParams {
+  RowPack rows;
+  int B, Hkv, N;      // key batches, kv heads, key rows
+  const int* lens;    // [B] or null
+  int splits;         // parts of the keys (1: O and LSE are final)
+  int pairs;          // tile pairs of one (batch, kv head)
+  int items;          // B * Hkv * splits * pairs
+  View<T> O;
+  float* LSE;         // [batch][q head][token]
+  float* part_o;      // splits > 1 or partial: [split][row][D], normalised
+  float* part_lse;    // [split][row]
+  bool partial;
+  float scale;
+  KernelStatus* status;
+  uint64_t timeout_ns;
+};
+
+template <int D>
+struct FwdCfg {
+  static constexpr int kTileBytes = (D / kBoxCols) * kBoxBytes;  // 128 rows
+  static constexpr int kSlots = D == 128 ? 5 : 8;                // K and V tiles, in the order of their use
+  static constexpr int kOffQ = 0;                                // two tiles
+  static constexpr int kOffKV = 2 * kTileBytes;
+  static constexpr int kOffStat = kOffKV + kSlots * kTileBytes;  // float2 [2][128]
+  static constexpr int kOffBar = kOffStat + 2 * 128 * 8;
+  static constexpr int kSmemBytes = kOffBar + 512;
+  static constexpr int kThreads = 512;
+  static constexpr uint32_t kColS = 0;    // + 128 * tile
+  static constexpr uint32_t kColO = 256;  // + D * tile
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+  // warpgroups 0 and 1 softmax, 2 epilogue, 3 loads and MMA: 2 * 128 * 184 +
+  // 2 * 128 * 72 registers, the 512 * 128 of the launch
+  static constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
+  static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs == 4 * 128, "register split");
+};
+
+enum FwdBar : int {
+  kFwQFull0 = 0,    // + tile
+  kFwQEmpty0 = 2,   // + tile: the item's last S of the tile is done
+  kFwKVFull0 = 4,   // + slot (up to 8)
+  kFwKVEmpty0 = 12, // + slot
+  kFwSFull0 = 20,   // + tile
+  kFwPFull0 = 22,   // + tile: p written (4 warps)
+  kFwOFull0 = 24,   // + tile: the item's last PV of the tile is done
+  kFwOEmpty0 = 26,  // + tile: the epilogue has read O (4 warps)
+  kFwStFull0 = 28,  // + tile: row maxima and sums written (4 warps)
+  kFwStEmpty0 = 30, // + tile: and read (4 warps)
+  kFwDrain = 32,
+  kNumFwdBars = 33,
+};
+static_assert(kNumFwdBars * 8 + 8 <= 512, "barrier area");
+
+// One item: a pair of row tiles of a (batch, kv head), a range of key tiles.
+struct FwdItem {
+  int b, hk, split, tile0, n;  // n: valid keys of the batch entry
+  int lo, hi;                  // key tiles
+  bool two;                    // the second tile exists
+};
+
+template <typename T>
+__device__ __forceinline__ FwdItem fwd_item(const FwdParams<T>& p, int t) {
+  FwdItem it;
+  const int pair = t % p.pairs;
+  int u = t / p.pairs;
+  it.split = u % p.splits;
+  u /= p.splits;
+  it.hk = u % p.Hkv;
+  it.b = u / p.Hkv;
+  it.tile0 = 2 * pair;
+  it.two = 2 * pair + 1 < p.rows.tiles;
+  it.n = valid_rows(p.lens, it.b, p.N);
+  const int nt = (it.n + kTile - 1) / kTile;
+  it.lo = static_cast<int>(static_cast<int64_t>(nt) * it.split / p.splits);
+  it.hi = static_cast<int>(static_cast<int64_t>(nt) * (it.split + 1) / p.splits);
+  return it;
+}
+
+// 16-byte chunks of 16-bit output rows held one row per lane, stored so that
+// each instruction writes whole row segments (the transpose of
+// store_rows_coalesced), each row at its own address; null rows are skipped.
+template <int S>
+__device__ __forceinline__ void store_rows_anywhere(uint4 (&c)[S], uint8_t* row, int lane) {
+#pragma unroll
+  for (int m = 1; m < S; m <<= 1) {
+    const bool hi = (lane & m) != 0;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      if (j & m) continue;
+      const uint4 snd = hi ? c[j] : c[j ^ m];
+      uint4 rcv;
+      rcv.x = __shfl_xor_sync(0xffffffffu, snd.x, m);
+      rcv.y = __shfl_xor_sync(0xffffffffu, snd.y, m);
+      rcv.z = __shfl_xor_sync(0xffffffffu, snd.z, m);
+      rcv.w = __shfl_xor_sync(0xffffffffu, snd.w, m);
+      if (hi) c[j] = rcv;
+      else c[j ^ m] = rcv;
+    }
+  }
+  const int g0 = lane & ~(S - 1), i = lane & (S - 1);
+#pragma unroll
+  for (int k = 0; k < S; ++k) {
+    uint8_t* at = reinterpret_cast<uint8_t*>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), g0 + k));
+    if (at) *reinterpret_cast<uint4*>(at + 16 * i) = c[k];
+  }
+}
+
+// 8 fp32 accumulators times `mul` as eight 16-bit values.
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const uint32_t* a, float mul) {
+  return make_uint4(Elem<T>::pack(mul * __uint_as_float(a[0]), mul * __uint_as_float(a[1])),
+                    Elem<T>::pack(mul * __uint_as_float(a[2]), mul * __uint_as_float(a[3])),
+                    Elem<T>::pack(mul * __uint_as_float(a[4]), mul * __uint_as_float(a[5])),
+                    Elem<T>::pack(mul * __uint_as_float(a[6]), mul * __uint_as_float(a[7])));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
+    attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_Q, const __grid_constant__ CUtensorMap tm_K,
+                    const __grid_constant__ CUtensorMap tm_V, const __grid_constant__ FwdParams<T> p) {
+  using Cfg = FwdCfg<D>;
+  constexpr int kSlots = Cfg::kSlots;
+  constexpr bool kB = Elem<T>::kBF16;
+  constexpr float kBias = kB ? 0.f : 6.f;
+  // aligned by declaration: the tiles leave no room to align by hand
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {  // never, short of a toolchain that drops the alignment
+    if (threadIdx.x == 0) publish_failure(1 + 200, p.status);
+    return;
+  }
+  float2* stat = reinterpret_cast<float2*>(smem + Cfg::kOffStat);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + kNumFwdBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bar[kFwQFull0 + t], 1);
+      mbar_init(&bar[kFwQEmpty0 + t], 1);
+      mbar_init(&bar[kFwSFull0 + t], 1);
+      mbar_init(&bar[kFwPFull0 + t], 4);
+      mbar_init(&bar[kFwOFull0 + t], 1);
+      mbar_init(&bar[kFwOEmpty0 + t], 4);
+      mbar_init(&bar[kFwStFull0 + t], 4);
+      mbar_init(&bar[kFwStEmpty0 + t], 4);
+    }
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&bar[kFwKVFull0 + s], 1);
+      mbar_init(&bar[kFwKVEmpty0 + s], 1);
+    }
+    mbar_init(&bar[kFwDrain], 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 13) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  WaitCtx ctx{abort_flag, p.timeout_ns};
+  const int first = blockIdx.x, step = gridDim.x;
+
+  if (warp >= 12) {
+    regs_lower<Cfg::kOtherRegs>();
+    if (warp == 12 && lane == 0) {
+      // ---- TMA producer. Ring order: K_lo, then V_j, K_(j+1) in turn, the
+      // order in which the MMA thread uses them.
+      tma_prefetch_desc(&tm_Q);
+      tma_prefetch_desc(&tm_K);
+      tma_prefetch_desc(&tm_V);
+      const uint64_t pol_q = l2_policy_evict_first(), pol_kv = l2_policy_evict_last();
+      const uint32_t q_bytes = static_cast<uint32_t>(p.rows.Mt * p.rows.Gt * p.rows.St) * 128u * (D / kBoxCols);
+      int nq[2] = {0, 0}, g = 0, slot = 0, turn = 0;
+      bool ok = true;
+      auto load_q = [&](const FwdItem& it, int t) {
+        if (nq[t] > 0 && !mbar_wait(&bar[kFwQEmpty0 + t], (nq[t] - 1) & 1, ctx, 201)) return false;
+        const int tile = it.tile0 + t;
+        const int im = tile % p.rows.nm, u = tile / p.rows.nm;
+        mbar_arrive_expect_tx(&bar[kFwQFull0 + t], q_bytes);
+#pragma unroll
+        for (int x = 0; x < D / kBoxCols; ++x)
+          tma_load_4d(smem + Cfg::kOffQ + t * Cfg::kTileBytes + x * kBoxBytes, &tm_Q, &bar[kFwQFull0 + t], x * kBoxCols,
+                      im * p.rows.Mt, it.hk * p.rows.G + (u % p.rows.ng) * p.rows.Gt,
+                      it.b * p.rows.S + (u / p.rows.ng) * p.rows.St, pol_q);
+        ++nq[t];
+        return true;
+      };
+      auto load_kv = [&](const CUtensorMap* tm, const FwdItem& it, int j) {
+        if (g >= kSlots && !mbar_wait(&bar[kFwKVEmpty0 + slot], (turn - 1) & 1, ctx, 202)) return false;
+        uint64_t* fb = &bar[kFwKVFull0 + slot];
+        uint8_t* dst = smem + Cfg::kOffKV + slot * Cfg::kTileBytes;
+        mbar_arrive_expect_tx(fb, Cfg::kTileBytes);
+#pragma unroll
+        for (int x = 0; x < D / kBoxCols; ++x)
+          tma_load_4d(dst + x * kBoxBytes, tm, fb, x * kBoxCols, j * kTile, it.hk, it.b, pol_kv);
+        ++g;
+        if (++slot == kSlots) {
+          slot = 0;
+          ++turn;
+        }
+        return true;
+      };
+      for (int t = first; t < p.items && ok; t += step) {
+        const FwdItem it = fwd_item(p, t);
+        if (it.lo == it.hi) continue;
+        ok = load_q(it, 0) && load_kv(&tm_K, it, it.lo) && (!it.two || load_q(it, 1));
+        for (int j = it.lo; j < it.hi && ok; ++j)
+          ok = load_kv(&tm_V, it, j) && (j + 1 == it.hi || load_kv(&tm_K, it, j + 1));
+      }
+      if (*abort_flag) {
+        for (int t = 0; t < 2; ++t)
+          if (nq[t] > 0) mbar_wait_drain(&bar[kFwQFull0 + t], (nq[t] - 1) & 1, p.timeout_ns);
+        for (int i = (g > kSlots ? g - kSlots : 0); i < g; ++i)
+          mbar_wait_drain(&bar[kFwKVFull0 + i % kSlots], (i / kSlots) & 1, p.timeout_ns);
+      }
+    } else if (warp == 13) {
+      // ---- MMA: lane 0 issues; the whole warp clears the V rows between the
+      // last valid key and the next multiple of 16 (the products' step), which
+      // the tensor core would multiply by p = 0 whatever they hold.
+      constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
+      constexpr uint32_t id_O = make_idesc_f16<kB>(kTile, D, false, true);
+      const uint32_t sQ = smem_u32(smem + Cfg::kOffQ), sKV = smem_u32(smem + Cfg::kOffKV);
+      // the walk over all (item, key tile) steps of this CTA
+      struct Walk {
+        int t, j;
+        FwdItem it;
+      };
+      auto seek = [&](Walk& w) {  // first step of the next item that has one
+        for (; w.t < p.items; w.t += step) {
+          w.it = fwd_item(p, w.t);
+          if (w.it.lo < w.it.hi) {
+            w.j = w.it.lo;
+            return true;
+          }
+        }
+        return false;
+      };
+      Walk cur{first, 0, {}};
+      bool more = seek(cur), ok = true;
+      int g = 0, nq[2] = {0, 0}, np[2] = {0, 0}, no[2] = {0, 0};
+      auto issue_s = [&](int t, int slot) {
+        const uint64_t dq = make_sw128_desc(sQ + t * Cfg::kTileBytes, 16, 1024);
+        const uint64_t dk = make_sw128_desc(sKV + slot * Cfg::kTileBytes, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * kBoxBytes + (k & 3) * 32;
+          umma_f16_ss(tmem + Cfg::kColS + 128 * t, desc_advance(dq, off), desc_advance(dk, off), id_S, k > 0 ? 1u : 0u);
+        }
+        umma_commit(&bar[kFwSFull0 + t]);
+      };
+      // S of step w, for each of its tiles in `which`
+      auto first_s = [&](const Walk& w, int t, int slot) {
+        if (w.j == w.it.lo) {
+          if (!mbar_wait(&bar[kFwQFull0 + t], nq[t] & 1, ctx, 211)) return false;
+          ++nq[t];
+        }
+        tc_fence_after();
+        issue_s(t, slot);
+        if (w.j + 1 == w.it.hi) umma_commit(&bar[kFwQEmpty0 + t]);
+        return true;
+      };
+      if (more && lane == 0) {
+        ok = mbar_wait(&bar[kFwKVFull0], 0, ctx, 210) && first_s(cur, 0, 0) && (!cur.it.two || first_s(cur, 1, 0));
+        if (ok) umma_commit(&bar[kFwKVEmpty0]);
+      }
+      g = 1;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      while (more && ok) {
+        Walk nxt = cur;
+        bool has_next = true;
+        if (++nxt.j == nxt.it.hi) {
+          nxt.t += step;
+          has_next = seek(nxt);
+        }
+        const int vslot = g % kSlots, vpar = (g / kSlots) & 1;
+        const int kslot = (g + 1) % kSlots, kpar = ((g + 1) / kSlots) & 1;
+        g += 2;
+        const int left = cur.it.n - cur.j * kTile;  // valid keys from this tile on
+        if (lane == 0) ok = mbar_wait(&bar[kFwKVFull0 + vslot], vpar, ctx, 212);
+        if (left < kTile && (left & 15) != 0) {
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (ok) {
+            uint8_t* v = smem + Cfg::kOffKV + vslot * Cfg::kTileBytes;
+            const int rows = 16 - (left & 15);
+            for (int i = lane; i < rows * (D / 8); i += 32) {
+              const int row = left + i / (D / 8), c = i % (D / 8);
+              *reinterpret_cast<uint4*>(v + (c >> 3) * kBoxBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+                  make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+        }
+        if (lane == 0 && ok) {
+          const int steps = left >= kTile ? kTile / 16 : (left + 15) / 16;
+          const uint64_t dv = make_sw128_desc(sKV + vslot * Cfg::kTileBytes, kBoxBytes, 1024);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (ok && (t == 0 || cur.it.two)) {
+              if (cur.j == cur.it.lo) {
+                if (no[t] > 0) ok = mbar_wait(&bar[kFwOEmpty0 + t], (no[t] - 1) & 1, ctx, 213);
+                ++no[t];
+              }
+              if (ok) ok = mbar_wait(&bar[kFwPFull0 + t], np[t] & 1, ctx, 214);
+              ++np[t];
+              if (ok) {
+                tc_fence_after();
+                const uint32_t tP = tmem + Cfg::kColS + 128 * t, tO = tmem + Cfg::kColO + D * t;
+                const uint32_t keep = cur.j > cur.it.lo ? 1u : 0u;
+                if (steps == kTile / 16) {
+#pragma unroll
+                  for (int k = 0; k < kTile / 16; ++k)
+                    umma_f16_ts(tO, tP + k * 8, desc_advance(dv, k * 2048), id_O, k > 0 ? 1u : keep);
+                } else {
+                  for (int k = 0; k < steps; ++k)
+                    umma_f16_ts(tO, tP + k * 8, desc_advance(dv, k * 2048), id_O, k > 0 ? 1u : keep);
+                }
+                if (cur.j + 1 == cur.it.hi) umma_commit(&bar[kFwOFull0 + t]);
+              }
+            }
+            if (ok && t == (cur.it.two ? 1 : 0)) umma_commit(&bar[kFwKVEmpty0 + vslot]);
+            if (ok && has_next && (t == 0 || nxt.it.two)) {
+              if (t == 0) ok = mbar_wait(&bar[kFwKVFull0 + kslot], kpar, ctx, 215);
+              if (ok) ok = first_s(nxt, t, kslot);
+              if (ok && t == (nxt.it.two ? 1 : 0)) umma_commit(&bar[kFwKVEmpty0 + kslot]);
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        more = has_next;
+        cur = nxt;
+      }
+      if (!ok && lane == 0) {
+        umma_commit(&bar[kFwDrain]);
+        mbar_wait_drain(&bar[kFwDrain], 0, p.timeout_ns);
+      }
+      __syncwarp();
+    }
+  } else if (warp < 8) {
+    // ---- softmax: warpgroup t owns tile t, thread = row (TMEM lane)
+    regs_raise<Cfg::kSoftmaxRegs>();
+    const int t = warp >> 2;
+    const int r = threadIdx.x & 127;
+    const uint32_t tS = tmem + Cfg::kColS + 128 * t + (static_cast<uint32_t>(r & 96) << 16);
+    const uint32_t tO = tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16);
+    const float sl2 = p.scale * kLog2e;
+    int ns = 0, nst = 0;
+    bool ok = true;
+    for (int i = first; i < p.items && ok; i += step) {
+      const FwdItem it = fwd_item(p, i);
+      if (t == 1 && !it.two) continue;
+      float m = 0.f;                                  // the row's reference, in powers of two
+      float2 l0 = make_float2(0.f, 0.f), l1 = l0;     // its sum, in four shares
+      for (int j = it.lo; j < it.hi; ++j, ++ns) {
+        if (!mbar_wait(&bar[kFwSFull0 + t], ns & 1, ctx, 220)) { ok = false; break; }
+        __syncwarp();
+        tc_fence_after();
+        uint32_t s[128];
+        tmem_load_64(tS, *reinterpret_cast<uint32_t(*)[64]>(s));
+        tmem_load_64(tS + 64, *reinterpret_cast<uint32_t(*)[64]>(s + 64));
+        const int left = it.n - j * kTile;
+        if (left < kTile) {
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (x >= left) s[x] = 0xff800000u;  // -inf
+        }
+        float mx[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) mx[x] = __uint_as_float(s[x]);
+#pragma unroll
+        for (int x = 4; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2 - kBias;
+        if (j == it.lo) {
+          m = top == -INFINITY ? 0.f : top;
+        } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
+          const bool move = top > m + 8.f;
+          const float f = move ? ex2_approx(m - top) : 1.f;
+          if (move) m = top;
+          l0 = mul_f32x2(l0, make_float2(f, f));
+          l1 = mul_f32x2(l1, make_float2(f, f));
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            uint32_t o[32];
+            tmem_load_32(tO + 32 * x, o);
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(f * __uint_as_float(o[y]));
+            tmem_store_32(tO + 32 * x, o);
+          }
+          tmem_store_wait();
+        }
+        const float2 nm = make_float2(-m, -m), sc = make_float2(sl2, sl2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t e[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const uint32_t* v = s + 64 * h + 2 * x;
+            float2 a = fma_f32x2(make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), sc, nm);
+            a.x = ex2_approx(a.x);
+            a.y = ex2_approx(a.y);
+            if (x & 1) l1 = add_f32x2(l1, a);
+            else l0 = add_f32x2(l0, a);
+            e[x] = Elem<T>::pack(a.x, a.y);
+          }
+          tmem_store_32(tS + 32 * h, e);
+        }
+        tmem_store_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar[kFwPFull0 + t]);
+      }
+      if (!ok) break;
+      if (nst > 0 && !mbar_wait(&bar[kFwStEmpty0 + t], (nst - 1) & 1, ctx, 221)) { ok = false; break; }
+      stat[128 * t + r] = make_float2(m, (l0.x + l0.y) + (l1.x + l1.y));
+      ++nst;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar[kFwStFull0 + t]);
+    }
+  } else {
+    // ---- epilogue: thread = row of each tile in turn
+    regs_lower<Cfg::kOtherRegs>();
+    const int r = threadIdx.x & 127;
+    int nst[2] = {0, 0}, no[2] = {0, 0};
+    bool ok = true;
+    const int64_t all_rows = static_cast<int64_t>(p.B) * p.rows.S * p.Hkv * p.rows.G * p.rows.M;
+    for (int i = first; i < p.items && ok; i += step) {
+      const FwdItem it = fwd_item(p, i);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (t == 1 && !it.two) continue;
+        if (!mbar_wait(&bar[kFwStFull0 + t], nst[t] & 1, ctx, 230)) { ok = false; break; }
+        ++nst[t];
+        const float2 ml = stat[128 * t + r];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar[kFwStEmpty0 + t]);
+        const bool keys = it.lo < it.hi;
+        if (keys) {
+          if (!mbar_wait(&bar[kFwOFull0 + t], no[t] & 1, ctx, 231)) { ok = false; break; }
+          ++no[t];
+        }
+        __syncwarp();
+        tc_fence_after();
+        int m, g, s;
+        const bool real = p.rows.row(it.tile0 + t, r, m, g, s);
+        const int b = it.b * p.rows.S + s, h = it.hk * p.rows.G + g;
+        // a sum of 0 has no keys behind it, or scores of -inf alone
+        const float inv = keys && ml.y != 0.f ? 1.f / ml.y : 0.f;
+        const float lse = keys ? (ml.x + log2f(ml.y)) * kLn2 : -INFINITY;
+        const int64_t row = (static_cast<int64_t>(b) * p.Hkv * p.rows.G + h) * p.rows.M + m;
+        const uint32_t tO = tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16);
+        if (p.partial) {
+          if (real) p.part_lse[it.split * all_rows + row] = lse;
+          float* out = p.part_o + (it.split * all_rows + row) * D;
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            uint32_t o[32];
+            __syncwarp();
+            if (keys) {
+              tmem_load_32(tO + 32 * x, o);
+            } else {
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = 0u;
+            }
+            if (real) {
+#pragma unroll
+              for (int y = 0; y < 8; ++y)
+                reinterpret_cast<float4*>(out + 32 * x)[y] =
+                    make_float4(inv * __uint_as_float(o[4 * y]), inv * __uint_as_float(o[4 * y + 1]),
+                                inv * __uint_as_float(o[4 * y + 2]), inv * __uint_as_float(o[4 * y + 3]));
+            }
+          }
+        } else {
+          if (real) p.LSE[row] = lse;
+          uint8_t* out = real ? reinterpret_cast<uint8_t*>(p.O.at(b, h, m)) : nullptr;
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            uint32_t o[32];
+            __syncwarp();
+            if (keys) {
+              tmem_load_32(tO + 32 * x, o);
+            } else {
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = 0u;
+            }
+            uint4 ch[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) ch[y] = pack8<T>(o + 8 * y, inv);
+            store_rows_anywhere<4>(ch, out ? out + 64 * x : nullptr, lane);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (keys && lane == 0) mbar_arrive(&bar[kFwOEmpty0 + t]);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0) publish_failure(*abort_flag, p.status);
+  if (warp == 13) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of split keys: with weights w_i = exp(LSE_i - max LSE),
+// O = sum w_i O_i / sum w_i and LSE = max LSE + log sum w_i, parts in order.
+// One thread per 4 columns.
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+    attn_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, int parts, int64_t rows,
+                     View<T> O, float* __restrict__ LSE, int Hq, int M) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = i / (D / 4);
+  const int c = static_cast<int>(i % (D / 4));
+  if (row >= rows) return;
+  float top = -INFINITY;
+  for (int k = 0; k < parts; ++k) top = fmaxf(top, part_lse[k * rows + row]);
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (top > -INFINITY) {
+    for (int k = 0; k < parts; ++k) {
+      const float w = ex2_approx((part_lse[k * rows + row] - top) * kLog2e);
+      const float4 o = reinterpret_cast<const float4*>(part_o + (k * rows + row) * D)[c];
+      sum += w;
+      acc.x = fmaf(w, o.x, acc.x);
+      acc.y = fmaf(w, o.y, acc.y);
+      acc.z = fmaf(w, o.z, acc.z);
+      acc.w = fmaf(w, o.w, acc.w);
+    }
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const int m = static_cast<int>(row % M), h = static_cast<int>(row / M % Hq), b = static_cast<int>(row / M / Hq);
+  const uint2 v = make_uint2(Elem<T>::pack(inv * acc.x, inv * acc.y), Elem<T>::pack(inv * acc.z, inv * acc.w));
+  *reinterpret_cast<uint2*>(O.at(b, h, m) + 4 * c) = v;
+  if (c == 0) LSE[row] = sum > 0.f ? top + logf(sum) : -INFINITY;
+}
+
+}  // namespace fmha_sm100

@@ -1,0 +1,160 @@
+// Host side of the attention entries: workspace, tensor maps and launches.
+#pragma once
+
+#include "fmha_attn_fwd.cuh"
+#include "fmha_attn_simple.cuh"
+
+namespace fmha_sm100 {
+
+// 4-D map over a strided [batch][heads][rows][D] tensor: boxes of 64 columns,
+// 128-byte swizzle, zero fill out of bounds.
+inline bool encode_map4(CUtensorMap* map, bool bf16, const fmha_tensor_t& t, int D, int rows, int heads, int batch,
+                        int box_rows, int box_heads, int box_batch) {
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(batch)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.row) * 2, static_cast<cuuint64_t>(t.head) * 2,
+                                 static_cast<cuuint64_t>(t.batch) * 2};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(kBoxCols), static_cast<cuuint32_t>(box_rows),
+                             static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_batch)};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  return encode_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.ptr, dims,
+                     strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The status slot of `device`. Its allocation on the first call is allowed
+// while a stream of this thread is being captured.
+inline KernelStatus* attn_status(int device) {
+  std::lock_guard<std::mutex> g(ws_mutex());
+  DeviceWorkspace& w = ws_map()[device];
+  if (!w.host_status) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const bool ok = ensure_status_slot(device, w);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) return nullptr;
+  }
+  return w.host_status_dev;
+}
+
+// Sets a kernel's shared-memory limit, once for each device.
+template <auto kKernel>
+void allow_smem(int bytes, int device) {
+  static std::atomic<bool> done[64];
+  if (device < 64 && done[device].load()) return;
+  cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (device < 64) done[device].store(true);
+}
+
+// How a forward over `B` key batches divides its work.
+struct FwdPlan {
+  RowPack rows;
+  int pairs, splits, items;
+  int64_t all_rows;
+  uint64_t ws_bytes;
+};
+
+// Parts of the keys: with fewer items than SMs, as many parts as still leave
+// each two key tiles, so that the loads of one item spread over idle SMs.
+inline FwdPlan plan_fwd(int M, int G, int S, int B, int Hkv, int N, int D, int sms, bool partial) {
+  FwdPlan f;
+  f.rows = pack_rows(M, G, S);
+  f.pairs = (f.rows.tiles + 1) / 2;
+  const int64_t base = static_cast<int64_t>(f.pairs) * B * Hkv;
+  const int nt = (N + kTile - 1) / kTile;
+  f.splits = 1;
+  if (base < sms) f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / base, nt / 2)));
+  f.items = static_cast<int>(base * f.splits);
+  f.all_rows = static_cast<int64_t>(B) * S * Hkv * G * M;
+  f.ws_bytes = partial || f.splits > 1 ? static_cast<uint64_t>(f.splits) * f.all_rows * (D + 1) * 4 : 0;
+  return f;
+}
+
+template <typename T>
+int enqueue_fwd(const fmha_attn_t& a, const FwdPlan& f, const fmha_tensor_t& K, const fmha_tensor_t& V, int B, int N,
+                const int* lens, bool partial, int device, int sms, cudaStream_t stream) {
+  constexpr bool kBF16 = Elem<T>::kBF16;
+  if (!encode_fn()) return set_error(kErrNoDriver, "cuTensorMapEncodeTiled is unavailable");
+  KernelStatus* st = attn_status(device);
+  if (!st) return kErrOutOfMemory;
+  CUtensorMap mQ, mK, mV;
+  if (!encode_map4(&mQ, kBF16, a.Q, a.K_dim, a.M, a.q_heads, a.batch, f.rows.Mt, f.rows.Gt, f.rows.St) ||
+      !encode_map4(&mK, kBF16, K, a.K_dim, N, a.kv_heads, B, kTile, 1, 1) ||
+      !encode_map4(&mV, kBF16, V, a.K_dim, N, a.kv_heads, B, kTile, 1, 1))
+    return set_error(kErrInvalidArgument, "tensor map encoding failed");
+  FwdParams<T> p;
+  p.rows = f.rows;
+  p.B = B;
+  p.Hkv = a.kv_heads;
+  p.N = N;
+  p.lens = lens;
+  p.splits = f.splits;
+  p.pairs = f.pairs;
+  p.items = f.items;
+  p.O = view_of<T>(a.O);
+  p.LSE = a.LSE;
+  p.partial = partial || f.splits > 1;
+  p.part_o = static_cast<float*>(a.workspace);
+  p.part_lse = p.part_o + static_cast<int64_t>(f.splits) * f.all_rows * a.K_dim;
+  p.scale = a.softmax_scale;
+  p.status = st;
+  p.timeout_ns = effective_timeout_ns();
+  const unsigned grid = static_cast<unsigned>(std::min(f.items, sms));
+  auto go = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    using Cfg = FwdCfg<D>;
+    allow_smem<attn_fwd_kernel<T, D>>(Cfg::kSmemBytes, device);
+    attn_fwd_kernel<T, D><<<grid, Cfg::kThreads, Cfg::kSmemBytes, stream>>>(mQ, mK, mV, p);
+    if (f.splits > 1 && !partial) {
+      const int64_t threads = f.all_rows * (D / 4);
+      attn_join_kernel<T, D><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, stream>>>(
+          p.part_o, p.part_lse, f.splits, f.all_rows, p.O, p.LSE, a.q_heads, a.M);
+    }
+  };
+  if (a.K_dim == 128) go(std::integral_constant<int, 128>{});
+  else go(std::integral_constant<int, 64>{});
+  return kOk;
+}
+
+// The SM count that workspace sizes go by: a call on a device with more SMs
+// than this would split finer than its workspace allows, so plans use it too.
+constexpr int kPlanSms = 148;
+
+inline FwdPlan cross_plan(const fmha_attn_t& a) {
+  return plan_fwd(a.M, a.q_heads / a.kv_heads, 1, a.batch, a.kv_heads, a.N, a.K_dim, kPlanSms, false);
+}
+
+inline int attn_workspace(const fmha_attn_t& a, AttnOp op, uint64_t* bytes) {
+  const int rc = check_attn_sizes(a, op);
+  if (rc != kOk) return rc;
+  *bytes = 0;
+  if (op == AttnOp::kCrossFwd) *bytes = cross_plan(a).ws_bytes;
+  return kOk;
+}
+
+template <typename T>
+int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
+  if (!args) return set_error(kErrInvalidArgument, "null arguments");
+  fmha_attn_t a = *args;
+  int rc = check_attn(a, op);
+  if (rc != kOk) return rc;
+  uint64_t need = 0;
+  if ((rc = attn_workspace(a, op, &need)) != kOk) return rc;
+  if (need > 0 && (!a.workspace || a.workspace_bytes < need))
+    return set_error(kErrInvalidArgument, "workspace of %llu bytes, %llu needed",
+                     static_cast<unsigned long long>(a.workspace ? a.workspace_bytes : 0),
+                     static_cast<unsigned long long>(need));
+  if (need > 0 && !aligned16(a.workspace)) return set_error(kErrMisaligned, "workspace must be 16-byte aligned");
+  int device = 0, sms = 0;
+  if ((rc = attn_device(device, sms)) != kOk) return rc;
+  if (op == AttnOp::kCrossFwd)
+    rc = enqueue_fwd<T>(a, cross_plan(a), a.K, a.V, a.batch, a.N, a.kv_lens, false, device, sms, stream);
+  else
+    rc = run_simple<T>(a, op, stream);
+  if (rc != kOk) return rc;
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(kErrLaunch, "launch failed: %s", cudaGetErrorString(e));
+  return set_error(kOk, "");
+}
+
+}  // namespace fmha_sm100
