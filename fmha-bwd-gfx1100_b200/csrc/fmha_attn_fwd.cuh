@@ -240,6 +240,8 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   WaitCtx ctx{abort_flag, p.timeout_ns};
   const int first = blockIdx.x, step = gridDim.x;
+  // a launch that joins the parts may start, and waits for them itself
+  if (p.partial) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp >= 12) {
     regs_lower<Cfg::kOtherRegs>();

@@ -1,7 +1,7 @@
 // Host side of the attention entries: workspace, tensor maps and launches.
 #pragma once
 
-#include "fmha_attn_fwd.cuh"
+#include "fmha_attn_decode.cuh"
 #include "fmha_attn_simple.cuh"
 
 namespace fmha_sm100 {
@@ -45,6 +45,10 @@ void allow_smem(int bytes, int device) {
   cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (device < 64) done[device].store(true);
 }
+
+// The SM count that workspace sizes go by: a call on a device with more SMs
+// than this would split finer than its workspace allows, so plans use it too.
+constexpr int kPlanSms = 148;
 
 // How a forward over `B` key batches divides its work.
 struct FwdPlan {
@@ -116,19 +120,124 @@ int enqueue_fwd(const fmha_attn_t& a, const FwdPlan& f, const fmha_tensor_t& K, 
   return kOk;
 }
 
-// The SM count that workspace sizes go by: a call on a device with more SMs
-// than this would split finer than its workspace allows, so plans use it too.
-constexpr int kPlanSms = 148;
+// How few-row attention divides its work: 8 or 16 rows a block, and the
+// number of blocks that share a kv head's keys.
+struct DecodePlan {
+  int R, row_tiles, splits;
+  int64_t tasks;
+};
+
+// Of 1 to 16 blocks a tile of rows, the number with the least estimated time:
+// waves of blocks (kDecodeSlots on the GPU at a time) times a block's steps of
+// 64 keys plus its fixed costs, which measure like kDecodeFixed such steps.
+constexpr int kDecodeSlots = 4 * kPlanSms, kDecodeFixed = 4;
+inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N) {
+  DecodePlan d;
+  const int64_t rows = static_cast<int64_t>(G) * M;
+  d.R = rows <= 8 ? 1 : 2;
+  d.row_tiles = static_cast<int>((rows + 8 * d.R - 1) / (8 * d.R));
+  d.tasks = static_cast<int64_t>(B) * Hkv * d.row_tiles;
+  const int64_t steps = (N + 16 * kDecodeWarps - 1) / (16 * kDecodeWarps);
+  d.splits = 1;
+  int64_t best = 0;
+  for (int s = 1; s <= 16 && s <= steps; s *= 2) {
+    const int64_t cost = (d.tasks * s + kDecodeSlots - 1) / kDecodeSlots * ((steps + s - 1) / s + kDecodeFixed);
+    if (s == 1 || cost < best) {
+      best = cost;
+      d.splits = s;
+    }
+  }
+  return d;
+}
+
+// Up to this many query rows a kv head go through attn_decode_kernel.
+constexpr int kDecodeRows = 16;
+inline bool is_decode(const fmha_attn_t& a) {
+  return static_cast<int64_t>(a.M) * (a.q_heads / a.kv_heads) <= kDecodeRows;
+}
+
+// `parts` > 0: joins that many parts of every row in the workspace, which the
+// launch before this one on the stream writes; token m then reads its entry's
+// keys up to itself.
+template <typename T>
+int enqueue_decode(const fmha_attn_t& a, bool prefix, int parts, int64_t all_rows, int device, cudaStream_t stream) {
+  const int G = a.q_heads / a.kv_heads;
+  const DecodePlan d = plan_decode(a.M, G, a.batch, a.kv_heads, a.N);
+  DecodeParams<T> p;
+  p.Q = view_of<T>(a.Q);
+  p.K = view_of<T>(a.K);
+  p.V = view_of<T>(a.V);
+  p.O = view_of<T>(a.O);
+  p.LSE = a.LSE;
+  p.lens = a.kv_lens;
+  p.B = a.batch;
+  p.Hkv = a.kv_heads;
+  p.G = G;
+  p.M = a.M;
+  p.N = a.N;
+  p.row_tiles = d.row_tiles;
+  p.splits = d.splits;
+  p.causal = prefix;
+  p.scale = a.softmax_scale;
+  p.parts = parts;
+  p.all_rows = all_rows;
+  p.part_o = parts > 0 ? static_cast<const float*>(a.workspace) : nullptr;
+  p.part_lse = parts > 0 ? p.part_o + parts * all_rows * a.K_dim : nullptr;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(d.tasks * d.splits));
+  cfg.blockDim = dim3(32 * kDecodeWarps);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  if (d.splits > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = d.splits;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (parts > 0) {  // starts while the parts are still being written
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.attrs = at;
+  auto go = [&](auto dim, auto r) {
+    constexpr int D = decltype(dim)::value, R = decltype(r)::value;
+    constexpr auto kernel = attn_decode_kernel<T, D, R>;
+    static std::atomic<bool> done[64];
+    if (device >= 64 || !done[device].load()) {
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (device < 64) done[device].store(true);
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  using R1 = std::integral_constant<int, 1>;
+  using R2 = std::integral_constant<int, 2>;
+  const cudaError_t e = a.K_dim == 128 ? (d.R == 1 ? go(D128{}, R1{}) : go(D128{}, R2{}))
+                                       : (d.R == 1 ? go(D64{}, R1{}) : go(D64{}, R2{}));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(kErrLaunch, "launch failed: %s", cudaGetErrorString(e));
+  }
+  return kOk;
+}
 
 inline FwdPlan cross_plan(const fmha_attn_t& a) {
   return plan_fwd(a.M, a.q_heads / a.kv_heads, 1, a.batch, a.kv_heads, a.N, a.K_dim, kPlanSms, false);
+}
+
+inline FwdPlan prefix_plan(const fmha_attn_t& a) {
+  return plan_fwd(a.M, a.q_heads / a.kv_heads, a.batch / a.prefixes, a.prefixes, a.kv_heads, a.N_prefix, a.K_dim,
+                  kPlanSms, true);
 }
 
 inline int attn_workspace(const fmha_attn_t& a, AttnOp op, uint64_t* bytes) {
   const int rc = check_attn_sizes(a, op);
   if (rc != kOk) return rc;
   *bytes = 0;
-  if (op == AttnOp::kCrossFwd) *bytes = cross_plan(a).ws_bytes;
+  if (op == AttnOp::kCrossFwd && !is_decode(a)) *bytes = cross_plan(a).ws_bytes;
+  if (op == AttnOp::kPrefix) *bytes = prefix_plan(a).ws_bytes;
   return kOk;
 }
 
@@ -147,10 +256,17 @@ int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
   if (need > 0 && !aligned16(a.workspace)) return set_error(kErrMisaligned, "workspace must be 16-byte aligned");
   int device = 0, sms = 0;
   if ((rc = attn_device(device, sms)) != kOk) return rc;
-  if (op == AttnOp::kCrossFwd)
+  if (op == AttnOp::kCrossFwd && is_decode(a)) {
+    rc = enqueue_decode<T>(a, false, 0, 0, device, stream);
+  } else if (op == AttnOp::kPrefix) {
+    const FwdPlan f = prefix_plan(a);
+    rc = enqueue_fwd<T>(a, f, a.Kp, a.Vp, a.prefixes, a.N_prefix, a.prefix_lens, true, device, sms, stream);
+    if (rc == kOk) rc = enqueue_decode<T>(a, true, f.splits, f.all_rows, device, stream);
+  } else if (op == AttnOp::kCrossFwd) {
     rc = enqueue_fwd<T>(a, cross_plan(a), a.K, a.V, a.batch, a.N, a.kv_lens, false, device, sms, stream);
-  else
-    rc = run_simple<T>(a, op, stream);
+  } else {
+    rc = run_simple<T>(a, stream);
+  }
   if (rc != kOk) return rc;
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(kErrLaunch, "launch failed: %s", cudaGetErrorString(e));

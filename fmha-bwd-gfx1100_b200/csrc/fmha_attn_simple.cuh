@@ -1,7 +1,6 @@
-// The attention operators written straight from their formulas: one warp per
-// output row, every product in fp32 on the CUDA cores, one pass over the keys
-// with a running maximum and sum. Right for every case; bounded by the
-// re-reading of K and V for every row.
+// The backward of attention written straight from its formulas: one warp per
+// output row, every product in fp32 on the CUDA cores. Right for every case;
+// bounded by the re-reading of the other rows for every row.
 #pragma once
 
 #include "fmha_attn.cuh"
@@ -26,47 +25,6 @@ __device__ __forceinline__ float warp_sum(float x) {
 template <typename T>
 __device__ __forceinline__ float as_float(T x) {
   return static_cast<float>(x);
-}
-
-// O and LSE. Lane l holds elements l, l + 32, ... of its warp's row.
-template <typename T, int D, bool kPrefix>
-__global__ void simple_fwd_kernel(SimpleParams<T> p) {
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
-  const int lane = threadIdx.x & 31;
-  if (row >= static_cast<int64_t>(p.B) * p.Hq * p.M) return;
-  const int m = static_cast<int>(row % p.M), h = static_cast<int>(row / p.M % p.Hq), b = static_cast<int>(row / p.M / p.Hq);
-  const int hk = h / (p.Hq / p.Hkv);
-  constexpr int E = D / 32;
-  float q[E], acc[E], mx = -INFINITY, sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = as_float(p.Q.at(b, h, m)[lane + 32 * e]) * p.scale;
-    acc[e] = 0.f;
-  }
-  auto walk = [&](const T* k, const T* v, int64_t sk, int64_t sv, int n) {
-    for (int j = 0; j < n; ++j, k += sk, v += sv) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) s = fmaf(q[e], as_float(k[lane + 32 * e]), s);
-      s = warp_sum(s);
-      const float top = fmaxf(mx, s);
-      const float keep = expf(mx - top), w = expf(s - top);
-      sum = sum * keep + w;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + w * as_float(v[lane + 32 * e]);
-      mx = top;
-    }
-  };
-  if (kPrefix) {
-    const int pi = b / (p.B / p.prefixes);
-    walk(p.Kp.at(pi, hk, 0), p.Vp.at(pi, hk, 0), p.Kp.sr, p.Vp.sr, valid_rows(p.prefix_lens, pi, p.Np));
-  }
-  const int own = valid_rows(p.kv_lens, b, p.N) - (kPrefix ? p.M - 1 - m : 0);
-  walk(p.K.at(b, hk, 0), p.V.at(b, hk, 0), p.K.sr, p.V.sr, own);
-  const bool any = sum > 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) p.O.at(b, h, m)[lane + 32 * e] = T(any ? acc[e] / sum : 0.f);
-  if (lane == 0) p.LSE[row] = any ? mx + logf(sum) : -INFINITY;
 }
 
 // dQ, one warp per query row.
@@ -151,7 +109,7 @@ __global__ void simple_dkv_kernel(SimpleParams<T> p) {
 }
 
 template <typename T>
-int run_simple(const fmha_attn_t& a, AttnOp op, cudaStream_t stream) {
+int run_simple(const fmha_attn_t& a, cudaStream_t stream) {
   const SimpleParams<T> p{view_of<T>(a.Q), view_of<T>(a.O), view_of<T>(a.K), view_of<T>(a.V), view_of<T>(a.dO),
                           view_of<T>(a.dQ), view_of<T>(a.dK), view_of<T>(a.dV), view_of<T>(a.Kp), view_of<T>(a.Vp),
                           a.LSE, a.kv_lens, a.prefix_lens, a.batch, a.q_heads, a.kv_heads, a.M, a.N, a.K_dim,
@@ -161,14 +119,8 @@ int run_simple(const fmha_attn_t& a, AttnOp op, cudaStream_t stream) {
   const unsigned gk = blocks(static_cast<int64_t>(a.batch) * a.kv_heads * a.N);
   auto go = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
-    if (op == AttnOp::kCrossFwd) {
-      simple_fwd_kernel<T, D, false><<<gq, 256, 0, stream>>>(p);
-    } else if (op == AttnOp::kPrefix) {
-      simple_fwd_kernel<T, D, true><<<gq, 256, 0, stream>>>(p);
-    } else {
-      simple_dq_kernel<T, D><<<gq, 256, 0, stream>>>(p);
-      simple_dkv_kernel<T, D><<<gk, 256, 0, stream>>>(p);
-    }
+    simple_dq_kernel<T, D><<<gq, 256, 0, stream>>>(p);
+    simple_dkv_kernel<T, D><<<gk, 256, 0, stream>>>(p);
   };
   if (a.K_dim == 128) go(std::integral_constant<int, 128>{});
   else go(std::integral_constant<int, 64>{});
