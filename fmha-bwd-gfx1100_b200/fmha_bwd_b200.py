@@ -259,97 +259,105 @@ def _tensor_arg(t):
     return t.data_ptr(), sb, sh, sr
 
 
-def _check_attn_tensor(name, t, like, shape):
-    if not t.is_cuda or t.device != like.device:
-        raise ValueError(f"{name} must be a CUDA tensor on {like.device}")
-    if t.dtype != like.dtype:
-        raise TypeError(f"{name} has dtype {t.dtype}, expected {like.dtype}")
+def _check_attn_tensor(name, t, dev, dtype, shape):
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be a CUDA tensor on device {dev}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.stride(3) != 1:
         raise ValueError(f"{name} must have unit stride along its last axis")
 
 
-def _check_lens(name, t, like, count):
-    if t is None:
-        return 0
-    if not t.is_cuda or t.device != like.device or t.dtype != torch.int32 or not t.is_contiguous() \
-            or t.shape != (count,):
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {count} elements on {like.device}")
-    return t.data_ptr()
+def _check_lens(name, t, dev, count):
+    if t is not None and (t.get_device() != dev or t.dtype != torch.int32 or t.dim() != 1 or t.numel() != count
+                          or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {count} elements on device {dev}")
 
 
-def _check_lse(LSE, Q):
-    if not LSE.is_cuda or LSE.device != Q.device or LSE.dtype != torch.float32 or not LSE.is_contiguous() \
-            or LSE.shape != Q.shape[:3]:
-        raise ValueError(f"LSE must be a contiguous fp32 tensor of shape {tuple(Q.shape[:3])} on {Q.device}")
+def _check_lse(LSE, dev, shape):
+    if LSE.get_device() != dev or LSE.dtype != torch.float32 or LSE.shape != shape[:3] or not LSE.is_contiguous():
+        raise ValueError(f"LSE must be a contiguous fp32 tensor of shape {tuple(shape[:3])} on device {dev}")
 
 
-def _check_qkv(Q, K, V, names=("K", "V")):
-    for name, t in zip(("Q", *names), (Q, K, V)):
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor")
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be [batch, heads, rows, d]")
-    library_path(Q.dtype)  # refuses other dtypes
-    B, Hq, _, d = Q.shape
-    if K.shape[1] == 0 or Hq % K.shape[1] != 0:
-        raise ValueError(f"{Hq} query heads do not divide among {K.shape[1]} kv heads")
-    _check_attn_tensor("Q", Q, Q, Q.shape)
-    _check_attn_tensor(names[0], K, Q, (K.shape[0], K.shape[1], K.shape[2], d))
-    _check_attn_tensor(names[1], V, Q, K.shape)
+def _check_qkv(Q, shape, K, V, names=("K", "V")):
+    """Checks Q (whose shape is `shape`) against K and V; returns K's shape and the device index."""
+    dev, dtype = Q.get_device(), Q.dtype
+    if dev < 0:
+        raise ValueError("Q must be a CUDA tensor")
+    if dtype not in LIB_NAMES:
+        raise TypeError(f"unsupported dtype {dtype}; use torch.bfloat16 or torch.float16")
+    kshape = K.shape
+    if len(shape) != 4 or len(kshape) != 4:
+        raise ValueError(f"Q and {names[0]} must be [batch, heads, rows, d]")
+    if kshape[1] == 0 or shape[1] % kshape[1] != 0:
+        raise ValueError(f"{shape[1]} query heads do not divide among {kshape[1]} kv heads")
+    if kshape[3] != shape[3]:
+        raise ValueError(f"{names[0]} has {kshape[3]} columns, Q has {shape[3]}")
+    if Q.stride(3) != 1:
+        raise ValueError("Q must have unit stride along its last axis")
+    _check_attn_tensor(names[0], K, dev, dtype, kshape)
+    _check_attn_tensor(names[1], V, dev, dtype, kshape)
+    return kshape, dev
 
 
 @functools.lru_cache(maxsize=4096)
-def _attn_workspace_bytes(dtype, op, sizes):
+def _attn_entry(dtype, op, sizes):
+    """The entry of `op` for `dtype`, its library, and the workspace bytes of these sizes."""
     lib = load_library(dtype)
     need = ctypes.c_uint64()
     rc = lib.fmha_attn_workspace(_ATTN.pack(*_NO_TENSOR * 10, 0, 0, 0, 0, 0, *sizes, 1.0, 0), op, ctypes.byref(need))
     _raise_if_error(lib, rc)
-    return need.value
+    return getattr(lib, ATTN_NAMES[dtype][op]), lib, need.value
 
 
-def _run_attn(op, Q, tensors, make_out, out, LSE, kv_lens, prefix_lens, sizes, scale, stream, sync):
+def _run_attn(op, Q, dev, tensors, make_out, out, LSE, kv_lens, prefix_lens, sizes, scale, stream, sync):
     """One call of an attention entry on `stream`. `tensors` are the ten of
     fmha_attn_t, with ... in the place of each output (an LSE that is one comes
-    last among them) and None for those that the entry does not take; outputs and workspace come from torch's allocator,
-    for the stream that the call runs on."""
+    last among them) and None for those that the entry does not take; outputs
+    and workspace come from torch's allocator, for the stream that the call
+    runs on."""
     if not 0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite, not {scale}")
-    dev = Q.device
-    if torch.cuda.current_device() != dev.index:
+    if torch.cuda.current_device() != dev:
         with torch.cuda.device(dev):
-            return _run_attn(op, Q, tensors, make_out, out, LSE, kv_lens, prefix_lens, sizes, scale, stream, sync)
-    current = torch.cuda.current_stream()
-    if stream is not None and stream != current:
-        if stream.device != dev:
-            raise ValueError(f"stream is on {stream.device}, the tensors on {dev}")
-        with torch.cuda.stream(stream):
-            res = _run_attn(op, Q, tensors, make_out, out, LSE, kv_lens, prefix_lens, sizes, scale, None, sync)
-        # memory used on a stream other than the one it was allocated for
-        for t in (*tensors, LSE, kv_lens, prefix_lens):
-            if isinstance(t, torch.Tensor):
-                t.record_stream(stream)
-        for t in res:
-            t.record_stream(stream if out is not None else current)
-        return res
-    res = make_out() if out is None else out
-    need = _attn_workspace_bytes(Q.dtype, op, sizes)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    made = iter(res)
+            return _run_attn(op, Q, dev, tensors, make_out, out, LSE, kv_lens, prefix_lens, sizes, scale, stream, sync)
+    if stream is not None:
+        current = torch.cuda.current_stream(dev)
+        if stream.device.index != dev:
+            raise ValueError(f"stream is on {stream.device}, the tensors on device {dev}")
+        if stream != current:
+            with torch.cuda.stream(stream):
+                res = _run_attn(op, Q, dev, tensors, make_out, out, LSE, kv_lens, prefix_lens, sizes, scale, None, sync)
+            # memory used on a stream other than the one it was allocated for
+            for t in (*tensors, LSE, kv_lens, prefix_lens):
+                if isinstance(t, torch.Tensor):
+                    t.record_stream(stream)
+            for t in res:
+                t.record_stream(stream if out is not None else current)
+            return res
+    entry, lib, need = _attn_entry(Q.dtype, op, sizes)
+    res = made = make_out() if out is None else out
+    ws = torch.empty(need, dtype=torch.uint8, device=Q.device).data_ptr() if need else 0
     args = []
+    k = 0
     for t in tensors:
-        args += _NO_TENSOR if t is None else _tensor_arg(next(made) if t is Ellipsis else t)
-    if LSE is Ellipsis:
-        LSE = next(made)
-    lib = load_library(Q.dtype)
-    rc = getattr(lib, ATTN_NAMES[Q.dtype][op])(
-        _ATTN.pack(*args, LSE.data_ptr(), 0 if kv_lens is None else kv_lens.data_ptr(),
-                   0 if prefix_lens is None else prefix_lens.data_ptr(), ws.data_ptr() if need else 0, need, *sizes,
-                   scale, 0), current.cuda_stream)
-    _raise_if_error(lib, rc)
+        if t is None:
+            args += _NO_TENSOR
+        elif t is Ellipsis:
+            args += _tensor_arg(made[k])
+            k += 1
+        else:
+            args += _tensor_arg(t)
+    rc = entry(
+        _ATTN.pack(*args, (made[k] if LSE is Ellipsis else LSE).data_ptr(),
+                   0 if kv_lens is None else kv_lens.data_ptr(), 0 if prefix_lens is None else prefix_lens.data_ptr(),
+                   ws, need, *sizes, scale, 0), torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        _raise_if_error(lib, rc)
     if sync:
-        current.synchronize()
+        torch.cuda.current_stream(dev).synchronize()
         if lib.fmha_bwd_poll_device_status() != 0:
             raise FmhaBwdError(6, f"{ATTN_NAMES[Q.dtype][op]}: an in-kernel wait gave up")
     return tuple(res)
@@ -372,18 +380,18 @@ def cross_attn_fwd(Q, K, V, kv_lens=None, scale=None, *, out=None, stream=None, 
     ``out`` may supply (O, LSE). Runs on ``stream`` (default: torch's current
     stream); with ``sync`` the call waits and raises on an in-kernel wait
     timeout. With sync=False it can be captured into a CUDA graph."""
-    _check_qkv(Q, K, V)
-    B, Hq, M, d = Q.shape
-    if K.shape[0] != B:
-        raise ValueError(f"K has batch {K.shape[0]}, expected {B}")
-    _check_lens("kv_lens", kv_lens, Q, B)
+    shape = B, Hq, M, d = Q.shape
+    kshape, dev = _check_qkv(Q, shape, K, V)
+    if kshape[0] != B:
+        raise ValueError(f"K has batch {kshape[0]}, expected {B}")
+    _check_lens("kv_lens", kv_lens, dev, B)
     if out is not None:
-        _check_attn_tensor("O", out[0], Q, Q.shape)
-        _check_lse(out[1], Q)
+        _check_attn_tensor("O", out[0], dev, Q.dtype, shape)
+        _check_lse(out[1], dev, shape)
     return _run_attn(
-        _CROSS_FWD, Q, (Q, ..., K, V, None, None, None, None, None, None),
-        lambda: (torch.empty_like(Q), torch.empty(B, Hq, M, dtype=torch.float32, device=Q.device)), out, ..., kv_lens, None,
-        (B, Hq, K.shape[1], M, K.shape[2], d, 0, 0), d ** -0.5 if scale is None else float(scale), stream, sync)
+        _CROSS_FWD, Q, dev, (Q, ..., K, V, None, None, None, None, None, None),
+        lambda: (torch.empty_like(Q), torch.empty(shape[:3], dtype=torch.float32, device=Q.device)), out, ..., kv_lens,
+        None, (B, Hq, kshape[1], M, kshape[2], d, 0, 0), d ** -0.5 if scale is None else float(scale), stream, sync)
 
 
 def cross_attn_bwd(Q, K, V, O, LSE, dO, kv_lens=None, scale=None, *, out=None, stream=None, sync: bool = True):
@@ -392,21 +400,21 @@ def cross_attn_bwd(Q, K, V, O, LSE, dO, kv_lens=None, scale=None, *, out=None, s
     the query heads of their kv head and are zero at and past kv_lens. There
     are no atomics: two calls give the same bits. ``out`` may supply (dQ, dK,
     dV), which are fully overwritten; ``stream`` and ``sync`` as there."""
-    _check_qkv(Q, K, V)
-    B, Hq, M, d = Q.shape
-    if K.shape[0] != B:
-        raise ValueError(f"K has batch {K.shape[0]}, expected {B}")
-    _check_attn_tensor("O", O, Q, Q.shape)
-    _check_attn_tensor("dO", dO, Q, Q.shape)
-    _check_lse(LSE, Q)
-    _check_lens("kv_lens", kv_lens, Q, B)
+    shape = B, Hq, M, d = Q.shape
+    kshape, dev = _check_qkv(Q, shape, K, V)
+    if kshape[0] != B:
+        raise ValueError(f"K has batch {kshape[0]}, expected {B}")
+    _check_attn_tensor("O", O, dev, Q.dtype, shape)
+    _check_attn_tensor("dO", dO, dev, Q.dtype, shape)
+    _check_lse(LSE, dev, shape)
+    _check_lens("kv_lens", kv_lens, dev, B)
     if out is not None:
-        for name, t, like in zip(("dQ", "dK", "dV"), out, (Q, K, V)):
-            _check_attn_tensor(name, t, Q, like.shape)
+        for name, t, like in zip(("dQ", "dK", "dV"), out, (shape, kshape, kshape)):
+            _check_attn_tensor(name, t, dev, Q.dtype, like)
     return _run_attn(
-        _CROSS_BWD, Q, (Q, O, K, V, dO, ..., ..., ..., None, None),
+        _CROSS_BWD, Q, dev, (Q, O, K, V, dO, ..., ..., ..., None, None),
         lambda: (torch.empty_like(Q), torch.empty_like(K), torch.empty_like(V)), out, LSE, kv_lens, None,
-        (B, Hq, K.shape[1], M, K.shape[2], d, 0, 0), d ** -0.5 if scale is None else float(scale), stream, sync)
+        (B, Hq, kshape[1], M, kshape[2], d, 0, 0), d ** -0.5 if scale is None else float(scale), stream, sync)
 
 
 def prefix_attn(Q, Kp, Vp, K, V, prefix_lens=None, kv_lens=None, scale=None, *, out=None, stream=None,
@@ -422,24 +430,24 @@ def prefix_attn(Q, Kp, Vp, K, V, prefix_lens=None, kv_lens=None, scale=None, *, 
     the M newest tokens' own rows last: row m sees all but the M - 1 - m
     newest. The softmax runs over both. The prefix is read once for all of
     its entries. Strides, ``out``, ``stream`` and ``sync`` as cross_attn_fwd."""
-    _check_qkv(Q, K, V)
-    _check_qkv(Q, Kp, Vp, ("Kp", "Vp"))
-    B, Hq, M, d = Q.shape
-    P, Hkv = Kp.shape[:2]
-    if K.shape[0] != B or K.shape[1] != Hkv:
-        raise ValueError(f"K has batch and heads {tuple(K.shape[:2])}, expected {(B, Hkv)}")
+    shape = B, Hq, M, d = Q.shape
+    kshape, dev = _check_qkv(Q, shape, K, V)
+    pshape, _ = _check_qkv(Q, shape, Kp, Vp, ("Kp", "Vp"))
+    P, Hkv = pshape[:2]
+    if kshape[0] != B or kshape[1] != Hkv:
+        raise ValueError(f"K has batch and heads {tuple(kshape[:2])}, expected {(B, Hkv)}")
     if P == 0 or B % P != 0:
         raise ValueError(f"{B} batch entries do not divide among {P} prefixes")
-    _check_lens("prefix_lens", prefix_lens, Q, P)
-    _check_lens("kv_lens", kv_lens, Q, B)
+    _check_lens("prefix_lens", prefix_lens, dev, P)
+    _check_lens("kv_lens", kv_lens, dev, B)
     if out is not None:
-        _check_attn_tensor("O", out[0], Q, Q.shape)
-        _check_lse(out[1], Q)
+        _check_attn_tensor("O", out[0], dev, Q.dtype, shape)
+        _check_lse(out[1], dev, shape)
     return _run_attn(
-        _PREFIX, Q, (Q, ..., K, V, None, None, None, None, Kp, Vp),
-        lambda: (torch.empty_like(Q), torch.empty(B, Hq, M, dtype=torch.float32, device=Q.device)), out, ..., kv_lens,
-        prefix_lens, (B, Hq, Hkv, M, K.shape[2], d, P, Kp.shape[2]), d ** -0.5 if scale is None else float(scale),
-        stream, sync)
+        _PREFIX, Q, dev, (Q, ..., K, V, None, None, None, None, Kp, Vp),
+        lambda: (torch.empty_like(Q), torch.empty(shape[:3], dtype=torch.float32, device=Q.device)), out, ..., kv_lens,
+        prefix_lens, (B, Hq, Hkv, M, kshape[2], d, P, pshape[2]), d ** -0.5 if scale is None else float(scale), stream,
+        sync)
 
 
 # ---------------------------------------------------------------- stage hooks
