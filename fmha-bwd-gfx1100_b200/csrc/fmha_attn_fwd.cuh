@@ -59,13 +59,15 @@ struct RowPack {
   }
 };
 
-inline RowPack pack_rows(int M, int G, int S) {
+// `divides`: boxes of whole groups, none of them reaching into the next kv head.
+inline RowPack pack_rows(int M, int G, int S, bool divides = false) {
   RowPack p;
   p.M = M;
   p.G = G;
   p.S = S;
   p.Mt = M < 128 ? M : 128;
   p.Gt = std::min(G, 128 / p.Mt);
+  while (divides && G % p.Gt != 0) --p.Gt;
   p.St = std::min(S, 128 / (p.Mt * p.Gt));
   p.nm = (M + p.Mt - 1) / p.Mt;
   p.ng = (G + p.Gt - 1) / p.Gt;

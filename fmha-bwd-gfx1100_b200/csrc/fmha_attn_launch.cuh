@@ -1,8 +1,8 @@
 // Host side of the attention entries: workspace, tensor maps and launches.
 #pragma once
 
+#include "fmha_attn_bwd.cuh"
 #include "fmha_attn_decode.cuh"
-#include "fmha_attn_simple.cuh"
 
 namespace fmha_sm100 {
 
@@ -232,12 +232,115 @@ inline FwdPlan prefix_plan(const fmha_attn_t& a) {
                   kPlanSms, true);
 }
 
+// How a backward divides its work, and its workspace: packed LSE and D, the
+// amplitudes (fp16), and two partial-sum slots for each CTA of both kernels.
+struct BwdPlan {
+  RowPack rows;
+  int pairs, grid_q, grid_k, delta_blocks;
+  bool join;  // some item may fall to several CTAs
+  int64_t packed_rows, slot_floats;
+  uint64_t ws_bytes;
+};
+
+inline BwdPlan plan_bwd(const fmha_attn_t& a) {
+  BwdPlan f;
+  f.rows = pack_rows(a.M, a.q_heads / a.kv_heads, 1, true);
+  f.pairs = (f.rows.tiles + 1) / 2;
+  const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
+  const int64_t nt = (a.N + kTile - 1) / kTile;
+  f.grid_q = static_cast<int>(std::min<int64_t>(kPlanSms, heads * f.pairs * nt));
+  f.grid_k = static_cast<int>(std::min<int64_t>(kPlanSms, heads * f.rows.tiles * nt));
+  f.join = a.kv_lens != nullptr ||
+           bwd_by_steps(heads * f.pairs, nt, heads * f.pairs * nt, f.grid_q) ||
+           bwd_by_steps(heads * nt, f.rows.tiles, heads * nt * f.rows.tiles, f.grid_k);
+  f.packed_rows = heads * f.rows.tiles * kTile;
+  const int per_block = 256 / (a.K_dim / 8);
+  f.delta_blocks = static_cast<int>(std::min<int64_t>(4 * kPlanSms, (f.packed_rows + per_block - 1) / per_block));
+  f.slot_floats = 2 * static_cast<int64_t>(kTile) * a.K_dim;
+  f.ws_bytes = 4 * static_cast<uint64_t>(2 * f.packed_rows + 2 * ((f.delta_blocks + 1) / 2 * 2) +
+                                         2 * (f.grid_q + f.grid_k) * f.slot_floats);
+  return f;
+}
+
+template <typename T>
+int enqueue_bwd(const fmha_attn_t& a, int device, cudaStream_t stream) {
+  constexpr bool kBF16 = Elem<T>::kBF16;
+  if (!encode_fn()) return set_error(kErrNoDriver, "cuTensorMapEncodeTiled is unavailable");
+  KernelStatus* st = attn_status(device);
+  if (!st) return kErrOutOfMemory;
+  const BwdPlan f = plan_bwd(a);
+  CUtensorMap mQ, mK, mV, mdO;
+  if (!encode_map4(&mQ, kBF16, a.Q, a.K_dim, a.M, a.q_heads, a.batch, f.rows.Mt, f.rows.Gt, 1) ||
+      !encode_map4(&mdO, kBF16, a.dO, a.K_dim, a.M, a.q_heads, a.batch, f.rows.Mt, f.rows.Gt, 1) ||
+      !encode_map4(&mK, kBF16, a.K, a.K_dim, a.N, a.kv_heads, a.batch, kTile, 1, 1) ||
+      !encode_map4(&mV, kBF16, a.V, a.K_dim, a.N, a.kv_heads, a.batch, kTile, 1, 1))
+    return set_error(kErrInvalidArgument, "tensor map encoding failed");
+  float* lse2 = static_cast<float*>(a.workspace);
+  float* delta = lse2 + f.packed_rows;
+  float2* amax = reinterpret_cast<float2*>(delta + f.packed_rows);
+  BwdParams<T> q;
+  q.rows = f.rows;
+  q.B = a.batch;
+  q.Hkv = a.kv_heads;
+  q.N = a.N;
+  q.pairs = f.pairs;
+  q.lens = a.kv_lens;
+  q.dQ = view_of<T>(a.dQ);
+  q.dK = view_of<T>(a.dK);
+  q.dV = view_of<T>(a.dV);
+  q.lse2 = lse2;
+  q.delta = delta;
+  q.amax = amax;
+  q.amax_count = f.delta_blocks;
+  q.part = reinterpret_cast<float*>(amax + (f.delta_blocks + 1) / 2 * 2);
+  q.scale = a.softmax_scale;
+  q.status = st;
+  q.timeout_ns = effective_timeout_ns();
+  BwdParams<T> k = q;
+  k.part = q.part + 2 * f.grid_q * f.slot_floats;
+  auto go = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    allow_smem<attn_dq_kernel<T, D>>(DqCfg2<D>::kSmemBytes, device);
+    allow_smem<attn_dkv_kernel<T, D>>(DkvCfg2<D>::kSmemBytes, device);
+    attn_delta_kernel<T, D><<<f.delta_blocks, 256, 0, stream>>>(view_of<T>(a.dO), view_of<T>(a.O), view_of<T>(a.V),
+                                                               a.LSE, q, lse2, delta, amax);
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = stream;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3(f.grid_q);
+    cfg.blockDim = dim3(DqCfg2<D>::kThreads);
+    cfg.dynamicSmemBytes = DqCfg2<D>::kSmemBytes;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, attn_dq_kernel<T, D>, mQ, mK, mV, mdO, q);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(f.grid_k);
+    cfg.blockDim = dim3(DkvCfg2<D>::kThreads);
+    cfg.dynamicSmemBytes = DkvCfg2<D>::kSmemBytes;
+    e = cudaLaunchKernelEx(&cfg, attn_dkv_kernel<T, D>, mQ, mK, mV, mdO, k);
+    const int marks = std::max(f.grid_q, f.grid_k) - 1;
+    if (e == cudaSuccess && f.join && marks > 0)
+      attn_bwd_join_kernel<T, D><<<dim3(2 * kTile * D / 4 / 256, marks), 256, 0, stream>>>(q, k, f.grid_q, f.grid_k);
+    return e;
+  };
+  const cudaError_t e =
+      a.K_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{});
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(kErrLaunch, "launch failed: %s", cudaGetErrorString(e));
+  }
+  return kOk;
+}
+
 inline int attn_workspace(const fmha_attn_t& a, AttnOp op, uint64_t* bytes) {
   const int rc = check_attn_sizes(a, op);
   if (rc != kOk) return rc;
   *bytes = 0;
   if (op == AttnOp::kCrossFwd && !is_decode(a)) *bytes = cross_plan(a).ws_bytes;
   if (op == AttnOp::kPrefix) *bytes = prefix_plan(a).ws_bytes;
+  if (op == AttnOp::kCrossBwd) *bytes = plan_bwd(a).ws_bytes;
   return kOk;
 }
 
@@ -265,7 +368,7 @@ int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
   } else if (op == AttnOp::kCrossFwd) {
     rc = enqueue_fwd<T>(a, cross_plan(a), a.K, a.V, a.batch, a.N, a.kv_lens, false, device, sms, stream);
   } else {
-    rc = run_simple<T>(a, stream);
+    rc = enqueue_bwd<T>(a, device, stream);
   }
   if (rc != kOk) return rc;
   const cudaError_t e = cudaGetLastError();
