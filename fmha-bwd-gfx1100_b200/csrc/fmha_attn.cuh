@@ -78,6 +78,12 @@ inline int check_attn_sizes(const fmha_attn_t& a, AttnOp op) {
   if (static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.N) + 127) / 128) > (int64_t(1) << 30))
     return set_error(kErrInvalidArgument, "batch * kv_heads * N / 128 exceeds 2^30 tiles");
   if (a.M > (1 << 30) || a.N > (1 << 30)) return set_error(kErrInvalidArgument, "M and N must be at most 2^30");
+  // the backward counts steps of 128 rows by 128 keys, a kv head's packed rows at a time
+  if (op == AttnOp::kCrossBwd) {
+    const double tiles = static_cast<double>(a.q_heads / a.kv_heads) * ((static_cast<double>(a.M) + 127) / 128);
+    if (tiles * a.batch * a.kv_heads * ((static_cast<double>(a.N) + 127) / 128) > 1073741824.0)
+      return set_error(kErrInvalidArgument, "more than 2^30 tiles of 128 rows by 128 keys");
+  }
   if (op == AttnOp::kPrefix) {
     if (a.prefixes <= 0 || a.N_prefix <= 0 || a.N_prefix > (1 << 30))
       return set_error(kErrInvalidArgument, "prefixes=%d and N_prefix=%d must be positive", a.prefixes, a.N_prefix);

@@ -254,8 +254,7 @@ inline BwdPlan plan_bwd(const fmha_attn_t& a) {
            bwd_by_steps(heads * f.pairs, nt, heads * f.pairs * nt, f.grid_q) ||
            bwd_by_steps(heads * nt, f.rows.tiles, heads * nt * f.rows.tiles, f.grid_k);
   f.packed_rows = heads * f.rows.tiles * kTile;
-  const int per_block = 256 / (a.K_dim / 8);
-  f.delta_blocks = static_cast<int>(std::min<int64_t>(4 * kPlanSms, (f.packed_rows + per_block - 1) / per_block));
+  f.delta_blocks = static_cast<int>(std::min<int64_t>(6 * kPlanSms, heads * std::max<int64_t>(f.rows.tiles, nt)));
   f.slot_floats = 2 * static_cast<int64_t>(kTile) * a.K_dim;
   f.ws_bytes = 4 * static_cast<uint64_t>(2 * f.packed_rows + 2 * ((f.delta_blocks + 1) / 2 * 2) +
                                          2 * (f.grid_q + f.grid_k) * f.slot_floats);
@@ -312,17 +311,16 @@ int enqueue_bwd(const fmha_attn_t& a, int device, cudaStream_t stream) {
     cfg.attrs = &at;
     cfg.numAttrs = 1;
     cfg.gridDim = dim3(f.grid_q);
-    cfg.blockDim = dim3(DqCfg2<D>::kThreads);
+    cfg.blockDim = dim3(kBwdThreads);
     cfg.dynamicSmemBytes = DqCfg2<D>::kSmemBytes;
     cudaError_t e = cudaLaunchKernelEx(&cfg, attn_dq_kernel<T, D>, mQ, mK, mV, mdO, q);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(f.grid_k);
-    cfg.blockDim = dim3(DkvCfg2<D>::kThreads);
     cfg.dynamicSmemBytes = DkvCfg2<D>::kSmemBytes;
     e = cudaLaunchKernelEx(&cfg, attn_dkv_kernel<T, D>, mQ, mK, mV, mdO, k);
     const int marks = std::max(f.grid_q, f.grid_k) - 1;
     if (e == cudaSuccess && f.join && marks > 0)
-      attn_bwd_join_kernel<T, D><<<dim3(2 * kTile * D / 4 / 256, marks), 256, 0, stream>>>(q, k, f.grid_q, f.grid_k);
+      attn_bwd_join_kernel<T, D><<<dim3(kJoinBlocks, marks, 2), 256, 0, stream>>>(q, k, f.grid_q, f.grid_k);
     return e;
   };
   const cudaError_t e =
