@@ -145,42 +145,24 @@ struct BwdSchedule {
   }
 };
 
-// One warp of a CTA walks the schedule and hands the units to the others
-// through a ring in shared memory: the divisions are done once, and the other
-// roles hold a unit's few numbers only.
-constexpr int kUnitRing = 4;
-struct UnitRing {
-  int4 a[kUnitRing];  // b, hk, idx, slot
-  int4 b[kUnitRing];  // lo, hi, n, whether it is a unit (else the end)
-};
-
 template <typename T, bool kQMajor>
 __device__ void feed_units(const BwdParams<T>& p, UnitRing* ring, uint64_t* full, uint64_t* empty, const WaitCtx& ctx,
                            int where) {
   BwdSchedule<T, kQMajor> sched(p, gridDim.x, blockIdx.x);
-  BwdUnit u;
+  BwdUnit u{};
   for (int k = 0;; ++k) {
     const bool more = sched.next(u);
-    const int i = k % kUnitRing;
-    if (k >= kUnitRing && !mbar_wait(&empty[i], ((k / kUnitRing) - 1) & 1, ctx, where)) return;
-    ring->a[i] = make_int4(u.b, u.hk, u.idx, u.slot);
-    ring->b[i] = make_int4(u.lo, u.hi, u.n, more ? 1 : 0);
-    mbar_arrive(&full[i]);
-    if (!more) return;
+    if (!put_unit(ring, full, empty, k, make_int4(u.b, u.hk, u.idx, u.slot), make_int4(u.lo, u.hi, u.n, more ? 1 : 0),
+                  ctx, where) || !more)
+      return;
   }
 }
 
-// Unit k, for a whole warp; false at the end or on a failed wait (`ok`).
+template <bool kWarp>
 __device__ __forceinline__ bool take_unit(const UnitRing* ring, uint64_t* full, uint64_t* empty, int& k, BwdUnit& u,
-                                          int lane, const WaitCtx& ctx, int where, bool& ok) {
-  const int i = k % kUnitRing;
-  if (!mbar_wait(&full[i], (k / kUnitRing) & 1, ctx, where)) ok = false;
-  ok = __all_sync(0xffffffffu, ok);
-  if (!ok) return false;
-  const int4 a = ring->a[i], b = ring->b[i];
-  __syncwarp();
-  if (lane == 0) mbar_arrive(&empty[i]);
-  ++k;
+                                          const WaitCtx& ctx, int where, bool& ok) {
+  int4 a, b;
+  if (!get_unit<kWarp>(ring, full, empty, k, a, b, ctx, where, ok)) return false;
   u.b = a.x;
   u.hk = a.y;
   u.idx = a.z;
@@ -188,7 +170,7 @@ __device__ __forceinline__ bool take_unit(const UnitRing* ring, uint64_t* full, 
   u.lo = b.x;
   u.hi = b.y;
   u.n = b.z;
-  return b.w != 0;
+  return true;
 }
 
 // The power of two by which fp16 holds dS (see the top), 0 for bf16.
@@ -509,7 +491,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ++nv;
         return true;
       };
-      while (take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 300, ok)) {
+      while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 300, ok)) {
         if (lane == 0) {
           ok = load_q(0, nq0) && load_k(u.lo) && (2 * u.idx + 1 >= q_tiles || load_q(1, nq1));
           for (int j = u.lo; j < u.hi && ok; ++j) ok = load_v(j) && (j + 1 == u.hi || load_k(j + 1));
@@ -607,7 +589,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         return good;
       };
-      bool has = take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 309, ok);
+      bool has = take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 309, ok);
       int g = 0, j = u.lo;
       bool two = 2 * u.idx + 1 < q_tiles;
       // what dQ1 of the step before needs
@@ -638,7 +620,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ++j;
         bool opens = false;
         if (ok && closes) {
-          has = take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 309, ok);
+          has = take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 309, ok);
           j = u.lo;
           two = 2 * u.idx + 1 < q_tiles;
           opens = true;
@@ -676,7 +658,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const float sl2 = p.scale * kLog2e;
     const float ds_mul = pow2(ds_exponent<T, D>(p, lane) - kPBias);
     int ns = 0;
-    while (take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 319, ok)) {
+    while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 319, ok)) {
       const int tile = 2 * u.idx + t;
       if (tile >= q_tiles) continue;
       const int64_t row = ((static_cast<int64_t>(u.b) * p.Hkv + u.hk) * q_tiles + tile) * kTile + r;
@@ -717,7 +699,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int r = threadIdx.x & 127;
     const float out_mul = p.scale * pow2(-ds_exponent<T, D>(p, lane));
     int na[2] = {0, 0};
-    while (take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 329, ok)) {
+    while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 329, ok)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int tile = 2 * u.idx + t;
@@ -854,7 +836,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const uint64_t pol_q = l2_policy_evict_last(), pol_kv = l2_policy_evict_first();
       const uint32_t q_bytes = static_cast<uint32_t>(box_rows) * 128u * (D / kBoxCols);
       int nu = 0, n = 0, no = 0;
-      while (take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 400, ok)) {
+      while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 400, ok)) {
         if (lane == 0) {
           ok = nu == 0 || mbar_wait(&bar[kBkKVEmpty], (nu - 1) & 1, ctx, 401);
           if (ok) {
@@ -938,7 +920,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (closes) umma_commit(&bar[kBkKVEmpty]);
         return true;
       };
-      bool has = take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 409, ok);
+      bool has = take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 409, ok);
       int n = 0, i = u.lo, lo = u.lo, hi = u.hi;
       if (has && lane == 0) ok = do_s(0, true) && do_dp(0, lo + 1 == hi);
       ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -947,7 +929,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         bool more = true;
         int i1 = i + 1;
         if (closes) {
-          more = take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 409, ok);
+          more = take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 409, ok);
           i1 = u.lo;
         }
         if (lane == 0 && ok) {
@@ -1003,7 +985,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const float sl2 = p.scale * kLog2e;
     const float ds_mul = pow2(ds_exponent<T, D>(p, lane) - kPBias);
     int n = 0;
-    while (take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 419, ok)) {
+    while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 419, ok)) {
       // a key that does not count gets P = dS = 0, whatever K and V hold
       const bool valid = u.idx * kTile + r < u.n;
       for (int i = u.lo; i < u.hi; ++i, ++n) {
@@ -1087,7 +1069,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(r & 96) << 16;
     const float dk_mul = p.scale * pow2(-ds_exponent<T, D>(p, lane)), dv_mul = pow2(-kPBias);
     int nu = 0;
-    while (take_unit(ring, unit_full, unit_empty, k, u, lane, ctx, 429, ok)) {
+    while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 429, ok)) {
       if (!mbar_wait(&bar[kBkAcc], nu & 1, ctx, 430)) { ok = false; continue; }
       ++nu;
       __syncwarp();

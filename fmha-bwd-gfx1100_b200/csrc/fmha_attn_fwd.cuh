@@ -36,6 +36,65 @@ namespace fmha_sm100 {
 
 constexpr float kLn2 = 0.6931471805599453f;
 
+// 2^x of two values on the FMA pipe instead of the SFU, whose 16 results a
+// clock bound these kernels: x = n + f with n the nearest integer (taken from
+// the low mantissa bits of x + 1.5 2^23) and 2^f on [-1/2, 1/2] by the
+// polynomial of degree 5 with the least largest relative error there (found by
+// Remez exchange): 7.5e-8, 2.4e-7 as evaluated in fp32, like ex2.approx. Below
+// 2^-126 the result stays there; NaN stays NaN.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  const float2 magic = make_float2(12582912.f, 12582912.f);
+  const float2 t = add_f32x2(x, magic);
+  const float2 n = add_f32x2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = fma_f32x2(n, make_float2(-1.f, -1.f), x);
+  auto both = [](float c) { return make_float2(c, c); };
+  float2 p = fma_f32x2(both(1.3276472e-3f), f, both(9.675541e-3f));
+  p = fma_f32x2(p, f, both(5.550713e-2f));
+  p = fma_f32x2(p, f, both(0.24022120f));
+  p = fma_f32x2(p, f, both(0.69314694f));
+  p = fma_f32x2(p, f, both(1.0000001f));
+  const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return mul_f32x2(p, scale);
+}
+
+// Units of work that one warp of a CTA works out and the others take from a
+// ring in shared memory: the divisions are done once, and the other roles hold
+// a unit's few numbers only. A unit is two int4; its last number is 0 behind
+// the last unit.
+constexpr int kUnitRing = 4;
+struct UnitRing {
+  int4 a[kUnitRing];
+  int4 b[kUnitRing];
+};
+__device__ __forceinline__ bool put_unit(UnitRing* ring, uint64_t* full, uint64_t* empty, int k, int4 a, int4 b,
+                                         const WaitCtx& ctx, int where) {
+  const int i = k % kUnitRing;
+  if (k >= kUnitRing && !mbar_wait(&empty[i], ((k / kUnitRing) - 1) & 1, ctx, where)) return false;
+  ring->a[i] = a;
+  ring->b[i] = b;
+  mbar_arrive(&full[i]);
+  return true;
+}
+// For a whole warp (kWarp) or one thread; false at the end, or with `ok`
+// cleared (before or by the wait here).
+template <bool kWarp>
+__device__ __forceinline__ bool get_unit(const UnitRing* ring, uint64_t* full, uint64_t* empty, int& k, int4& a, int4& b,
+                                         const WaitCtx& ctx, int where, bool& ok) {
+  const int i = k % kUnitRing;
+  if (ok && !mbar_wait(&full[i], (k / kUnitRing) & 1, ctx, where)) ok = false;
+  if (kWarp) ok = __all_sync(0xffffffffu, ok);
+  if (!ok) return false;
+  a = ring->a[i];
+  b = ring->b[i];
+  if (kWarp) __syncwarp();
+  if (!kWarp || (threadIdx.x & 31) == 0) mbar_arrive(&empty[i]);
+  ++k;
+  return b.w != 0;
+}
+
 // How query rows fall into tiles (see above).
 struct RowPack {
   int M, G, S;     // tokens, query heads of a kv head, batch entries that share keys
@@ -101,31 +160,37 @@ struct FwdCfg {
   static constexpr int kOffQ = 0;                                // two tiles
   static constexpr int kOffKV = 2 * kTileBytes;
   static constexpr int kOffStat = kOffKV + kSlots * kTileBytes;  // float2 [2][128]
-  static constexpr int kOffBar = kOffStat + 2 * 128 * 8;
+  static constexpr int kOffRing = kOffStat + 2 * 128 * 8;
+  static constexpr int kOffBar = kOffRing + sizeof(UnitRing);
   static constexpr int kSmemBytes = kOffBar + 512;
   static constexpr int kThreads = 512;
   static constexpr uint32_t kColS = 0;    // + 128 * tile
   static constexpr uint32_t kColO = 256;  // + D * tile
   static_assert(kSmemBytes <= 232448, "shared memory budget");
-  // warpgroups 0 and 1 softmax, 2 epilogue, 3 loads and MMA: 2 * 128 * 184 +
-  // 2 * 128 * 72 registers, the 512 * 128 of the launch
+  // warpgroups 0 and 1 softmax, 2 epilogue, 3 loads, MMA and schedule: 2 * 128
+  // * 184 + 2 * 128 * 72 registers, the 512 * 128 of the launch
   static constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
   static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs == 4 * 128, "register split");
+  static constexpr int kReaders = 15;  // of a unit: warps 0-13 and 15
 };
 
 enum FwdBar : int {
   kFwQFull0 = 0,    // + tile
   kFwQEmpty0 = 2,   // + tile: the item's last S of the tile is done
   kFwKVFull0 = 4,   // + slot (up to 8)
-  kFwKVEmpty0 = 12, // + slot
-  kFwSFull0 = 20,   // + tile
-  kFwPFull0 = 22,   // + tile: p written (4 warps)
-  kFwOFull0 = 24,   // + tile: the item's last PV of the tile is done
-  kFwOEmpty0 = 26,  // + tile: the epilogue has read O (4 warps)
-  kFwStFull0 = 28,  // + tile: row maxima and sums written (4 warps)
-  kFwStEmpty0 = 30, // + tile: and read (4 warps)
-  kFwDrain = 32,
-  kNumFwdBars = 33,
+  kFwKVEmpty0 = 12, // + slot: both MMA issuers are done with it
+  kFwTail0 = 20,    // + slot: a last V tile has landed, its rows behind the keys not yet cleared
+  kFwSFull0 = 28,   // + tile
+  kFwPFull0 = 30,   // + tile: the first 96 columns of p written (4 warps)
+  kFwPRest0 = 32,   // + tile: and the others
+  kFwOFull0 = 34,   // + tile: the item's last PV of the tile is done
+  kFwOEmpty0 = 36,  // + tile: the epilogue has read O (4 warps)
+  kFwStFull0 = 38,  // + tile: row maxima and sums written (4 warps)
+  kFwStEmpty0 = 40, // + tile: and read (4 warps)
+  kFwUnitFull0 = 42,
+  kFwUnitEmpty0 = 46,
+  kFwDrain0 = 50,   // + tile
+  kNumFwdBars = 52,
 };
 static_assert(kNumFwdBars * 8 + 8 <= 512, "barrier area");
 
@@ -136,23 +201,45 @@ struct FwdItem {
   bool two;                    // the second tile exists
 };
 
-template <typename T>
-__device__ __forceinline__ FwdItem fwd_item(const FwdParams<T>& p, int t) {
-  FwdItem it;
-  const int pair = t % p.pairs;
-  int u = t / p.pairs;
-  it.split = u % p.splits;
-  u /= p.splits;
-  it.hk = u % p.Hkv;
-  it.b = u / p.Hkv;
-  it.tile0 = 2 * pair;
-  it.two = 2 * pair + 1 < p.rows.tiles;
-  it.n = valid_rows(p.lens, it.b, p.N);
-  const int nt = (it.n + kTile - 1) / kTile;
-  it.lo = static_cast<int>(static_cast<int64_t>(nt) * it.split / p.splits);
-  it.hi = static_cast<int>(static_cast<int64_t>(nt) * (it.split + 1) / p.splits);
-  return it;
+__device__ __forceinline__ FwdItem fwd_item(const int4& a, const int4& b) {
+  return FwdItem{a.x, a.y, a.z, a.w, b.z, b.x, b.y, b.w == 2};
 }
+
+// The items of this CTA. kv heads lie innermost: with the usual [token][head]
+// layouts of Q and O, the CTAs then read and write neighbouring memory.
+template <typename T>
+__device__ void feed_fwd(const FwdParams<T>& p, UnitRing* ring, uint64_t* full, uint64_t* empty, const WaitCtx& ctx) {
+  int k = 0;
+  for (int t = blockIdx.x; t < p.items; t += gridDim.x, ++k) {
+    const int hk = t % p.Hkv;
+    int u = t / p.Hkv;
+    const int pair = u % p.pairs;
+    u /= p.pairs;
+    const int split = u % p.splits, b = u / p.splits;
+    const int n = valid_rows(p.lens, b, p.N), nt = (n + kTile - 1) / kTile;
+    const int lo = static_cast<int>(static_cast<int64_t>(nt) * split / p.splits);
+    const int hi = static_cast<int>(static_cast<int64_t>(nt) * (split + 1) / p.splits);
+    if (!put_unit(ring, full, empty, k, make_int4(b, hk, split, 2 * pair),
+                  make_int4(lo, hi, n, 2 * pair + 1 < p.rows.tiles ? 2 : 1), ctx, 205))
+      return;
+  }
+  put_unit(ring, full, empty, k, make_int4(0, 0, 0, 0), make_int4(0, 0, 0, 0), ctx, 205);
+}
+
+// Clears rows [left, left rounded up to 16) of a landed 128-row tile, by a
+// warp: the products go over keys by 16, and would multiply what lies behind
+// the last key by 0, whatever that is.
+template <int D>
+__device__ __forceinline__ void clear_tail(uint8_t* tile, int left, int lane) {
+  const int rows = 16 - (left & 15);
+  for (int i = lane; i < rows * (D / 8); i += 32) {
+    const int row = left + i / (D / 8), c = i % (D / 8);
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * kBoxBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+        make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+}
+__device__ __forceinline__ bool has_tail(int n, int hi) { return hi * kTile > n && (n & 15) != 0; }
 
 // 16-byte chunks of 16-bit output rows held one row per lane, stored so that
 // each instruction writes whole row segments (the transpose of
@@ -193,6 +280,26 @@ __device__ __forceinline__ uint4 pack8(const uint32_t* a, float mul) {
                     Elem<T>::pack(mul * __uint_as_float(a[6]), mul * __uint_as_float(a[7])));
 }
 
+// 32 weights of a row: p = 2^(s sl2 - m), every fourth pair by polynomial
+// (with kTail, where s holds -inf, none), summed into l and packed.
+template <typename T, bool kTail>
+__device__ __forceinline__ void weights_32(const uint32_t* s, float2 sc, float2 nm, float2& l0, float2& l1,
+                                           uint32_t (&e)[16]) {
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    float2 a = fma_f32x2(make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), sc, nm);
+    if (!kTail && (x & 3) == 3) {
+      a = ex2_poly(a);
+    } else {
+      a.x = ex2_approx(a.x);
+      a.y = ex2_approx(a.y);
+    }
+    if (x & 1) l1 = add_f32x2(l1, a);
+    else l0 = add_f32x2(l0, a);
+    e[x] = Elem<T>::pack(a.x, a.y);
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_Q, const __grid_constant__ CUtensorMap tm_K,
@@ -208,27 +315,20 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     return;
   }
   float2* stat = reinterpret_cast<float2*>(smem + Cfg::kOffStat);
+  UnitRing* ring = reinterpret_cast<UnitRing*>(smem + Cfg::kOffRing);
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + kNumFwdBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&bar[kFwQFull0 + t], 1);
-      mbar_init(&bar[kFwQEmpty0 + t], 1);
-      mbar_init(&bar[kFwSFull0 + t], 1);
-      mbar_init(&bar[kFwPFull0 + t], 4);
-      mbar_init(&bar[kFwOFull0 + t], 1);
-      mbar_init(&bar[kFwOEmpty0 + t], 4);
-      mbar_init(&bar[kFwStFull0 + t], 4);
-      mbar_init(&bar[kFwStEmpty0 + t], 4);
+    for (int i = 0; i < kNumFwdBars; ++i) {
+      int count = 1;
+      if (i >= kFwKVEmpty0 && i < kFwTail0) count = 2;
+      if ((i >= kFwPFull0 && i < kFwOFull0) || (i >= kFwOEmpty0 && i < kFwUnitFull0)) count = 4;
+      if (i >= kFwUnitEmpty0 && i < kFwDrain0) count = Cfg::kReaders;
+      mbar_init(&bar[i], count);
     }
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&bar[kFwKVFull0 + s], 1);
-      mbar_init(&bar[kFwKVEmpty0 + s], 1);
-    }
-    mbar_init(&bar[kFwDrain], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -241,183 +341,156 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   WaitCtx ctx{abort_flag, p.timeout_ns};
-  const int first = blockIdx.x, step = gridDim.x;
+  uint64_t *unit_full = &bar[kFwUnitFull0], *unit_empty = &bar[kFwUnitEmpty0];
+  int4 ua, ub;
+  int k = 0;
+  bool ok = true;
   // a launch that joins the parts may start, and waits for them itself
   if (p.partial) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp >= 12) {
     regs_lower<Cfg::kOtherRegs>();
-    if (warp == 12 && lane == 0) {
-      // ---- TMA producer. Ring order: K_lo, then V_j, K_(j+1) in turn, the
-      // order in which the MMA thread uses them.
-      tma_prefetch_desc(&tm_Q);
-      tma_prefetch_desc(&tm_K);
-      tma_prefetch_desc(&tm_V);
-      const uint64_t pol_q = l2_policy_evict_first(), pol_kv = l2_policy_evict_last();
-      const uint32_t q_bytes = static_cast<uint32_t>(p.rows.Mt * p.rows.Gt * p.rows.St) * 128u * (D / kBoxCols);
-      int nq[2] = {0, 0}, g = 0, slot = 0, turn = 0;
-      bool ok = true;
-      auto load_q = [&](const FwdItem& it, int t) {
-        if (nq[t] > 0 && !mbar_wait(&bar[kFwQEmpty0 + t], (nq[t] - 1) & 1, ctx, 201)) return false;
-        const int tile = it.tile0 + t;
-        const int im = tile % p.rows.nm, u = tile / p.rows.nm;
-        mbar_arrive_expect_tx(&bar[kFwQFull0 + t], q_bytes);
+    if (warp == 12) {
+      if (elect_one()) {
+        // ---- TMA producer. Ring order: K_lo, then V_j, K_(j+1) in turn, the
+        // order in which the MMA issuers use them.
+        tma_prefetch_desc(&tm_Q);
+        tma_prefetch_desc(&tm_K);
+        tma_prefetch_desc(&tm_V);
+        const uint64_t pol_q = l2_policy_evict_first(), pol_kv = l2_policy_evict_last();
+        const uint32_t q_bytes = static_cast<uint32_t>(p.rows.Mt * p.rows.Gt * p.rows.St) * 128u * (D / kBoxCols);
+        int nq0 = 0, nq1 = 0, g = 0, slot = 0, turn = 0, tails = 0;
+        auto load_q = [&](const FwdItem& it, int t, int& n) {
+          if (n > 0 && !mbar_wait(&bar[kFwQEmpty0 + t], (n - 1) & 1, ctx, 201)) return false;
+          const int tile = it.tile0 + t;
+          const int im = tile % p.rows.nm, u = tile / p.rows.nm;
+          mbar_arrive_expect_tx(&bar[kFwQFull0 + t], q_bytes);
 #pragma unroll
-        for (int x = 0; x < D / kBoxCols; ++x)
-          tma_load_4d(smem + Cfg::kOffQ + t * Cfg::kTileBytes + x * kBoxBytes, &tm_Q, &bar[kFwQFull0 + t], x * kBoxCols,
-                      im * p.rows.Mt, it.hk * p.rows.G + (u % p.rows.ng) * p.rows.Gt,
-                      it.b * p.rows.S + (u / p.rows.ng) * p.rows.St, pol_q);
-        ++nq[t];
-        return true;
-      };
-      auto load_kv = [&](const CUtensorMap* tm, const FwdItem& it, int j) {
-        if (g >= kSlots && !mbar_wait(&bar[kFwKVEmpty0 + slot], (turn - 1) & 1, ctx, 202)) return false;
-        uint64_t* fb = &bar[kFwKVFull0 + slot];
-        uint8_t* dst = smem + Cfg::kOffKV + slot * Cfg::kTileBytes;
-        mbar_arrive_expect_tx(fb, Cfg::kTileBytes);
+          for (int x = 0; x < D / kBoxCols; ++x)
+            tma_load_4d(smem + Cfg::kOffQ + t * Cfg::kTileBytes + x * kBoxBytes, &tm_Q, &bar[kFwQFull0 + t], x * kBoxCols,
+                        im * p.rows.Mt, it.hk * p.rows.G + (u % p.rows.ng) * p.rows.Gt,
+                        it.b * p.rows.S + (u / p.rows.ng) * p.rows.St, pol_q);
+          ++n;
+          return true;
+        };
+        auto load_kv = [&](const CUtensorMap* tm, const FwdItem& it, int j, int full) {
+          if (g >= kSlots && !mbar_wait(&bar[kFwKVEmpty0 + slot], (turn - 1) & 1, ctx, 202)) return false;
+          uint64_t* fb = &bar[full + slot];
+          if (full == kFwTail0) tails |= 1 << slot;
+          uint8_t* dst = smem + Cfg::kOffKV + slot * Cfg::kTileBytes;
+          mbar_arrive_expect_tx(fb, Cfg::kTileBytes);
 #pragma unroll
-        for (int x = 0; x < D / kBoxCols; ++x)
-          tma_load_4d(dst + x * kBoxBytes, tm, fb, x * kBoxCols, j * kTile, it.hk, it.b, pol_kv);
-        ++g;
-        if (++slot == kSlots) {
-          slot = 0;
-          ++turn;
+          for (int x = 0; x < D / kBoxCols; ++x)
+            tma_load_4d(dst + x * kBoxBytes, tm, fb, x * kBoxCols, j * kTile, it.hk, it.b, pol_kv);
+          ++g;
+          if (++slot == kSlots) {
+            slot = 0;
+            ++turn;
+          }
+          return true;
+        };
+        while (get_unit<false>(ring, unit_full, unit_empty, k, ua, ub, ctx, 203, ok)) {
+          const FwdItem it = fwd_item(ua, ub);
+          if (it.lo == it.hi) continue;
+          ok = load_q(it, 0, nq0) && load_kv(&tm_K, it, it.lo, kFwKVFull0) && (!it.two || load_q(it, 1, nq1));
+          for (int j = it.lo; j < it.hi && ok; ++j)
+            ok = load_kv(&tm_V, it, j, j + 1 == it.hi && has_tail(it.n, it.hi) ? kFwTail0 : kFwKVFull0) &&
+                 (j + 1 == it.hi || load_kv(&tm_K, it, j + 1, kFwKVFull0));
         }
-        return true;
-      };
-      for (int t = first; t < p.items && ok; t += step) {
-        const FwdItem it = fwd_item(p, t);
-        if (it.lo == it.hi) continue;
-        ok = load_q(it, 0) && load_kv(&tm_K, it, it.lo) && (!it.two || load_q(it, 1));
-        for (int j = it.lo; j < it.hi && ok; ++j)
-          ok = load_kv(&tm_V, it, j) && (j + 1 == it.hi || load_kv(&tm_K, it, j + 1));
-      }
-      if (*abort_flag) {
-        for (int t = 0; t < 2; ++t)
-          if (nq[t] > 0) mbar_wait_drain(&bar[kFwQFull0 + t], (nq[t] - 1) & 1, p.timeout_ns);
-        for (int i = (g > kSlots ? g - kSlots : 0); i < g; ++i)
-          mbar_wait_drain(&bar[kFwKVFull0 + i % kSlots], (i / kSlots) & 1, p.timeout_ns);
-      }
-    } else if (warp == 13) {
-      // ---- MMA: lane 0 issues; the whole warp clears the V rows between the
-      // last valid key and the next multiple of 16 (the products' step), which
-      // the tensor core would multiply by p = 0 whatever they hold.
-      constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
-      constexpr uint32_t id_O = make_idesc_f16<kB>(kTile, D, false, true);
-      const uint32_t sQ = smem_u32(smem + Cfg::kOffQ), sKV = smem_u32(smem + Cfg::kOffKV);
-      // the walk over all (item, key tile) steps of this CTA
-      struct Walk {
-        int t, j;
-        FwdItem it;
-      };
-      auto seek = [&](Walk& w) {  // first step of the next item that has one
-        for (; w.t < p.items; w.t += step) {
-          w.it = fwd_item(p, w.t);
-          if (w.it.lo < w.it.hi) {
-            w.j = w.it.lo;
-            return true;
+        if (*abort_flag) {
+          // every copy in flight ends before the block does
+          if (nq0 > 0) mbar_wait_drain(&bar[kFwQFull0], (nq0 - 1) & 1, p.timeout_ns);
+          if (nq1 > 0) mbar_wait_drain(&bar[kFwQFull0 + 1], (nq1 - 1) & 1, p.timeout_ns);
+          for (int i = (g > kSlots ? g - kSlots : 0); i < g; ++i) {
+            mbar_wait_drain(&bar[kFwKVFull0 + i % kSlots], (i / kSlots) & 1, 1000000);
+            if (tails >> (i % kSlots) & 1)
+              for (int par = 0; par < 2; ++par) mbar_wait_drain(&bar[kFwTail0 + i % kSlots], par, 1000000);
           }
         }
-        return false;
-      };
-      Walk cur{first, 0, {}};
-      bool more = seek(cur), ok = true;
-      int g = 0, nq[2] = {0, 0}, np[2] = {0, 0}, no[2] = {0, 0};
-      auto issue_s = [&](int t, int slot) {
-        const uint64_t dq = make_sw128_desc(sQ + t * Cfg::kTileBytes, 16, 1024);
-        const uint64_t dk = make_sw128_desc(sKV + slot * Cfg::kTileBytes, 16, 1024);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * kBoxBytes + (k & 3) * 32;
-          umma_f16_ss(tmem + Cfg::kColS + 128 * t, desc_advance(dq, off), desc_advance(dk, off), id_S, k > 0 ? 1u : 0u);
-        }
-        umma_commit(&bar[kFwSFull0 + t]);
-      };
-      // S of step w, for each of its tiles in `which`
-      auto first_s = [&](const Walk& w, int t, int slot) {
-        if (w.j == w.it.lo) {
-          if (!mbar_wait(&bar[kFwQFull0 + t], nq[t] & 1, ctx, 211)) return false;
-          ++nq[t];
-        }
-        tc_fence_after();
-        issue_s(t, slot);
-        if (w.j + 1 == w.it.hi) umma_commit(&bar[kFwQEmpty0 + t]);
-        return true;
-      };
-      if (more && lane == 0) {
-        ok = mbar_wait(&bar[kFwKVFull0], 0, ctx, 210) && first_s(cur, 0, 0) && (!cur.it.two || first_s(cur, 1, 0));
-        if (ok) umma_commit(&bar[kFwKVEmpty0]);
       }
-      g = 1;
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      while (more && ok) {
-        Walk nxt = cur;
-        bool has_next = true;
-        if (++nxt.j == nxt.it.hi) {
-          nxt.t += step;
-          has_next = seek(nxt);
-        }
-        const int vslot = g % kSlots, vpar = (g / kSlots) & 1;
-        const int kslot = (g + 1) % kSlots, kpar = ((g + 1) / kSlots) & 1;
-        g += 2;
-        const int left = cur.it.n - cur.j * kTile;  // valid keys from this tile on
-        if (lane == 0) ok = mbar_wait(&bar[kFwKVFull0 + vslot], vpar, ctx, 212);
-        if (left < kTile && (left & 15) != 0) {
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (ok) {
-            uint8_t* v = smem + Cfg::kOffKV + vslot * Cfg::kTileBytes;
-            const int rows = 16 - (left & 15);
-            for (int i = lane; i < rows * (D / 8); i += 32) {
-              const int row = left + i / (D / 8), c = i % (D / 8);
-              *reinterpret_cast<uint4*>(v + (c >> 3) * kBoxBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-                  make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
+      __syncwarp();
+    } else if (warp == 14) {
+      if (elect_one()) feed_fwd(p, ring, unit_full, unit_empty, ctx);
+      __syncwarp();
+    } else {
+      // ---- MMA issuer of tile t: S_(j+1) behind PV_j, for each item in turn.
+      // The pipe takes only about a product ahead, so a thread for each tile
+      // keeps one tile's wait from holding up the other's products.
+      const int t = warp == 13 ? 0 : 1;
+      if (elect_one()) {
+        constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
+        constexpr uint32_t id_O = make_idesc_f16<kB>(kTile, D, false, true);
+        const uint32_t sKV = smem_u32(smem + Cfg::kOffKV);
+        const uint64_t dq = make_sw128_desc(smem_u32(smem + Cfg::kOffQ + t * Cfg::kTileBytes), 16, 1024);
+        const uint32_t tS = tmem + Cfg::kColS + 128 * t, tO = tmem + Cfg::kColO + D * t;
+        int slot = 0, turn = 0, nq = 0, np = 0;
+        auto advance = [&](int n) {
+          slot += n;
+          while (slot >= kSlots) {
+            slot -= kSlots;
+            turn ^= 1;
           }
-          __syncwarp();
-        }
-        if (lane == 0 && ok) {
-          const int steps = left >= kTile ? kTile / 16 : (left + 15) / 16;
-          const uint64_t dv = make_sw128_desc(sKV + vslot * Cfg::kTileBytes, kBoxBytes, 1024);
+        };
+        auto done_with = [&](bool alone) {
+          umma_commit(&bar[kFwKVEmpty0 + slot]);
+          if (alone) umma_commit(&bar[kFwKVEmpty0 + slot]);
+          advance(1);
+        };
+        while (get_unit<false>(ring, unit_full, unit_empty, k, ua, ub, ctx, 210 + 10 * t, ok)) {
+          const FwdItem it = fwd_item(ua, ub);
+          if (it.lo == it.hi) continue;
+          if (t == 1 && !it.two) {
+            advance(2 * (it.hi - it.lo));
+            continue;
+          }
+          ok = mbar_wait(&bar[kFwQFull0 + t], nq & 1, ctx, 211 + 10 * t);
+          for (int j = it.lo - 1; ok && j < it.hi; ++j) {
+            if (j >= it.lo) {  // O += p V_j
+              if (!(ok = mbar_wait(&bar[kFwKVFull0 + slot], turn, ctx, 212 + 10 * t))) break;
+              if (j == it.lo && nq > 0 && !(ok = mbar_wait(&bar[kFwOEmpty0 + t], (nq - 1) & 1, ctx, 213 + 10 * t))) break;
+              if (!(ok = mbar_wait(&bar[kFwPFull0 + t], np & 1, ctx, 214 + 10 * t))) break;
+              tc_fence_after();
+              const uint64_t dv = make_sw128_desc(sKV + slot * Cfg::kTileBytes, kBoxBytes, 1024);
+              const uint32_t keep = j > it.lo ? 1u : 0u;
+              const int left = it.n - j * kTile;
+              if (left >= kTile) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (ok && (t == 0 || cur.it.two)) {
-              if (cur.j == cur.it.lo) {
-                if (no[t] > 0) ok = mbar_wait(&bar[kFwOEmpty0 + t], (no[t] - 1) & 1, ctx, 213);
-                ++no[t];
-              }
-              if (ok) ok = mbar_wait(&bar[kFwPFull0 + t], np[t] & 1, ctx, 214);
-              ++np[t];
-              if (ok) {
+                for (int x = 0; x < 6; ++x)
+                  umma_f16_ts(tO, tS + x * 8, desc_advance(dv, x * 2048), id_O, x > 0 ? 1u : keep);
+                if (!(ok = mbar_wait(&bar[kFwPRest0 + t], np & 1, ctx, 215 + 10 * t))) break;
                 tc_fence_after();
-                const uint32_t tP = tmem + Cfg::kColS + 128 * t, tO = tmem + Cfg::kColO + D * t;
-                const uint32_t keep = cur.j > cur.it.lo ? 1u : 0u;
-                if (steps == kTile / 16) {
 #pragma unroll
-                  for (int k = 0; k < kTile / 16; ++k)
-                    umma_f16_ts(tO, tP + k * 8, desc_advance(dv, k * 2048), id_O, k > 0 ? 1u : keep);
-                } else {
-                  for (int k = 0; k < steps; ++k)
-                    umma_f16_ts(tO, tP + k * 8, desc_advance(dv, k * 2048), id_O, k > 0 ? 1u : keep);
-                }
-                if (cur.j + 1 == cur.it.hi) umma_commit(&bar[kFwOFull0 + t]);
+                for (int x = 6; x < 8; ++x) umma_f16_ts(tO, tS + x * 8, desc_advance(dv, x * 2048), id_O, 1u);
+              } else {
+                if (!(ok = mbar_wait(&bar[kFwPRest0 + t], np & 1, ctx, 215 + 10 * t))) break;
+                tc_fence_after();
+                for (int x = 0; x < (left + 15) / 16; ++x)
+                  umma_f16_ts(tO, tS + x * 8, desc_advance(dv, x * 2048), id_O, x > 0 ? 1u : keep);
               }
+              ++np;
+              done_with(!it.two);
+              if (j + 1 == it.hi) umma_commit(&bar[kFwOFull0 + t]);
             }
-            if (ok && t == (cur.it.two ? 1 : 0)) umma_commit(&bar[kFwKVEmpty0 + vslot]);
-            if (ok && has_next && (t == 0 || nxt.it.two)) {
-              if (t == 0) ok = mbar_wait(&bar[kFwKVFull0 + kslot], kpar, ctx, 215);
-              if (ok) ok = first_s(nxt, t, kslot);
-              if (ok && t == (nxt.it.two ? 1 : 0)) umma_commit(&bar[kFwKVEmpty0 + kslot]);
+            if (j + 1 < it.hi) {  // S = Q K_(j+1)^T
+              if (!(ok = mbar_wait(&bar[kFwKVFull0 + slot], turn, ctx, 216 + 10 * t))) break;
+              tc_fence_after();
+              const uint64_t dk = make_sw128_desc(sKV + slot * Cfg::kTileBytes, 16, 1024);
+#pragma unroll
+              for (int x = 0; x < D / 16; ++x) {
+                const uint32_t off = (x >> 2) * kBoxBytes + (x & 3) * 32;
+                umma_f16_ss(tS, desc_advance(dq, off), desc_advance(dk, off), id_S, x > 0 ? 1u : 0u);
+              }
+              umma_commit(&bar[kFwSFull0 + t]);
+              if (j + 2 == it.hi) umma_commit(&bar[kFwQEmpty0 + t]);
+              done_with(!it.two);
             }
           }
+          ++nq;
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        more = has_next;
-        cur = nxt;
-      }
-      if (!ok && lane == 0) {
-        umma_commit(&bar[kFwDrain]);
-        mbar_wait_drain(&bar[kFwDrain], 0, p.timeout_ns);
+        if (!ok) {
+          umma_commit(&bar[kFwDrain0 + t]);
+          mbar_wait_drain(&bar[kFwDrain0 + t], 0, p.timeout_ns);
+        }
       }
       __syncwarp();
     }
@@ -430,30 +503,38 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     const uint32_t tO = tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16);
     const float sl2 = p.scale * kLog2e;
     int ns = 0, nst = 0;
-    bool ok = true;
-    for (int i = first; i < p.items && ok; i += step) {
-      const FwdItem it = fwd_item(p, i);
+    while (get_unit<true>(ring, unit_full, unit_empty, k, ua, ub, ctx, 230, ok)) {
+      const FwdItem it = fwd_item(ua, ub);
       if (t == 1 && !it.two) continue;
       float m = 0.f;                                  // the row's reference, in powers of two
       float2 l0 = make_float2(0.f, 0.f), l1 = l0;     // its sum, in four shares
       for (int j = it.lo; j < it.hi; ++j, ++ns) {
-        if (!mbar_wait(&bar[kFwSFull0 + t], ns & 1, ctx, 220)) { ok = false; break; }
+        if (!mbar_wait(&bar[kFwSFull0 + t], ns & 1, ctx, 231)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
         uint32_t s[128];
-        tmem_load_64(tS, *reinterpret_cast<uint32_t(*)[64]>(s));
-        tmem_load_64(tS + 64, *reinterpret_cast<uint32_t(*)[64]>(s + 64));
+        tmem_load_64_start(tS, s);
+        tmem_load_64_wait(s);
+        tmem_load_64_start(tS + 64, s + 64);
         const int left = it.n - j * kTile;
         if (left < kTile) {
 #pragma unroll
-          for (int x = 0; x < 128; ++x)
+          for (int x = 0; x < 64; ++x)
             if (x >= left) s[x] = 0xff800000u;  // -inf
         }
         float mx[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) mx[x] = __uint_as_float(s[x]);
 #pragma unroll
-        for (int x = 4; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
+        for (int x = 4; x < 64; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
+        tmem_load_64_wait(s + 64);
+        if (left < kTile) {
+#pragma unroll
+          for (int x = 64; x < 128; ++x)
+            if (x >= left) s[x] = 0xff800000u;
+        }
+#pragma unroll
+        for (int x = 64; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2 - kBias;
         if (j == it.lo) {
           m = top == -INFINITY ? 0.f : top;
@@ -463,64 +544,73 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
           if (move) m = top;
           l0 = mul_f32x2(l0, make_float2(f, f));
           l1 = mul_f32x2(l1, make_float2(f, f));
+#pragma unroll 1
+          for (int x = 0; x < D / 16; ++x) {
+            uint32_t o[16];
+            tmem_load_16(tO + 16 * x, o);
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            uint32_t o[32];
-            tmem_load_32(tO + 32 * x, o);
-#pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(f * __uint_as_float(o[y]));
-            tmem_store_32(tO + 32 * x, o);
+            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(f * __uint_as_float(o[y]));
+            tmem_store_16(tO + 16 * x, o);
           }
           tmem_store_wait();
         }
         const float2 nm = make_float2(-m, -m), sc = make_float2(sl2, sl2);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t e[32];
-#pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const uint32_t* v = s + 64 * h + 2 * x;
-            float2 a = fma_f32x2(make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), sc, nm);
-            a.x = ex2_approx(a.x);
-            a.y = ex2_approx(a.y);
-            if (x & 1) l1 = add_f32x2(l1, a);
-            else l0 = add_f32x2(l0, a);
-            e[x] = Elem<T>::pack(a.x, a.y);
+        for (int h = 0; h < 4; ++h) {
+          uint32_t e[16];
+          if (left >= kTile) weights_32<T, false>(s + 32 * h, sc, nm, l0, l1, e);
+          else weights_32<T, true>(s + 32 * h, sc, nm, l0, l1, e);
+          __syncwarp();
+          tmem_store_16(tS + 16 * h, e);
+          if (h >= 2) {
+            tmem_store_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar[(h == 2 ? kFwPFull0 : kFwPRest0) + t]);
           }
-          tmem_store_32(tS + 32 * h, e);
         }
-        tmem_store_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar[kFwPFull0 + t]);
       }
-      if (!ok) break;
-      if (nst > 0 && !mbar_wait(&bar[kFwStEmpty0 + t], (nst - 1) & 1, ctx, 221)) { ok = false; break; }
+      if (!ok) continue;
+      if (nst > 0 && !mbar_wait(&bar[kFwStEmpty0 + t], (nst - 1) & 1, ctx, 232)) { ok = false; continue; }
       stat[128 * t + r] = make_float2(m, (l0.x + l0.y) + (l1.x + l1.y));
       ++nst;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[kFwStFull0 + t]);
     }
   } else {
-    // ---- epilogue: thread = row of each tile in turn
+    // ---- epilogue: thread = row of each tile in turn. It also clears the
+    // last V tile behind the last key, for the issuers that wait for it.
     regs_lower<Cfg::kOtherRegs>();
     const int r = threadIdx.x & 127;
-    int nst[2] = {0, 0}, no[2] = {0, 0};
-    bool ok = true;
+    int nst[2] = {0, 0}, no[2] = {0, 0}, g = 0;
     const int64_t all_rows = static_cast<int64_t>(p.B) * p.rows.S * p.Hkv * p.rows.G * p.rows.M;
-    for (int i = first; i < p.items && ok; i += step) {
-      const FwdItem it = fwd_item(p, i);
+    uint32_t tail_turns = 0;  // a bit for each slot
+    while (get_unit<true>(ring, unit_full, unit_empty, k, ua, ub, ctx, 240, ok)) {
+      const FwdItem it = fwd_item(ua, ub);
+      const bool keys = it.lo < it.hi;
+      if (keys) {
+        g += 2 * (it.hi - it.lo);
+        if (warp == 8 && has_tail(it.n, it.hi)) {
+          const int slot = (g - 1) % kSlots;
+          if (!mbar_wait(&bar[kFwTail0 + slot], tail_turns >> slot & 1, ctx, 241)) ok = false;
+          tail_turns ^= 1u << slot;
+          __syncwarp();
+          if (ok) clear_tail<D>(smem + Cfg::kOffKV + slot * Cfg::kTileBytes, it.n - (it.hi - 1) * kTile, lane);
+          __syncwarp();
+          if (ok && lane == 0) mbar_arrive(&bar[kFwKVFull0 + slot]);
+        }
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (t == 1 && !it.two) continue;
-        if (!mbar_wait(&bar[kFwStFull0 + t], nst[t] & 1, ctx, 230)) { ok = false; break; }
+        if (ok && !mbar_wait(&bar[kFwStFull0 + t], nst[t] & 1, ctx, 242)) ok = false;
+        if (!ok) break;
         ++nst[t];
         const float2 ml = stat[128 * t + r];
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[kFwStEmpty0 + t]);
-        const bool keys = it.lo < it.hi;
         if (keys) {
-          if (!mbar_wait(&bar[kFwOFull0 + t], no[t] & 1, ctx, 231)) { ok = false; break; }
+          if (!mbar_wait(&bar[kFwOFull0 + t], no[t] & 1, ctx, 243)) { ok = false; break; }
           ++no[t];
         }
         __syncwarp();
@@ -533,40 +623,29 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         const float lse = keys ? (ml.x + log2f(ml.y)) * kLn2 : -INFINITY;
         const int64_t row = (static_cast<int64_t>(b) * p.Hkv * p.rows.G + h) * p.rows.M + m;
         const uint32_t tO = tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16);
-        if (p.partial) {
-          if (real) p.part_lse[it.split * all_rows + row] = lse;
-          float* out = p.part_o + (it.split * all_rows + row) * D;
+        float* part = p.partial ? p.part_o + (it.split * all_rows + row) * D : nullptr;
+        uint8_t* out = p.partial ? nullptr : reinterpret_cast<uint8_t*>(p.O.at(b, h, m));
+        if (real) *(p.partial ? p.part_lse + it.split * all_rows + row : p.LSE + row) = lse;
+        if (!real) out = nullptr;
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            uint32_t o[32];
-            __syncwarp();
-            if (keys) {
-              tmem_load_32(tO + 32 * x, o);
-            } else {
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t o[32];
+          __syncwarp();
+          if (keys) {
+            tmem_load_32(tO + 32 * x, o);
+          } else {
 #pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = 0u;
-            }
+            for (int y = 0; y < 32; ++y) o[y] = 0u;
+          }
+          if (p.partial) {
             if (real) {
 #pragma unroll
               for (int y = 0; y < 8; ++y)
-                reinterpret_cast<float4*>(out + 32 * x)[y] =
+                reinterpret_cast<float4*>(part + 32 * x)[y] =
                     make_float4(inv * __uint_as_float(o[4 * y]), inv * __uint_as_float(o[4 * y + 1]),
                                 inv * __uint_as_float(o[4 * y + 2]), inv * __uint_as_float(o[4 * y + 3]));
             }
-          }
-        } else {
-          if (real) p.LSE[row] = lse;
-          uint8_t* out = real ? reinterpret_cast<uint8_t*>(p.O.at(b, h, m)) : nullptr;
-#pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            uint32_t o[32];
-            __syncwarp();
-            if (keys) {
-              tmem_load_32(tO + 32 * x, o);
-            } else {
-#pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = 0u;
-            }
+          } else {
             uint4 ch[4];
 #pragma unroll
             for (int y = 0; y < 4; ++y) ch[y] = pack8<T>(o + 8 * y, inv);
