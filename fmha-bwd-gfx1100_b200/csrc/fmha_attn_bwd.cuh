@@ -298,30 +298,17 @@ __device__ __forceinline__ void zero_rows(const View<T>& v, int b, int heads, in
   }
 }
 
-// One row's 32 columns: 16-bit, scaled, or fp32 into a partial-sum slot.
-__device__ __forceinline__ void store_part_32(float* out, const uint32_t (&v)[32]) {
-#pragma unroll
-  for (int y = 0; y < 8; ++y)
-    reinterpret_cast<uint4*>(out)[y] = make_uint4(v[4 * y], v[4 * y + 1], v[4 * y + 2], v[4 * y + 3]);
-}
-
 // This thread's row of D sums in TMEM, to a partial-sum slot or, scaled, to
 // its 16-bit output row (null: none).
 template <typename T, int D>
-__device__ __forceinline__ void store_sums(uint32_t taddr, uint8_t* out, float mul, float* part, int lane) {
-#pragma unroll
+__device__ __forceinline__ void store_sums(uint32_t taddr, T* out, float mul, float* part, int lane) {
+  uint8_t* row = part ? reinterpret_cast<uint8_t*>(part) : reinterpret_cast<uint8_t*>(out);
+  const float by = part ? 1.f : mul;
+#pragma unroll 1
   for (int x = 0; x < D / 32; ++x) {
     uint32_t v[32];
-    __syncwarp();
     tmem_load_32(taddr + 32 * x, v);
-    if (part) {
-      store_part_32(part + 32 * x, v);
-    } else {
-      uint4 ch[4];
-#pragma unroll
-      for (int y = 0; y < 4; ++y) ch[y] = pack8<T>(v + 8 * y, mul);
-      store_rows_anywhere<4>(ch, out ? out + 64 * x : nullptr, lane);
-    }
+    store_row_32(part != nullptr, row, x, v, by, lane, T());
   }
 }
 
@@ -346,12 +333,12 @@ struct DqCfg2 {
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 // Both kernels: warpgroups 0 and 1 form P and dS, 2 stores the sums, 3 holds
-// the TMA producer (warp 12), the MMA issuer (13), the scheduler (14) and the
-// warp that zeroes what has no keys (15). Registers: 2 * 128 * 184 + 2 * 128 *
+// the TMA producer (warp 12), two MMA issuers (13, 15) and the scheduler (14),
+// whose other lanes zero what has no keys. Registers: 2 * 128 * 184 + 2 * 128 *
 // 72, the 512 * 128 of the launch.
 constexpr int kBwdThreads = 512, kBwdComputeRegs = 184, kBwdOtherRegs = 72;
 static_assert(2 * kBwdComputeRegs + 2 * kBwdOtherRegs == 4 * 128, "register split");
-constexpr int kUnitReaders = 14;  // warps 0-13
+constexpr int kUnitReaders = 15;  // warps 0-13 and 15
 
 enum DqBar2 : int {
   kBqQFull0 = 0,    // + tile: Q and dO
@@ -366,32 +353,26 @@ enum DqBar2 : int {
   kBqDSFull0 = 26,  // + tile: dS written (4 warps)
   kBqAcc0 = 28,     // + tile: the unit's dQ is complete
   kBqAccEmpty0 = 30,// + tile: and read (4 warps)
-  kBqDrain = 32,
-  kBqUnitFull0 = 33,
-  kBqUnitEmpty0 = 37,
-  kNumBqBars = 41,
+  kBqDrain0 = 32,   // + tile
+  kBqUnitFull0 = 34,
+  kBqUnitEmpty0 = 38,
+  kBqTail0 = 42,    // + slot: a last K tile has landed, its rows behind the keys not yet cleared
+  kNumBqBars = 46,
 };
 
-// dS of one row from P (in `s`) and dP (TMEM), 16 bits each, over dP. Columns
-// at and past `left` do not count, whatever K and V held there.
-template <typename T, bool kTail>
-__device__ __forceinline__ void form_ds(const uint32_t (&s)[128], uint32_t tR, float mul, float nd, int left) {
+// Zeroes the dS (16-bit pairs in TMEM) of the keys of the last 16 that count
+// in part, at and past `left`; the products do not reach further.
+__device__ __forceinline__ void clear_ds(uint32_t taddr, int left) {
+  if ((left & 15) == 0) return;
+  uint32_t v[8];
+  const int c = left & ~15;
+  tmem_load_8(taddr + c / 2, v);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    uint32_t dp[16], e[8];
-    tmem_load_16(tR + 16 * q, dp);
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const int col = 16 * q + 2 * x;
-      float2 a = fma_f32x2(make_float2(__uint_as_float(dp[2 * x]), __uint_as_float(dp[2 * x + 1])),
-                           make_float2(mul, mul), make_float2(nd, nd));
-      a = mul_f32x2(a, make_float2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])));
-      if (kTail && col >= left) a.x = 0.f;
-      if (kTail && col + 1 >= left) a.y = 0.f;
-      e[x] = Elem<T>::pack(a.x, a.y);
-    }
-    tmem_store_8(tR + 8 * q, e);
+  for (int x = 0; x < 8; ++x) {
+    if (c + 2 * x >= left) v[x] = 0u;
+    else if (c + 2 * x + 1 >= left) v[x] &= 0xffffu;
   }
+  tmem_store_8(taddr + c / 2, v);
 }
 
 template <typename T, int D>
@@ -416,9 +397,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kNumBqBars; ++i) {
-      const bool four = (i >= kBqSRead0 && i < kBqXFull0) || (i >= kBqDSFull0 && i < kBqAcc0) ||
-                        (i >= kBqAccEmpty0 && i < kBqDrain);
-      mbar_init(&bar[i], i >= kBqUnitEmpty0 ? kUnitReaders : (four ? 4 : 1));
+      int count = 1;
+      if ((i >= kBqKEmpty0 && i < kBqVFull0) || (i >= kBqVEmpty0 && i < kBqSFull0)) count = 2;
+      if ((i >= kBqSRead0 && i < kBqXFull0) || (i >= kBqDSFull0 && i < kBqAcc0) || (i >= kBqAccEmpty0 && i < kBqDrain0))
+        count = 4;
+      if (i >= kBqUnitEmpty0 && i < kBqTail0) count = kUnitReaders;
+      mbar_init(&bar[i], count);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -444,211 +428,159 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (warp >= 12) {
     regs_lower<kBwdOtherRegs>();
     if (warp == 12) {
-      // ---- TMA producer (the whole warp walks the units, lane 0 loads)
-      if (lane == 0) {
+      // ---- TMA producer
+      if (elect_one()) {
         tma_prefetch_desc(&tm_Q);
         tma_prefetch_desc(&tm_K);
         tma_prefetch_desc(&tm_V);
         tma_prefetch_desc(&tm_dO);
-      }
-      const uint64_t pol_q = l2_policy_evict_first(), pol_kv = l2_policy_evict_last();
-      const uint32_t q_bytes = static_cast<uint32_t>(p.rows.Mt * p.rows.Gt) * 128u * (D / kBoxCols);
-      int nq0 = 0, nq1 = 0, nk = 0, nv = 0;
-      auto load_q = [&](int t, int& n) {
-        if (n > 0 && !mbar_wait(&bar[kBqQEmpty0 + t], (n - 1) & 1, ctx, 301)) return false;
-        const int tile = 2 * u.idx + t;
-        const int m0 = tile % p.rows.nm * p.rows.Mt, h0 = u.hk * p.rows.G + tile / p.rows.nm * p.rows.Gt;
-        mbar_arrive_expect_tx(&bar[kBqQFull0 + t], 2 * q_bytes);
+        const uint64_t pol_q = l2_policy_evict_first(), pol_kv = l2_policy_evict_last();
+        const uint32_t q_bytes = static_cast<uint32_t>(p.rows.Mt * p.rows.Gt) * 128u * (D / kBoxCols);
+        int nq[2] = {0, 0}, nk = 0, nv = 0, tails = 0;
+        auto load_k = [&](int j) {
+          const int s = nk % SK;
+          if (nk >= SK && !mbar_wait(&bar[kBqKEmpty0 + s], ((nk / SK) - 1) & 1, ctx, 302)) return false;
+          const bool tail = j + 1 == u.hi && has_tail(u.n, u.hi);
+          if (tail) tails |= 1 << s;
+          uint64_t* fb = &bar[(tail ? kBqTail0 : kBqKFull0) + s];
+          mbar_arrive_expect_tx(fb, Cfg::kTileBytes);
 #pragma unroll
-        for (int x = 0; x < D / kBoxCols; ++x) {
-          tma_load_4d(smem + Cfg::kOffQ + t * Cfg::kTileBytes + x * kBoxBytes, &tm_Q, &bar[kBqQFull0 + t], x * kBoxCols,
-                      m0, h0, u.b, pol_q);
-          tma_load_4d(smem + Cfg::kOffdO + t * Cfg::kTileBytes + x * kBoxBytes, &tm_dO, &bar[kBqQFull0 + t], x * kBoxCols,
-                      m0, h0, u.b, pol_q);
-        }
-        ++n;
-        return true;
-      };
-      auto load_k = [&](int j) {
-        const int s = nk % SK;
-        if (nk >= SK && !mbar_wait(&bar[kBqKEmpty0 + s], ((nk / SK) - 1) & 1, ctx, 302)) return false;
-        mbar_arrive_expect_tx(&bar[kBqKFull0 + s], Cfg::kTileBytes);
+          for (int x = 0; x < D / kBoxCols; ++x)
+            tma_load_4d(smem + Cfg::kOffK + s * Cfg::kTileBytes + x * kBoxBytes, &tm_K, fb, x * kBoxCols, j * kTile, u.hk,
+                        u.b, pol_kv);
+          ++nk;
+          return true;
+        };
+        while (take_unit<false>(ring, unit_full, unit_empty, k, u, ctx, 300, ok)) {
+#pragma unroll 1
+          for (int t = 0; t < 2 && ok; ++t) {
+            const int tile = 2 * u.idx + t;
+            if (tile >= q_tiles) break;
+            if (nq[t] > 0 && !(ok = mbar_wait(&bar[kBqQEmpty0 + t], (nq[t] - 1) & 1, ctx, 301))) break;
+            const int m0 = tile % p.rows.nm * p.rows.Mt, h0 = u.hk * p.rows.G + tile / p.rows.nm * p.rows.Gt;
+            mbar_arrive_expect_tx(&bar[kBqQFull0 + t], 2 * q_bytes);
 #pragma unroll
-        for (int x = 0; x < D / kBoxCols; ++x)
-          tma_load_4d(smem + Cfg::kOffK + s * Cfg::kTileBytes + x * kBoxBytes, &tm_K, &bar[kBqKFull0 + s], x * kBoxCols,
-                      j * kTile, u.hk, u.b, pol_kv);
-        ++nk;
-        return true;
-      };
-      auto load_v = [&](int j) {
-        const int s = nv % SV;
-        if (nv >= SV && !mbar_wait(&bar[kBqVEmpty0 + s], ((nv / SV) - 1) & 1, ctx, 303)) return false;
-        mbar_arrive_expect_tx(&bar[kBqVFull0 + s], Cfg::kTileBytes);
-#pragma unroll
-        for (int x = 0; x < D / kBoxCols; ++x)
-          tma_load_4d(smem + Cfg::kOffV + s * Cfg::kTileBytes + x * kBoxBytes, &tm_V, &bar[kBqVFull0 + s], x * kBoxCols,
-                      j * kTile, u.hk, u.b, pol_kv);
-        ++nv;
-        return true;
-      };
-      while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 300, ok)) {
-        if (lane == 0) {
-          ok = load_q(0, nq0) && load_k(u.lo) && (2 * u.idx + 1 >= q_tiles || load_q(1, nq1));
-          for (int j = u.lo; j < u.hi && ok; ++j) ok = load_v(j) && (j + 1 == u.hi || load_k(j + 1));
-        }
-      }
-      if (lane == 0 && *abort_flag) {
-        if (nq0 > 0) mbar_wait_drain(&bar[kBqQFull0], (nq0 - 1) & 1, p.timeout_ns);
-        if (nq1 > 0) mbar_wait_drain(&bar[kBqQFull0 + 1], (nq1 - 1) & 1, p.timeout_ns);
-        for (int i = (nk > SK ? nk - SK : 0); i < nk; ++i)
-          mbar_wait_drain(&bar[kBqKFull0 + i % SK], (i / SK) & 1, p.timeout_ns);
-        for (int i = (nv > SV ? nv - SV : 0); i < nv; ++i)
-          mbar_wait_drain(&bar[kBqVFull0 + i % SV], (i / SV) & 1, p.timeout_ns);
-      }
-      __syncwarp();
-    } else if (warp == 13) {
-      // ---- MMA: lane 0 issues, per step: dP0, [dQ1 of the step before, S1],
-      // dP1, [dQ0, S0 of the next step], so that each warpgroup forms P and dS
-      // while the tensor core works on the other tile. The whole warp clears
-      // the K rows between the last valid key and the next multiple of 16,
-      // which dQ would multiply by dS = 0 whatever they hold.
-      constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
-      constexpr uint32_t id_A = make_idesc_f16<kB>(kTile, D, false, true);
-      const uint32_t base = smem_u32(smem);
-      auto product = [&](uint32_t d, uint32_t a, uint32_t b) {  // A, B K-major over D
-        const uint64_t da = make_sw128_desc(a, 16, 1024), db = make_sw128_desc(b, 16, 1024);
-#pragma unroll
-        for (int x = 0; x < D / 16; ++x) {
-          const uint32_t off = (x >> 2) * kBoxBytes + (x & 3) * 32;
-          umma_f16_ss(d, desc_advance(da, off), desc_advance(db, off), id_S, x > 0 ? 1u : 0u);
-        }
-      };
-      int nq = 0, n0 = 0, n1 = 0, a0 = 0, a1 = 0;  // units; steps of tiles 0, 1; units of tiles 0, 1 (sums)
-      int nq1 = 0;
-      auto do_s = [&](int t, int g, bool opens) {
-        if (opens) {
-          if (!mbar_wait(&bar[kBqQFull0 + t], (t == 0 ? nq : nq1) & 1, ctx, 311)) return false;
-          if (t == 0) ++nq;
-          else ++nq1;
-        }
-        tc_fence_after();
-        product(tmem + 128 * t, base + Cfg::kOffQ + t * Cfg::kTileBytes, base + Cfg::kOffK + (g % SK) * Cfg::kTileBytes);
-        umma_commit(&bar[kBqSFull0 + t]);
-        return true;
-      };
-      auto do_dp = [&](int t, int n, int g, bool frees_v, bool closes) {
-        if (t == 0 && !mbar_wait(&bar[kBqVFull0 + g % SV], (g / SV) & 1, ctx, 312)) return false;
-        if (!mbar_wait(&bar[kBqSRead0 + t], n & 1, ctx, 313)) return false;
-        tc_fence_after();
-        product(tmem + 128 * t, base + Cfg::kOffdO + t * Cfg::kTileBytes, base + Cfg::kOffV + (g % SV) * Cfg::kTileBytes);
-        umma_commit(&bar[kBqXFull0 + t]);
-        if (frees_v) umma_commit(&bar[kBqVEmpty0 + g % SV]);
-        if (closes) umma_commit(&bar[kBqQEmpty0 + t]);
-        return true;
-      };
-      // `steps` of 16 keys; keep: not the unit's first step
-      auto do_dq = [&](int t, int n, int& na, int g, int steps, bool keep, bool frees_k, bool closes) {
-        if (!keep) {
-          if (na > 0 && !mbar_wait(&bar[kBqAccEmpty0 + t], (na - 1) & 1, ctx, 314)) return false;
-          ++na;
-        }
-        if (!mbar_wait(&bar[kBqDSFull0 + t], n & 1, ctx, 315)) return false;
-        tc_fence_after();
-        const uint64_t dk = make_sw128_desc(base + Cfg::kOffK + (g % SK) * Cfg::kTileBytes, kBoxBytes, 1024);
-        const uint32_t tA = tmem + 256 + D * t, tR = tmem + 128 * t;
-        if (steps == kTile / 16) {
-#pragma unroll
-          for (int x = 0; x < kTile / 16; ++x)
-            umma_f16_ts(tA, tR + x * 8, desc_advance(dk, x * 2048), id_A, x > 0 || keep ? 1u : 0u);
-        } else {
-          for (int x = 0; x < steps; ++x)
-            umma_f16_ts(tA, tR + x * 8, desc_advance(dk, x * 2048), id_A, x > 0 || keep ? 1u : 0u);
-        }
-        if (frees_k) umma_commit(&bar[kBqKEmpty0 + g % SK]);
-        if (closes) umma_commit(&bar[kBqAcc0 + t]);
-        return true;
-      };
-      // whole warp: K of step g (`left` keys from its tile on) has landed and
-      // its rows behind the last key are zero
-      auto have_k = [&](int g, int left) {
-        bool good = true;
-        if (lane == 0) good = mbar_wait(&bar[kBqKFull0 + g % SK], (g / SK) & 1, ctx, 310);
-        if (left < kTile && (left & 15) != 0) {
-          good = __shfl_sync(0xffffffffu, good, 0);
-          if (good) {
-            uint8_t* kt = smem + Cfg::kOffK + (g % SK) * Cfg::kTileBytes;
-            const int rows = 16 - (left & 15);
-            for (int i = lane; i < rows * (D / 8); i += 32) {
-              const int row = left + i / (D / 8), c = i % (D / 8);
-              *reinterpret_cast<uint4*>(kt + (c >> 3) * kBoxBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-                  make_uint4(0, 0, 0, 0);
+            for (int x = 0; x < D / kBoxCols; ++x) {
+              tma_load_4d(smem + Cfg::kOffQ + t * Cfg::kTileBytes + x * kBoxBytes, &tm_Q, &bar[kBqQFull0 + t],
+                          x * kBoxCols, m0, h0, u.b, pol_q);
+              tma_load_4d(smem + Cfg::kOffdO + t * Cfg::kTileBytes + x * kBoxBytes, &tm_dO, &bar[kBqQFull0 + t],
+                          x * kBoxCols, m0, h0, u.b, pol_q);
             }
-            fence_proxy_async_smem();
+            ++nq[t];
+            if (t == 0) ok = load_k(u.lo);
           }
-          __syncwarp();
+          for (int j = u.lo; j < u.hi && ok; ++j) {
+            const int s = nv % SV;
+            if (nv >= SV && !(ok = mbar_wait(&bar[kBqVEmpty0 + s], ((nv / SV) - 1) & 1, ctx, 303))) break;
+            mbar_arrive_expect_tx(&bar[kBqVFull0 + s], Cfg::kTileBytes);
+#pragma unroll
+            for (int x = 0; x < D / kBoxCols; ++x)
+              tma_load_4d(smem + Cfg::kOffV + s * Cfg::kTileBytes + x * kBoxBytes, &tm_V, &bar[kBqVFull0 + s],
+                          x * kBoxCols, j * kTile, u.hk, u.b, pol_kv);
+            ++nv;
+            if (j + 1 < u.hi) ok = load_k(j + 1);
+          }
         }
-        return good;
-      };
-      bool has = take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 309, ok);
-      int g = 0, j = u.lo;
-      bool two = 2 * u.idx + 1 < q_tiles;
-      // what dQ1 of the step before needs
-      bool prev = false, prev_keep = false, prev_closes = false;
-      int prev_steps = 0;
-      if (has) {
-        ok = have_k(0, u.n - j * kTile);
-        if (lane == 0 && ok) ok = do_s(0, 0, true);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-      }
-      while (has && ok) {
-        const int left = u.n - j * kTile, steps = left >= kTile ? kTile / 16 : (left + 15) / 16;
-        const bool keep = j > u.lo, closes = j + 1 == u.hi;
-        if (lane == 0) {
-          ok = do_dp(0, n0, g, !two, closes);
-          if (ok && prev) ok = do_dq(1, n1 - 1, a1, g - 1, prev_steps, prev_keep, true, prev_closes);
-          if (ok && two) ok = do_s(1, g, !keep) && do_dp(1, n1, g, true, closes);
-          if (ok) ok = do_dq(0, n0, a0, g, steps, keep, !two, closes);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        prev = two;
-        prev_keep = keep;
-        prev_closes = closes;
-        prev_steps = steps;
-        ++n0;
-        if (two) ++n1;
-        ++g;
-        ++j;
-        bool opens = false;
-        if (ok && closes) {
-          has = take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 309, ok);
-          j = u.lo;
-          two = 2 * u.idx + 1 < q_tiles;
-          opens = true;
-        }
-        if (ok && has) {
-          ok = have_k(g, u.n - j * kTile);
-          if (lane == 0 && ok) ok = do_s(0, g, opens);
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-        }
-      }
-      if (lane == 0) {
-        if (ok && prev) ok = do_dq(1, n1 - 1, a1, g - 1, prev_steps, prev_keep, true, prev_closes);
-        if (!ok) {
-          umma_commit(&bar[kBqDrain]);
-          mbar_wait_drain(&bar[kBqDrain], 0, p.timeout_ns);
+        if (*abort_flag) {  // every copy in flight ends before the block does
+          for (int t = 0; t < 2; ++t)
+            if (nq[t] > 0) mbar_wait_drain(&bar[kBqQFull0 + t], (nq[t] - 1) & 1, p.timeout_ns);
+          for (int i = (nk > SK ? nk - SK : 0); i < nk; ++i) {
+            mbar_wait_drain(&bar[kBqKFull0 + i % SK], (i / SK) & 1, 1000000);
+            if (tails >> (i % SK) & 1)
+              for (int par = 0; par < 2; ++par) mbar_wait_drain(&bar[kBqTail0 + i % SK], par, 1000000);
+          }
+          for (int i = (nv > SV ? nv - SV : 0); i < nv; ++i)
+            mbar_wait_drain(&bar[kBqVFull0 + i % SV], (i / SV) & 1, p.timeout_ns);
         }
       }
       __syncwarp();
     } else if (warp == 14) {
-      if (lane == 0) feed_units<T, true>(p, ring, unit_full, unit_empty, ctx, 305);
-      __syncwarp();
-    } else {
-      // ---- entries without keys: dQ = 0
-      if (p.lens)
+      if (lane == 0) {
+        feed_units<T, true>(p, ring, unit_full, unit_empty, ctx, 305);
+      } else if (p.lens) {
+        // the other lanes: entries without keys have dQ = 0
         for (int b = 0; b < p.B; ++b)
           if (valid_rows(p.lens, b, p.N) == 0)
-            zero_rows<T, D>(p.dQ, b, p.Hkv * p.rows.G, 0, p.rows.M, static_cast<int64_t>(blockIdx.x) * 32 + lane,
-                            32ll * gridDim.x);
+            zero_rows<T, D>(p.dQ, b, p.Hkv * p.rows.G, 0, p.rows.M, static_cast<int64_t>(blockIdx.x) * 31 + lane - 1,
+                            31ll * gridDim.x);
+      }
+      __syncwarp();
+    } else {
+      // ---- MMA issuer of tile t: per step dP, dQ, and S of the next step. A
+      // thread for each tile keeps one tile's wait from holding up the other's
+      // products.
+      const int t = warp == 13 ? 0 : 1;
+      if (elect_one()) {
+        constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
+        constexpr uint32_t id_A = make_idesc_f16<kB>(kTile, D, false, true);
+        const uint32_t sK = smem_u32(smem + Cfg::kOffK), sV = smem_u32(smem + Cfg::kOffV);
+        const uint64_t dq = make_sw128_desc(smem_u32(smem + Cfg::kOffQ + t * Cfg::kTileBytes), 16, 1024);
+        const uint64_t ddo = make_sw128_desc(smem_u32(smem + Cfg::kOffdO + t * Cfg::kTileBytes), 16, 1024);
+        const uint32_t tR = tmem + 128 * t, tA = tmem + 256 + D * t;
+        int g = 0, n = 0, nq = 0;  // steps of the CTA, steps and units of the tile
+        auto product = [&](uint64_t da, uint32_t b) {  // A, B K-major over D
+          const uint64_t db = make_sw128_desc(b, 16, 1024);
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x) {
+            const uint32_t off = (x >> 2) * kBoxBytes + (x & 3) * 32;
+            umma_f16_ss(tR, desc_advance(da, off), desc_advance(db, off), id_S, x > 0 ? 1u : 0u);
+          }
+        };
+        while (take_unit<false>(ring, unit_full, unit_empty, k, u, ctx, 309 + 10 * t, ok)) {
+          const bool alone = 2 * u.idx + 1 >= q_tiles;
+          if (t == 1 && alone) {
+            g += u.hi - u.lo;
+            continue;
+          }
+          if (!(ok = mbar_wait(&bar[kBqQFull0 + t], nq & 1, ctx, 311 + 10 * t))) break;
+          for (int j = u.lo - 1; j < u.hi; ++j) {
+            if (j >= u.lo) {
+              // dP_j over S_j once the warps have that in registers
+              if (!(ok = mbar_wait(&bar[kBqVFull0 + g % SV], (g / SV) & 1, ctx, 312 + 10 * t))) break;
+              if (!(ok = mbar_wait(&bar[kBqSRead0 + t], n & 1, ctx, 313 + 10 * t))) break;
+              tc_fence_after();
+              product(ddo, sV + (g % SV) * Cfg::kTileBytes);
+              umma_commit(&bar[kBqXFull0 + t]);
+              umma_commit(&bar[kBqVEmpty0 + g % SV]);
+              if (alone) umma_commit(&bar[kBqVEmpty0 + g % SV]);
+              if (j + 1 == u.hi) umma_commit(&bar[kBqQEmpty0 + t]);
+              // dQ += dS_j K_j
+              if (j == u.lo && nq > 0 && !(ok = mbar_wait(&bar[kBqAccEmpty0 + t], (nq - 1) & 1, ctx, 314 + 10 * t))) break;
+              if (!(ok = mbar_wait(&bar[kBqDSFull0 + t], n & 1, ctx, 315 + 10 * t))) break;
+              tc_fence_after();
+              const uint64_t dk = make_sw128_desc(sK + (g % SK) * Cfg::kTileBytes, kBoxBytes, 1024);
+              const uint32_t keep = j > u.lo ? 1u : 0u;
+              const int left = u.n - j * kTile;
+              if (left >= kTile) {
+#pragma unroll
+                for (int x = 0; x < kTile / 16; ++x)
+                  umma_f16_ts(tA, tR + x * 8, desc_advance(dk, x * 2048), id_A, x > 0 ? 1u : keep);
+              } else {
+                for (int x = 0; x < (left + 15) / 16; ++x)
+                  umma_f16_ts(tA, tR + x * 8, desc_advance(dk, x * 2048), id_A, x > 0 ? 1u : keep);
+              }
+              umma_commit(&bar[kBqKEmpty0 + g % SK]);
+              if (alone) umma_commit(&bar[kBqKEmpty0 + g % SK]);
+              if (j + 1 == u.hi) umma_commit(&bar[kBqAcc0 + t]);
+              ++n;
+              ++g;
+            }
+            if (j + 1 < u.hi) {  // S_(j+1)
+              if (!(ok = mbar_wait(&bar[kBqKFull0 + g % SK], (g / SK) & 1, ctx, 310 + 10 * t))) break;
+              tc_fence_after();
+              product(dq, sK + (g % SK) * Cfg::kTileBytes);
+              umma_commit(&bar[kBqSFull0 + t]);
+            }
+          }
+          if (!ok) break;
+          ++nq;
+        }
+        if (!ok) {
+          umma_commit(&bar[kBqDrain0 + t]);
+          mbar_wait_drain(&bar[kBqDrain0 + t], 0, p.timeout_ns);
+        }
+      }
+      __syncwarp();
     }
   } else if (warp < 8) {
     // ---- P and dS: warpgroup t owns tile t, thread = row (TMEM lane)
@@ -669,24 +601,50 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         __syncwarp();
         tc_fence_after();
         uint32_t s[128];
-        tmem_load_64(tR, *reinterpret_cast<uint32_t(*)[64]>(s));
-        tmem_load_64(tR + 64, *reinterpret_cast<uint32_t(*)[64]>(s + 64));
+        auto weights = [&](uint32_t* v) {  // P of 64 columns, every fourth pair by polynomial
+#pragma unroll
+          for (int x = 0; x < 64; x += 2) {
+            float2 a = fma_f32x2(make_float2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])), make_float2(sl2, sl2),
+                                 make_float2(nl, nl));
+            if ((x & 7) == 6) {
+              a = ex2_poly(a);
+            } else {
+              a.x = ex2_approx(a.x);
+              a.y = ex2_approx(a.y);
+            }
+            v[x] = __float_as_uint(a.x);
+            v[x + 1] = __float_as_uint(a.y);
+          }
+        };
+        tmem_load_64_start(tR, s);
+        tmem_load_64_wait(s);
+        tmem_load_64_start(tR + 64, s + 64);
+        weights(s);
+        tmem_load_64_wait(s + 64);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[kBqSRead0 + t]);
-#pragma unroll
-        for (int x = 0; x < 128; x += 2) {
-          const float2 a = fma_f32x2(make_float2(__uint_as_float(s[x]), __uint_as_float(s[x + 1])),
-                                     make_float2(sl2, sl2), make_float2(nl, nl));
-          s[x] = __float_as_uint(ex2_approx(a.x));
-          s[x + 1] = __float_as_uint(ex2_approx(a.y));
-        }
+        weights(s + 64);
         if (!mbar_wait(&bar[kBqXFull0 + t], ns & 1, ctx, 321)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
-        const int left = u.n - j * kTile;
-        if (left >= kTile) form_ds<T, false>(s, tR, ds_mul, nd, left);
-        else form_ds<T, true>(s, tR, ds_mul, nd, left);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          uint32_t dp[16], e[8];
+          tmem_load_16(tR + 16 * q, dp);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float2 a = fma_f32x2(make_float2(__uint_as_float(dp[2 * x]), __uint_as_float(dp[2 * x + 1])),
+                                       make_float2(ds_mul, ds_mul), make_float2(nd, nd));
+            const float2 d = mul_f32x2(a, make_float2(__uint_as_float(s[16 * q + 2 * x]), __uint_as_float(s[16 * q + 2 * x + 1])));
+            e[x] = Elem<T>::pack(d.x, d.y);
+          }
+          tmem_store_8(tR + 8 * q, e);
+        }
+        if (u.n - j * kTile < kTile) {
+          tmem_store_wait();
+          clear_ds(tR, u.n - j * kTile);
+        }
         tmem_store_wait();
         tc_fence_before();
         __syncwarp();
@@ -694,23 +652,37 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     }
   } else {
-    // ---- dQ: thread = row of each tile in turn
+    // ---- dQ: thread = row of each tile in turn; warp 8 also clears the last
+    // K tile behind the last key, for the issuers that wait for it
     regs_lower<kBwdOtherRegs>();
     const int r = threadIdx.x & 127;
     const float out_mul = p.scale * pow2(-ds_exponent<T, D>(p, lane));
-    int na[2] = {0, 0};
+    int na0 = 0, na1 = 0, g = 0;
+    uint32_t tail_turns = 0;
     while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 329, ok)) {
-#pragma unroll
+      g += u.hi - u.lo;
+      if (warp == 8 && has_tail(u.n, u.hi)) {
+        const int slot = (g - 1) % SK;
+        if (!mbar_wait(&bar[kBqTail0 + slot], tail_turns >> slot & 1, ctx, 331)) ok = false;
+        tail_turns ^= 1u << slot;
+        __syncwarp();
+        if (ok) clear_tail<D>(smem + Cfg::kOffK + slot * Cfg::kTileBytes, u.n - (u.hi - 1) * kTile, lane);
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(&bar[kBqKFull0 + slot]);
+      }
+#pragma unroll 1
       for (int t = 0; t < 2; ++t) {
         const int tile = 2 * u.idx + t;
         if (tile >= q_tiles) continue;
-        if (!mbar_wait(&bar[kBqAcc0 + t], na[t] & 1, ctx, 330)) { ok = false; break; }
-        ++na[t];
+        if (ok && !mbar_wait(&bar[kBqAcc0 + t], (t == 0 ? na0 : na1) & 1, ctx, 330)) ok = false;
+        if (!ok) break;
+        if (t == 0) ++na0;
+        else ++na1;
         __syncwarp();
         tc_fence_after();
         int m, g, s;
         const bool real = p.rows.row(tile, r, m, g, s);
-        uint8_t* out = real ? reinterpret_cast<uint8_t*>(p.dQ.at(u.b, u.hk * p.rows.G + g, m)) : nullptr;
+        T* out = real ? p.dQ.at(u.b, u.hk * p.rows.G + g, m) : nullptr;
         store_sums<T, D>(tmem + 256 + D * t + (static_cast<uint32_t>(r & 96) << 16), out, out_mul,
                          u.slot < 0 ? nullptr : p.part + ((static_cast<int64_t>(u.slot) * 2 + t) * kTile + r) * D, lane);
         tc_fence_before();
@@ -734,8 +706,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // stream. Keys lie on the TMEM lanes. Per row tile:
 //   S^T = K Q^T -> TMEM;  P^T = 2^(S^T scale log2e - lse2), 16-bit, over S^T;
 //   dV += P^T dO;  dP^T = V dO^T -> TMEM;  dS^T, 16-bit, over dP^T;  dK += dS^T Q
-// issued as dV, S^T of the next tile, dK, dP^T of the next tile: the warps
-// form dS^T during dV and S^T, and the next P^T during dK and dP^T.
+// The warps form dS^T during dV and S^T of the next tile, and its P^T during
+// dK and the next dP^T.
 //
 // Shared memory (D = 128): K, V 64 KB, Q x2, dO x2 128 KB, lse2 and delta.
 // TMEM: S^T [0, 128), dP^T [128, 256), dV, dK behind. Warps 0-7 form P and dS:
@@ -767,10 +739,10 @@ enum DkvBar2 : int {
   kBkDSFull = 13,  // 8 warps
   kBkAcc = 14,
   kBkAccEmpty = 15, // 4 warps
-  kBkDrain = 16,
-  kBkUnitFull0 = 17,
-  kBkUnitEmpty0 = 21,
-  kNumBkBars = 25,
+  kBkDrain0 = 16,   // + issuer
+  kBkUnitFull0 = 18,
+  kBkUnitEmpty0 = 22,
+  kNumBkBars = 26,
 };
 
 template <typename T, int D>
@@ -795,7 +767,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kNumBkBars; ++i)
-      mbar_init(&bar[i], i == kBkPFull || i == kBkDSFull ? 8 : (i == kBkAccEmpty ? 4 : (i >= kBkUnitEmpty0 ? kUnitReaders : 1)));
+      {
+      int count = 1;
+      if (i == kBkKVEmpty || i == kBkOEmpty0 || i == kBkOEmpty0 + 1 || i == kBkAcc) count = 2;
+      if (i == kBkPFull || i == kBkDSFull) count = 8;
+      if (i == kBkAccEmpty) count = 4;
+      if (i >= kBkUnitEmpty0) count = kUnitReaders;
+      mbar_init(&bar[i], count);
+    }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -827,34 +806,30 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     regs_lower<kBwdOtherRegs>();
     if (warp == 12) {
       // ---- TMA producer
-      if (lane == 0) {
+      if (elect_one()) {
         tma_prefetch_desc(&tm_Q);
         tma_prefetch_desc(&tm_K);
         tma_prefetch_desc(&tm_V);
         tma_prefetch_desc(&tm_dO);
-      }
-      const uint64_t pol_q = l2_policy_evict_last(), pol_kv = l2_policy_evict_first();
-      const uint32_t q_bytes = static_cast<uint32_t>(box_rows) * 128u * (D / kBoxCols);
-      int nu = 0, n = 0, no = 0;
-      while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 400, ok)) {
-        if (lane == 0) {
-          ok = nu == 0 || mbar_wait(&bar[kBkKVEmpty], (nu - 1) & 1, ctx, 401);
-          if (ok) {
-            mbar_arrive_expect_tx(&bar[kBkKV], 2 * Cfg::kTileBytes);
+        const uint64_t pol_q = l2_policy_evict_last(), pol_kv = l2_policy_evict_first();
+        const uint32_t q_bytes = static_cast<uint32_t>(box_rows) * 128u * (D / kBoxCols);
+        int nu = 0, n = 0, no = 0;
+        while (take_unit<false>(ring, unit_full, unit_empty, k, u, ctx, 400, ok)) {
+          if (nu > 0 && !(ok = mbar_wait(&bar[kBkKVEmpty], (nu - 1) & 1, ctx, 401))) break;
+          mbar_arrive_expect_tx(&bar[kBkKV], 2 * Cfg::kTileBytes);
 #pragma unroll
-            for (int x = 0; x < D / kBoxCols; ++x) {
-              tma_load_4d(smem + Cfg::kOffK + x * kBoxBytes, &tm_K, &bar[kBkKV], x * kBoxCols, u.idx * kTile, u.hk, u.b,
-                          pol_kv);
-              tma_load_4d(smem + Cfg::kOffV + x * kBoxBytes, &tm_V, &bar[kBkKV], x * kBoxCols, u.idx * kTile, u.hk, u.b,
-                          pol_kv);
-            }
-            ++nu;
+          for (int x = 0; x < D / kBoxCols; ++x) {
+            tma_load_4d(smem + Cfg::kOffK + x * kBoxBytes, &tm_K, &bar[kBkKV], x * kBoxCols, u.idx * kTile, u.hk, u.b,
+                        pol_kv);
+            tma_load_4d(smem + Cfg::kOffV + x * kBoxBytes, &tm_V, &bar[kBkKV], x * kBoxCols, u.idx * kTile, u.hk, u.b,
+                        pol_kv);
           }
-          for (int i = u.lo; i < u.hi && ok; ++i) {
+          ++nu;
+          for (int i = u.lo; i < u.hi; ++i) {
             const int s = n & 1;
             const int m0 = i % p.rows.nm * p.rows.Mt, h0 = u.hk * p.rows.G + i / p.rows.nm * p.rows.Gt;
             const int64_t row = ((static_cast<int64_t>(u.b) * p.Hkv + u.hk) * q_tiles + i) * kTile;
-            if (n >= 2 && !mbar_wait(&bar[kBkQEmpty0 + s], ((n >> 1) - 1) & 1, ctx, 402)) { ok = false; break; }
+            if (n >= 2 && !(ok = mbar_wait(&bar[kBkQEmpty0 + s], ((n >> 1) - 1) & 1, ctx, 402))) break;
             mbar_arrive_expect_tx(&bar[kBkQFull0 + s], q_bytes + 2 * kTile * 4);
 #pragma unroll
             for (int x = 0; x < D / kBoxCols; ++x)
@@ -863,7 +838,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             bulk_load(smem + Cfg::kOffL + s * 2 * kTile * 4, p.lse2 + row, kTile * 4, &bar[kBkQFull0 + s]);
             bulk_load(smem + Cfg::kOffL + (s * 2 + 1) * kTile * 4, p.delta + row, kTile * 4, &bar[kBkQFull0 + s]);
             ++n;
-            if (no >= 2 && !mbar_wait(&bar[kBkOEmpty0 + s], ((no >> 1) - 1) & 1, ctx, 403)) { ok = false; break; }
+            if (no >= 2 && !(ok = mbar_wait(&bar[kBkOEmpty0 + s], ((no >> 1) - 1) & 1, ctx, 403))) break;
             mbar_arrive_expect_tx(&bar[kBkOFull0 + s], q_bytes);
 #pragma unroll
             for (int x = 0; x < D / kBoxCols; ++x)
@@ -871,103 +846,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                           x * kBoxCols, m0, h0, u.b, pol_q);
             ++no;
           }
+          if (!ok) break;
         }
-      }
-      if (lane == 0 && *abort_flag) {
-        if (nu > 0) mbar_wait_drain(&bar[kBkKV], (nu - 1) & 1, p.timeout_ns);
-        for (int i = (n > 2 ? n - 2 : 0); i < n; ++i)
-          mbar_wait_drain(&bar[kBkQFull0 + (i & 1)], (i >> 1) & 1, p.timeout_ns);
-        for (int i = (no > 2 ? no - 2 : 0); i < no; ++i)
-          mbar_wait_drain(&bar[kBkOFull0 + (i & 1)], (i >> 1) & 1, p.timeout_ns);
-      }
-      __syncwarp();
-    } else if (warp == 13) {
-      // ---- MMA (the whole warp walks the units, lane 0 issues)
-      constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
-      constexpr uint32_t id_A = make_idesc_f16<kB>(kTile, D, false, true);
-      const uint32_t base = smem_u32(smem);
-      auto product = [&](uint32_t d, uint32_t a, uint32_t b) {
-        const uint64_t da = make_sw128_desc(a, 16, 1024), db = make_sw128_desc(b, 16, 1024);
-#pragma unroll
-        for (int x = 0; x < D / 16; ++x) {
-          const uint32_t off = (x >> 2) * kBoxBytes + (x & 3) * 32;
-          umma_f16_ss(d, desc_advance(da, off), desc_advance(db, off), id_S, x > 0 ? 1u : 0u);
+        if (*abort_flag) {  // every copy in flight ends before the block does
+          if (nu > 0) mbar_wait_drain(&bar[kBkKV], (nu - 1) & 1, p.timeout_ns);
+          for (int i = (n > 2 ? n - 2 : 0); i < n; ++i)
+            mbar_wait_drain(&bar[kBkQFull0 + (i & 1)], (i >> 1) & 1, p.timeout_ns);
+          for (int i = (no > 2 ? no - 2 : 0); i < no; ++i)
+            mbar_wait_drain(&bar[kBkOFull0 + (i & 1)], (i >> 1) & 1, p.timeout_ns);
         }
-      };
-      auto accumulate = [&](uint32_t d, uint32_t a, uint32_t b, bool keep) {
-        const uint64_t db = make_sw128_desc(b, kBoxBytes, 1024);
-#pragma unroll
-        for (int x = 0; x < kTile / 16; ++x)
-          umma_f16_ts(d, a + (x >> 2) * 64 + (x & 3) * 8, desc_advance(db, x * 2048), id_A, x > 0 || keep ? 1u : 0u);
-      };
-      int nu = 0;
-      auto do_s = [&](int n, bool opens) {
-        if (opens) {
-          if (!mbar_wait(&bar[kBkKV], nu & 1, ctx, 410)) return false;
-          ++nu;
-        }
-        if (!mbar_wait(&bar[kBkQFull0 + (n & 1)], (n >> 1) & 1, ctx, 411)) return false;
-        tc_fence_after();
-        product(tmem + Cfg::kColS, base + Cfg::kOffK, base + Cfg::kOffQ + (n & 1) * Cfg::kTileBytes);
-        umma_commit(&bar[kBkSFull]);
-        return true;
-      };
-      auto do_dp = [&](int n, bool closes) {
-        if (!mbar_wait(&bar[kBkOFull0 + (n & 1)], (n >> 1) & 1, ctx, 412)) return false;
-        tc_fence_after();
-        product(tmem + Cfg::kColX, base + Cfg::kOffV, base + Cfg::kOffdO + (n & 1) * Cfg::kTileBytes);
-        umma_commit(&bar[kBkXFull]);
-        if (closes) umma_commit(&bar[kBkKVEmpty]);
-        return true;
-      };
-      bool has = take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 409, ok);
-      int n = 0, i = u.lo, lo = u.lo, hi = u.hi;
-      if (has && lane == 0) ok = do_s(0, true) && do_dp(0, lo + 1 == hi);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      while (has && ok) {
-        const bool keep = i > lo, closes = i + 1 == hi;
-        bool more = true;
-        int i1 = i + 1;
-        if (closes) {
-          more = take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 409, ok);
-          i1 = u.lo;
-        }
-        if (lane == 0 && ok) {
-          do {
-            // the sums of the unit before have been read
-            if (!keep && nu > 1 && !(ok = mbar_wait(&bar[kBkAccEmpty], (nu - 2) & 1, ctx, 413))) break;
-            if (!(ok = mbar_wait(&bar[kBkPFull], n & 1, ctx, 414))) break;
-            tc_fence_after();
-            accumulate(tmem + Cfg::kColdV, tmem + Cfg::kColS, base + Cfg::kOffdO + (n & 1) * Cfg::kTileBytes, keep);
-            umma_commit(&bar[kBkOEmpty0 + (n & 1)]);
-            if (more && !(ok = do_s(n + 1, closes))) break;
-            if (!(ok = mbar_wait(&bar[kBkDSFull], n & 1, ctx, 415))) break;
-            tc_fence_after();
-            accumulate(tmem + Cfg::kColdK, tmem + Cfg::kColX, base + Cfg::kOffQ + (n & 1) * Cfg::kTileBytes, keep);
-            umma_commit(&bar[kBkQEmpty0 + (n & 1)]);
-            if (closes) umma_commit(&bar[kBkAcc]);
-            if (more && !(ok = do_dp(n + 1, i1 + 1 == u.hi))) break;
-          } while (false);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        lo = u.lo;
-        hi = u.hi;
-        i = i1;
-        has = more;
-        ++n;
-      }
-      if (!ok && lane == 0) {
-        umma_commit(&bar[kBkDrain]);
-        mbar_wait_drain(&bar[kBkDrain], 0, p.timeout_ns);
       }
       __syncwarp();
     } else if (warp == 14) {
-      if (lane == 0) feed_units<T, false>(p, ring, unit_full, unit_empty, ctx, 405);
-      __syncwarp();
-    } else {
-      // ---- key tiles without a valid key: dK = dV = 0
-      const int64_t thread = static_cast<int64_t>(blockIdx.x) * 32 + lane, threads = 32ll * gridDim.x;
-      if (p.lens)
+      if (lane == 0) {
+        feed_units<T, false>(p, ring, unit_full, unit_empty, ctx, 405);
+      } else if (p.lens) {
+        // the other lanes: key tiles without a valid key have dK = dV = 0
+        const int64_t thread = static_cast<int64_t>(blockIdx.x) * 31 + lane - 1, threads = 31ll * gridDim.x;
         for (int b = 0; b < p.B; ++b) {
           const int from = (valid_rows(p.lens, b, p.N) + kTile - 1) / kTile * kTile;
           if (from < p.N) {
@@ -975,6 +870,64 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             zero_rows<T, D>(p.dV, b, p.Hkv, from, p.N, thread, threads);
           }
         }
+      }
+      __syncwarp();
+    } else {
+      // ---- MMA issuers: warp 13 dV and S^T of the next row tile (TMEM S, P),
+      // warp 15 dK and dP^T of the next (TMEM X), so that neither chain's
+      // waits hold up the other's products.
+      const int w = warp == 13 ? 0 : 1;
+      if (elect_one()) {
+        constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
+        constexpr uint32_t id_A = make_idesc_f16<kB>(kTile, D, false, true);
+        const uint32_t base = smem_u32(smem);
+        const uint64_t da = make_sw128_desc(base + (w == 0 ? Cfg::kOffK : Cfg::kOffV), 16, 1024);  // K or V
+        const uint32_t first = base + (w == 0 ? Cfg::kOffQ : Cfg::kOffdO);   // Q or dO slots: S^T, dP^T
+        const uint32_t second = base + (w == 0 ? Cfg::kOffdO : Cfg::kOffQ);  // dO or Q slots: dV, dK
+        const uint32_t tR = tmem + (w == 0 ? Cfg::kColS : Cfg::kColX), tA = tmem + (w == 0 ? Cfg::kColdV : Cfg::kColdK);
+        uint64_t* landed = &bar[w == 0 ? kBkQFull0 : kBkOFull0];
+        uint64_t* formed = &bar[w == 0 ? kBkPFull : kBkDSFull];
+        int n = 0, nu = 0;
+        while (take_unit<false>(ring, unit_full, unit_empty, k, u, ctx, 409 + 10 * w, ok)) {
+          if (!(ok = mbar_wait(&bar[kBkKV], nu & 1, ctx, 410 + 10 * w))) break;
+          for (int i = u.lo - 1; i < u.hi; ++i) {
+            if (i >= u.lo) {
+              if (i == u.lo && nu > 0 && !(ok = mbar_wait(&bar[kBkAccEmpty], (nu - 1) & 1, ctx, 413 + 10 * w))) break;
+              if (!(ok = mbar_wait(formed, n & 1, ctx, 414 + 10 * w))) break;
+              tc_fence_after();
+              const uint64_t db = make_sw128_desc(second + (n & 1) * Cfg::kTileBytes, kBoxBytes, 1024);
+#pragma unroll
+              for (int x = 0; x < kTile / 16; ++x)
+                umma_f16_ts(tA, tR + (x >> 2) * 64 + (x & 3) * 8, desc_advance(db, x * 2048), id_A,
+                            x > 0 || i > u.lo ? 1u : 0u);
+              umma_commit(&bar[(w == 0 ? kBkOEmpty0 : kBkQEmpty0) + (n & 1)]);
+              if (i + 1 == u.hi) umma_commit(&bar[kBkAcc]);
+              ++n;
+            }
+            if (i + 1 < u.hi) {
+              if (!(ok = mbar_wait(landed + (n & 1), (n >> 1) & 1, ctx, 411 + 10 * w))) break;
+              tc_fence_after();
+              const uint64_t db = make_sw128_desc(first + (n & 1) * Cfg::kTileBytes, 16, 1024);
+#pragma unroll
+              for (int x = 0; x < D / 16; ++x) {
+                const uint32_t off = (x >> 2) * kBoxBytes + (x & 3) * 32;
+                umma_f16_ss(tR, desc_advance(da, off), desc_advance(db, off), id_S, x > 0 ? 1u : 0u);
+              }
+              umma_commit(&bar[w == 0 ? kBkSFull : kBkXFull]);
+              // dO has two readers that do not wait for one another; Q's second, dK, waits for its first
+              if (w == 1) umma_commit(&bar[kBkOEmpty0 + (n & 1)]);
+              if (i + 2 == u.hi) umma_commit(&bar[kBkKVEmpty]);
+            }
+          }
+          if (!ok) break;
+          ++nu;
+        }
+        if (!ok) {
+          umma_commit(&bar[kBkDrain0 + w]);
+          mbar_wait_drain(&bar[kBkDrain0 + w], 0, p.timeout_ns);
+        }
+      }
+      __syncwarp();
     }
   } else if (warp < 8) {
     // ---- P^T and dS^T
@@ -1006,8 +959,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                                make_float2(sl2, sl2), make_float2(kPBias - l.z, kPBias - l.w));
           a.x = ex2_approx(a.x);
           a.y = ex2_approx(a.y);
-          b.x = ex2_approx(b.x);
-          b.y = ex2_approx(b.y);
+          if (x & 1) {
+            b = ex2_poly(b);
+          } else {
+            b.x = ex2_approx(b.x);
+            b.y = ex2_approx(b.y);
+          }
           s[4 * x] = __float_as_uint(a.x);
           s[4 * x + 1] = __float_as_uint(a.y);
           s[4 * x + 2] = __float_as_uint(b.x);
@@ -1075,11 +1032,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       __syncwarp();
       tc_fence_after();
       const int key = u.idx * kTile + r;
-#pragma unroll
+#pragma unroll 1
       for (int which = 0; which < 2; ++which) {
         const View<T>& v = which == 0 ? p.dV : p.dK;
         store_sums<T, D>(tmem + (which == 0 ? Cfg::kColdV : Cfg::kColdK) + lanes,
-                         key < p.N ? reinterpret_cast<uint8_t*>(v.at(u.b, u.hk, key)) : nullptr,
+                         key < p.N ? v.at(u.b, u.hk, key) : nullptr,
                          which == 0 ? dv_mul : dk_mul,
                          u.slot < 0 ? nullptr : p.part + ((static_cast<int64_t>(u.slot) * 2 + which) * kTile + r) * D, lane);
       }

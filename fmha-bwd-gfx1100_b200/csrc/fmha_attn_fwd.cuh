@@ -280,15 +280,55 @@ __device__ __forceinline__ uint4 pack8(const uint32_t* a, float mul) {
                     Elem<T>::pack(mul * __uint_as_float(a[6]), mul * __uint_as_float(a[7])));
 }
 
-// 32 weights of a row: p = 2^(s sl2 - m), every fourth pair by polynomial
-// (with kTail, where s holds -inf, none), summed into l and packed.
-template <typename T, bool kTail>
+// Columns [32 x, 32 x + 32) of each lane's row, times `mul`, as fp32 or as
+// 16-bit with the warp's rows transposed for whole segments a store.
+template <typename T>
+__device__ __forceinline__ void store_row_32(bool fp32, uint8_t* row, int x, uint32_t (&v)[32], float mul, int lane, T) {
+  if (fp32) {
+    if (row) {
+#pragma unroll
+      for (int y = 0; y < 8; ++y)
+        reinterpret_cast<float4*>(row + 128 * x)[y] =
+            make_float4(mul * __uint_as_float(v[4 * y]), mul * __uint_as_float(v[4 * y + 1]),
+                        mul * __uint_as_float(v[4 * y + 2]), mul * __uint_as_float(v[4 * y + 3]));
+    }
+    __syncwarp();
+  } else {
+    uint4 ch[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) ch[y] = pack8<T>(v + 8 * y, mul);
+    store_rows_anywhere<4>(ch, row ? row + 64 * x : nullptr, lane);
+  }
+}
+
+// The instruction caches hold little next to these kernels' unrolled loops, and
+// straight-line code that runs once an item is fetched at some 50 cycles a
+// line: what is not the inner loop is kept short and rolled.
+
+// Overwrites columns [left, 128) of the warp's rows of S with -inf.
+__device__ __forceinline__ void mask_columns(uint32_t taddr, int left) {
+#pragma unroll 1
+  for (int c = left & ~15; c < 128; c += 16) {
+    uint32_t v[16];
+    tmem_load_16(taddr + c, v);
+#pragma unroll
+    for (int x = 0; x < 16; ++x)
+      if (c + x >= left) v[x] = 0xff800000u;
+    tmem_store_16(taddr + c, v);
+  }
+  tmem_store_wait();
+}
+
+// 32 weights of a row: p = 2^(s sl2 - m), every fourth pair by polynomial,
+// summed into l and packed. (The polynomial makes 2^-126 of a masked -inf: in
+// the sum that is nothing, and the products do not reach its key or find 0 in V.)
+template <typename T>
 __device__ __forceinline__ void weights_32(const uint32_t* s, float2 sc, float2 nm, float2& l0, float2& l1,
                                            uint32_t (&e)[16]) {
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
     float2 a = fma_f32x2(make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), sc, nm);
-    if (!kTail && (x & 3) == 3) {
+    if ((x & 3) == 3) {
       a = ex2_poly(a);
     } else {
       a.x = ex2_approx(a.x);
@@ -512,27 +552,17 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         if (!mbar_wait(&bar[kFwSFull0 + t], ns & 1, ctx, 231)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
+        if (it.n - j * kTile < kTile) mask_columns(tS, it.n - j * kTile);
         uint32_t s[128];
         tmem_load_64_start(tS, s);
         tmem_load_64_wait(s);
         tmem_load_64_start(tS + 64, s + 64);
-        const int left = it.n - j * kTile;
-        if (left < kTile) {
-#pragma unroll
-          for (int x = 0; x < 64; ++x)
-            if (x >= left) s[x] = 0xff800000u;  // -inf
-        }
         float mx[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) mx[x] = __uint_as_float(s[x]);
 #pragma unroll
         for (int x = 4; x < 64; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
         tmem_load_64_wait(s + 64);
-        if (left < kTile) {
-#pragma unroll
-          for (int x = 64; x < 128; ++x)
-            if (x >= left) s[x] = 0xff800000u;
-        }
 #pragma unroll
         for (int x = 64; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2 - kBias;
@@ -558,9 +588,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           uint32_t e[16];
-          if (left >= kTile) weights_32<T, false>(s + 32 * h, sc, nm, l0, l1, e);
-          else weights_32<T, true>(s + 32 * h, sc, nm, l0, l1, e);
-          __syncwarp();
+          weights_32<T>(s + 32 * h, sc, nm, l0, l1, e);
           tmem_store_16(tS + 16 * h, e);
           if (h >= 2) {
             tmem_store_wait();
@@ -623,34 +651,18 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         const float lse = keys ? (ml.x + log2f(ml.y)) * kLn2 : -INFINITY;
         const int64_t row = (static_cast<int64_t>(b) * p.Hkv * p.rows.G + h) * p.rows.M + m;
         const uint32_t tO = tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16);
-        float* part = p.partial ? p.part_o + (it.split * all_rows + row) * D : nullptr;
-        uint8_t* out = p.partial ? nullptr : reinterpret_cast<uint8_t*>(p.O.at(b, h, m));
         if (real) *(p.partial ? p.part_lse + it.split * all_rows + row : p.LSE + row) = lse;
+        // bytes of this row's output, 16-bit or fp32; null where there is no row
+        uint8_t* out = reinterpret_cast<uint8_t*>(p.partial ? reinterpret_cast<void*>(p.part_o + (it.split * all_rows + row) * D)
+                                                            : reinterpret_cast<void*>(p.O.at(b, h, m)));
         if (!real) out = nullptr;
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < D / 32; ++x) {
           uint32_t o[32];
-          __syncwarp();
-          if (keys) {
-            tmem_load_32(tO + 32 * x, o);
-          } else {
 #pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] = 0u;
-          }
-          if (p.partial) {
-            if (real) {
-#pragma unroll
-              for (int y = 0; y < 8; ++y)
-                reinterpret_cast<float4*>(part + 32 * x)[y] =
-                    make_float4(inv * __uint_as_float(o[4 * y]), inv * __uint_as_float(o[4 * y + 1]),
-                                inv * __uint_as_float(o[4 * y + 2]), inv * __uint_as_float(o[4 * y + 3]));
-            }
-          } else {
-            uint4 ch[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) ch[y] = pack8<T>(o + 8 * y, inv);
-            store_rows_anywhere<4>(ch, out ? out + 64 * x : nullptr, lane);
-          }
+          for (int y = 0; y < 32; ++y) o[y] = 0u;
+          if (keys) tmem_load_32(tO + 32 * x, o);
+          store_row_32(p.partial, out, x, o, inv, lane, T());
         }
         tc_fence_before();
         __syncwarp();
