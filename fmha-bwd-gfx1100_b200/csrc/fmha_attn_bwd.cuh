@@ -12,7 +12,7 @@
 //
 // Rows are packed into tiles of 128 as in the forward (RowPack), so that the
 // short query rows of all heads of a kv head share a tile; the rows of a box
-// that hold no row have LSE = +inf, hence P = 0.
+// that hold no row have -LSE = -inf, hence P = 0.
 //
 // Work is divided by steps (one key tile for one pair of row tiles; one row
 // tile for one key tile), counted on the device from the lengths. If whole
@@ -36,8 +36,8 @@ struct BwdParams {
   int B, Hkv, N, pairs;
   const int* lens;
   View<T> dQ, dK, dV;
-  const float* lse2;  // [B * Hkv * tiles * 128] LSE log2e, packed rows
-  const float* delta; // the same rows' D
+  const float* nlse2;   // [B * Hkv * tiles * 128] -LSE log2e (+ 10 in fp16), packed rows
+  const float* ndelta;  // the same rows' -D
   const float2* amax; // [blocks of attn_delta_kernel]: largest |dO|, |V| (fp16 only)
   int amax_count;
   float* part;        // [2 * grid][2][128][D] partial sums
@@ -198,15 +198,15 @@ __device__ __forceinline__ int ds_exponent(const BwdParams<T>& p, int lane) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 // ==================================================================== delta
-// Per packed row: lse2 = LSE log2e (0 for a row without keys, +inf where the
-// tile holds no row) and D. A block takes row tiles one by one, D / 8 threads
+// Per packed row: -LSE log2e (0 for a row without keys, -inf where the tile
+// holds no row: P = 0) plus fp16's power of two of P, and -D. A block takes row tiles one by one, D / 8 threads
 // a row, several rows' loads in flight. In fp16 also the largest |dO| and
 // valid |V| that the block saw.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
     attn_delta_kernel(View<T> dO, View<T> O, View<T> V, const float* __restrict__ LSE, BwdParams<T> p,
-                      float* __restrict__ lse2, float* __restrict__ delta, float2* __restrict__ amax) {
-  constexpr int kPer = D / 8, kStep = 256 / kPer;
+                      float* __restrict__ nlse2, float* __restrict__ ndelta, float2* __restrict__ amax) {
+  constexpr int kPer = D / 8, kStep = 256 / kPer, kBatch = 4;  // threads a row, rows a pass, passes at once
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int chunk = threadIdx.x % kPer, r0 = threadIdx.x / kPer;
   const int tiles = p.B * p.Hkv * p.rows.tiles;
@@ -220,17 +220,30 @@ __global__ void __launch_bounds__(256)
     return top;
   };
   for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
-    const int tile = i % p.rows.tiles, bh = i / p.rows.tiles;
-    const int hk = bh % p.Hkv, b = bh / p.Hkv;
-#pragma unroll 4
-    for (int r = r0; r < kTile; r += kStep) {
-      int m, g, s;
-      const bool real = p.rows.row(tile, r, m, g, s);
-      float acc = 0.f;
-      if (real) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(dO.at(b, hk * p.rows.G + g, m)) + chunk);
-        const uint4 y = __ldg(reinterpret_cast<const uint4*>(O.at(b, hk * p.rows.G + g, m)) + chunk);
-        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+    // kv heads innermost: with the usual [token][head] layouts, the blocks read neighbouring memory
+    const int hk = i % p.Hkv, tile = i / p.Hkv % p.rows.tiles, b = i / p.Hkv / p.rows.tiles;
+    const int64_t base = ((static_cast<int64_t>(b) * p.Hkv + hk) * p.rows.tiles + tile) * kTile;
+#pragma unroll 1
+    for (int r = r0; r < kTile; r += kBatch * kStep) {
+      uint4 x[kBatch], y[kBatch];
+      float l[kBatch];
+      bool real[kBatch];
+#pragma unroll
+      for (int i4 = 0; i4 < kBatch; ++i4) {  // all of the batch's loads first
+        int m, g, s;
+        real[i4] = p.rows.row(tile, r + i4 * kStep, m, g, s);
+        x[i4] = y[i4] = make_uint4(0, 0, 0, 0);
+        l[i4] = 0.f;
+        if (real[i4]) {
+          x[i4] = __ldg(reinterpret_cast<const uint4*>(dO.at(b, hk * p.rows.G + g, m)) + chunk);
+          y[i4] = __ldg(reinterpret_cast<const uint4*>(O.at(b, hk * p.rows.G + g, m)) + chunk);
+          l[i4] = __ldg(LSE + (static_cast<int64_t>(b) * p.Hkv * p.rows.G + hk * p.rows.G + g) * p.rows.M + m);
+        }
+      }
+#pragma unroll
+      for (int i4 = 0; i4 < kBatch; ++i4) {
+        const uint32_t xw[4] = {x[i4].x, x[i4].y, x[i4].z, x[i4].w}, yw[4] = {y[i4].x, y[i4].y, y[i4].z, y[i4].w};
+        float acc = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const float2 a = Elem<T>::unpack(xw[t]), c = Elem<T>::unpack(yw[t]);
@@ -238,18 +251,13 @@ __global__ void __launch_bounds__(256)
           acc = fmaf(a.y, c.y, acc);
         }
         if (!Elem<T>::kBF16) top_do = widest(top_do, xw);
-      }
 #pragma unroll
-      for (int o = kPer / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o, kPer);
-      if (chunk == 0) {
-        float l = INFINITY;
-        if (real) {
-          l = LSE[(static_cast<int64_t>(b) * p.Hkv * p.rows.G + hk * p.rows.G + g) * p.rows.M + m];
-          l = l == -INFINITY ? 0.f : l * kLog2e;
+        for (int o = kPer / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o, kPer);
+        if (chunk == 0) {
+          const float nl = (l[i4] == -INFINITY ? 0.f : -l[i4] * kLog2e) + (Elem<T>::kBF16 ? 0.f : 10.f);
+          nlse2[base + r + i4 * kStep] = real[i4] ? nl : -INFINITY;
+          ndelta[base + r + i4 * kStep] = -acc;
         }
-        const int64_t at = static_cast<int64_t>(i) * kTile + r;
-        lse2[at] = l;
-        delta[at] = acc;
       }
     }
   }
@@ -298,20 +306,6 @@ __device__ __forceinline__ void zero_rows(const View<T>& v, int b, int heads, in
   }
 }
 
-// This thread's row of D sums in TMEM, to a partial-sum slot or, scaled, to
-// its 16-bit output row (null: none).
-template <typename T, int D>
-__device__ __forceinline__ void store_sums(uint32_t taddr, T* out, float mul, float* part, int lane) {
-  uint8_t* row = part ? reinterpret_cast<uint8_t*>(part) : reinterpret_cast<uint8_t*>(out);
-  const float by = part ? 1.f : mul;
-#pragma unroll 1
-  for (int x = 0; x < D / 32; ++x) {
-    uint32_t v[32];
-    tmem_load_32(taddr + 32 * x, v);
-    store_row_32(part != nullptr, row, x, v, by, lane, T());
-  }
-}
-
 // ======================================================================= dq
 // One CTA walks units (two row tiles, a run of key tiles). Per tile and step:
 //   S = Q K^T -> TMEM R;  the tile's warpgroup (thread = row) takes S into
@@ -321,6 +315,17 @@ __device__ __forceinline__ void store_sums(uint32_t taddr, T* out, float mul, fl
 //
 // Shared memory (D = 128): Q, dO of both tiles 128 KB, K x2, V x1 = 224 KB.
 // TMEM: R_t [128 t, +128), dQ_t [256 + D t, +D).
+// Both kernels: warpgroups 0 to 3 form P and dS, 4 stores the sums, 5 holds the
+// TMA producer (warp 20), two MMA issuers (21, 23) and the scheduler (22). The
+// dQ kernel holds 64 columns a thread and splits its registers, 4 * 128 * 96 +
+// 2 * 128 * 48, the 768 * 80 of the launch; the other needs no more than 80.
+// (With two warpgroups for P and dS a step took 10 % longer in both: a warp's
+// own latencies were the longest part of the loop.)
+constexpr int kBwdThreads = 768, kDqComputeRegs = 96, kDqOtherRegs = 48;
+static_assert(4 * kDqComputeRegs + 2 * kDqOtherRegs == 6 * 80, "register split");
+constexpr int kStoreWarp = 16, kLoadWarp = 20, kMmaWarp0 = 21, kUnitWarp = 22, kMmaWarp1 = 23;
+constexpr int kBwdReaders = 23;  // of a unit: every warp but the scheduler
+
 template <int D>
 struct DqCfg2 {
   static constexpr int kTileBytes = (D / kBoxCols) * kBoxBytes;
@@ -332,33 +337,28 @@ struct DqCfg2 {
   static constexpr int kSmemBytes = kOffBar + 512;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
-// Both kernels: warpgroups 0 and 1 form P and dS, 2 stores the sums, 3 holds
-// the TMA producer (warp 12), two MMA issuers (13, 15) and the scheduler (14),
-// whose other lanes zero what has no keys. Registers: 2 * 128 * 184 + 2 * 128 *
-// 72, the 512 * 128 of the launch.
-constexpr int kBwdThreads = 512, kBwdComputeRegs = 184, kBwdOtherRegs = 72;
-static_assert(2 * kBwdComputeRegs + 2 * kBwdOtherRegs == 4 * 128, "register split");
-constexpr int kUnitReaders = 15;  // warps 0-13 and 15
-
 enum DqBar2 : int {
-  kBqQFull0 = 0,    // + tile: Q and dO
-  kBqQEmpty0 = 2,   // + tile: the unit's last dP of the tile is done
+  kBqQFull0 = 0,    // + tile
+  kBqQEmpty0 = 2,   // + tile: the unit's last S of the tile is done
   kBqKFull0 = 4,    // + slot (up to 4)
   kBqKEmpty0 = 8,
   kBqVFull0 = 12,
   kBqVEmpty0 = 16,
   kBqSFull0 = 20,   // + tile
-  kBqSRead0 = 22,   // + tile: S is in registers (4 warps)
+  kBqSRead0 = 22,   // + tile: S is in registers (8 warps)
   kBqXFull0 = 24,   // + tile: dP
-  kBqDSFull0 = 26,  // + tile: dS written (4 warps)
+  kBqDSFull0 = 26,  // + tile: dS written (8 warps)
   kBqAcc0 = 28,     // + tile: the unit's dQ is complete
   kBqAccEmpty0 = 30,// + tile: and read (4 warps)
   kBqDrain0 = 32,   // + tile
   kBqUnitFull0 = 34,
   kBqUnitEmpty0 = 38,
   kBqTail0 = 42,    // + slot: a last K tile has landed, its rows behind the keys not yet cleared
-  kNumBqBars = 46,
+  kBqOFull0 = 46,   // + tile: dO
+  kBqOEmpty0 = 48,  // + tile: the unit's last dP of the tile is done
+  kNumBqBars = 50,
 };
+static_assert(kNumBqBars * 8 + 8 <= 512, "barrier area");
 
 // Zeroes the dS (16-bit pairs in TMEM) of the keys of the last 16 that count
 // in part, at and past `left`; the products do not reach further.
@@ -399,15 +399,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (int i = 0; i < kNumBqBars; ++i) {
       int count = 1;
       if ((i >= kBqKEmpty0 && i < kBqVFull0) || (i >= kBqVEmpty0 && i < kBqSFull0)) count = 2;
-      if ((i >= kBqSRead0 && i < kBqXFull0) || (i >= kBqDSFull0 && i < kBqAcc0) || (i >= kBqAccEmpty0 && i < kBqDrain0))
-        count = 4;
-      if (i >= kBqUnitEmpty0 && i < kBqTail0) count = kUnitReaders;
+      if ((i >= kBqSRead0 && i < kBqXFull0) || (i >= kBqDSFull0 && i < kBqAcc0)) count = 8;
+      if (i >= kBqAccEmpty0 && i < kBqDrain0) count = 4;
+      if (i >= kBqUnitEmpty0 && i < kBqTail0) count = kBwdReaders;
       mbar_init(&bar[i], count);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 13) {
+  if (warp == kMmaWarp0) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -416,18 +416,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   WaitCtx ctx{abort_flag, p.timeout_ns};
-  // lse2, delta and the exponents come from the launch before; the launch after needs only those
+  // nlse2, ndelta and the exponents come from the launch before; the launch after needs only those
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int q_tiles = p.rows.tiles;
   uint64_t *unit_full = &bar[kBqUnitFull0], *unit_empty = &bar[kBqUnitEmpty0];
-  BwdUnit u;
+  BwdUnit u{};
   int k = 0;
   bool ok = true;
 
-  if (warp >= 12) {
-    regs_lower<kBwdOtherRegs>();
-    if (warp == 12) {
+  if (warp >= kLoadWarp) {
+    regs_lower<kDqOtherRegs>();
+    if (warp == kLoadWarp) {
       // ---- TMA producer
       if (elect_one()) {
         tma_prefetch_desc(&tm_Q);
@@ -436,7 +436,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tma_prefetch_desc(&tm_dO);
         const uint64_t pol_q = l2_policy_evict_first(), pol_kv = l2_policy_evict_last();
         const uint32_t q_bytes = static_cast<uint32_t>(p.rows.Mt * p.rows.Gt) * 128u * (D / kBoxCols);
-        int nq[2] = {0, 0}, nk = 0, nv = 0, tails = 0;
+        uint32_t nq = 0;  // a byte each for Q and dO of both tiles
+        int nk = 0, nv = 0, tails = 0;
         auto load_k = [&](int j) {
           const int s = nk % SK;
           if (nk >= SK && !mbar_wait(&bar[kBqKEmpty0 + s], ((nk / SK) - 1) & 1, ctx, 302)) return false;
@@ -452,22 +453,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           return true;
         };
         while (take_unit<false>(ring, unit_full, unit_empty, k, u, ctx, 300, ok)) {
+          // Q before K, dO behind it: each as soon as its own last product of
+          // the unit before is done
 #pragma unroll 1
-          for (int t = 0; t < 2 && ok; ++t) {
-            const int tile = 2 * u.idx + t;
-            if (tile >= q_tiles) break;
-            if (nq[t] > 0 && !(ok = mbar_wait(&bar[kBqQEmpty0 + t], (nq[t] - 1) & 1, ctx, 301))) break;
+          for (int x4 = 0; x4 < 4 && ok; ++x4) {
+            const int t = x4 & 1, tile = 2 * u.idx + t;
+            const bool first = x4 < 2;  // Q, else dO
+            if (x4 == 1) ok = load_k(u.lo);
+            if (tile >= q_tiles || !ok) continue;
+            const int full = first ? kBqQFull0 : kBqOFull0, empty = first ? kBqQEmpty0 : kBqOEmpty0;
+            const int n = nq >> (8 * x4) & 1, any = nq >> (8 * x4 + 1) & 1;  // turns of its barrier, whether it was used
+            if (any && !(ok = mbar_wait(&bar[empty + t], n ^ 1, ctx, 301))) break;
+            nq ^= 1u << (8 * x4);
+            nq |= 2u << (8 * x4);
             const int m0 = tile % p.rows.nm * p.rows.Mt, h0 = u.hk * p.rows.G + tile / p.rows.nm * p.rows.Gt;
-            mbar_arrive_expect_tx(&bar[kBqQFull0 + t], 2 * q_bytes);
+            mbar_arrive_expect_tx(&bar[full + t], q_bytes);
+            const CUtensorMap* tm = first ? &tm_Q : &tm_dO;
+            uint8_t* dst = smem + (first ? Cfg::kOffQ : Cfg::kOffdO) + t * Cfg::kTileBytes;
 #pragma unroll
-            for (int x = 0; x < D / kBoxCols; ++x) {
-              tma_load_4d(smem + Cfg::kOffQ + t * Cfg::kTileBytes + x * kBoxBytes, &tm_Q, &bar[kBqQFull0 + t],
-                          x * kBoxCols, m0, h0, u.b, pol_q);
-              tma_load_4d(smem + Cfg::kOffdO + t * Cfg::kTileBytes + x * kBoxBytes, &tm_dO, &bar[kBqQFull0 + t],
-                          x * kBoxCols, m0, h0, u.b, pol_q);
-            }
-            ++nq[t];
-            if (t == 0) ok = load_k(u.lo);
+            for (int x = 0; x < D / kBoxCols; ++x)
+              tma_load_4d(dst + x * kBoxBytes, tm, &bar[full + t], x * kBoxCols, m0, h0, u.b, pol_q);
           }
           for (int j = u.lo; j < u.hi && ok; ++j) {
             const int s = nv % SV;
@@ -482,8 +487,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           }
         }
         if (*abort_flag) {  // every copy in flight ends before the block does
-          for (int t = 0; t < 2; ++t)
-            if (nq[t] > 0) mbar_wait_drain(&bar[kBqQFull0 + t], (nq[t] - 1) & 1, p.timeout_ns);
+          for (int x = 0; x < 4; ++x)
+            if (nq >> (8 * x + 1) & 1)
+              mbar_wait_drain(&bar[(x < 2 ? kBqQFull0 : kBqOFull0) + (x & 1)], (nq >> (8 * x) & 1) ^ 1, p.timeout_ns);
           for (int i = (nk > SK ? nk - SK : 0); i < nk; ++i) {
             mbar_wait_drain(&bar[kBqKFull0 + i % SK], (i / SK) & 1, 1000000);
             if (tails >> (i % SK) & 1)
@@ -494,7 +500,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
       __syncwarp();
-    } else if (warp == 14) {
+    } else if (warp == kUnitWarp) {
       if (lane == 0) {
         feed_units<T, true>(p, ring, unit_full, unit_empty, ctx, 305);
       } else if (p.lens) {
@@ -509,7 +515,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       // ---- MMA issuer of tile t: per step dP, dQ, and S of the next step. A
       // thread for each tile keeps one tile's wait from holding up the other's
       // products.
-      const int t = warp == 13 ? 0 : 1;
+      const int t = warp == kMmaWarp0 ? 0 : 1;
       if (elect_one()) {
         constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
         constexpr uint32_t id_A = make_idesc_f16<kB>(kTile, D, false, true);
@@ -536,6 +542,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           for (int j = u.lo - 1; j < u.hi; ++j) {
             if (j >= u.lo) {
               // dP_j over S_j once the warps have that in registers
+              if (j == u.lo && !(ok = mbar_wait(&bar[kBqOFull0 + t], nq & 1, ctx, 316 + 10 * t))) break;
               if (!(ok = mbar_wait(&bar[kBqVFull0 + g % SV], (g / SV) & 1, ctx, 312 + 10 * t))) break;
               if (!(ok = mbar_wait(&bar[kBqSRead0 + t], n & 1, ctx, 313 + 10 * t))) break;
               tc_fence_after();
@@ -543,7 +550,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               umma_commit(&bar[kBqXFull0 + t]);
               umma_commit(&bar[kBqVEmpty0 + g % SV]);
               if (alone) umma_commit(&bar[kBqVEmpty0 + g % SV]);
-              if (j + 1 == u.hi) umma_commit(&bar[kBqQEmpty0 + t]);
+              if (j + 1 == u.hi) umma_commit(&bar[kBqOEmpty0 + t]);
               // dQ += dS_j K_j
               if (j == u.lo && nq > 0 && !(ok = mbar_wait(&bar[kBqAccEmpty0 + t], (nq - 1) & 1, ctx, 314 + 10 * t))) break;
               if (!(ok = mbar_wait(&bar[kBqDSFull0 + t], n & 1, ctx, 315 + 10 * t))) break;
@@ -554,10 +561,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               if (left >= kTile) {
 #pragma unroll
                 for (int x = 0; x < kTile / 16; ++x)
-                  umma_f16_ts(tA, tR + x * 8, desc_advance(dk, x * 2048), id_A, x > 0 ? 1u : keep);
+                  umma_f16_ts(tA, tR + (x >> 2) * 64 + (x & 3) * 8, desc_advance(dk, x * 2048), id_A, x > 0 ? 1u : keep);
               } else {
                 for (int x = 0; x < (left + 15) / 16; ++x)
-                  umma_f16_ts(tA, tR + x * 8, desc_advance(dk, x * 2048), id_A, x > 0 ? 1u : keep);
+                  umma_f16_ts(tA, tR + (x >> 2) * 64 + (x & 3) * 8, desc_advance(dk, x * 2048), id_A, x > 0 ? 1u : keep);
               }
               umma_commit(&bar[kBqKEmpty0 + g % SK]);
               if (alone) umma_commit(&bar[kBqKEmpty0 + g % SK]);
@@ -570,6 +577,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               tc_fence_after();
               product(dq, sK + (g % SK) * Cfg::kTileBytes);
               umma_commit(&bar[kBqSFull0 + t]);
+              if (j + 2 == u.hi) umma_commit(&bar[kBqQEmpty0 + t]);
             }
           }
           if (!ok) break;
@@ -582,11 +590,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       __syncwarp();
     }
-  } else if (warp < 8) {
-    // ---- P and dS: warpgroup t owns tile t, thread = row (TMEM lane)
-    regs_raise<kBwdComputeRegs>();
-    const int t = warp >> 2, r = threadIdx.x & 127;
-    const uint32_t tR = tmem + 128 * t + (static_cast<uint32_t>(r & 96) << 16);
+  } else if (warp < kStoreWarp) {
+    // ---- P and dS: two warpgroups a tile, thread = row (TMEM lane), columns
+    // 64 c to 64 c + 63; dS lies in columns [64 c, 64 c + 32)
+    regs_raise<kDqComputeRegs>();
+    const int t = warp >> 3, c = warp >> 2 & 1, r = threadIdx.x & 127;
+    const uint32_t tR = tmem + 128 * t + 64 * c + (static_cast<uint32_t>(r & 96) << 16);
     const float sl2 = p.scale * kLog2e;
     const float ds_mul = pow2(ds_exponent<T, D>(p, lane) - kPBias);
     int ns = 0;
@@ -594,42 +603,33 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int tile = 2 * u.idx + t;
       if (tile >= q_tiles) continue;
       const int64_t row = ((static_cast<int64_t>(u.b) * p.Hkv + u.hk) * q_tiles + tile) * kTile + r;
-      const float nl = static_cast<float>(kPBias) - __ldcg(p.lse2 + row);
-      const float nd = -ds_mul * __ldcg(p.delta + row);
+      const float nl = __ldcg(p.nlse2 + row);
+      const float nd = ds_mul * __ldcg(p.ndelta + row);
       for (int j = u.lo; j < u.hi; ++j, ++ns) {
         if (!mbar_wait(&bar[kBqSFull0 + t], ns & 1, ctx, 320)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
-        uint32_t s[128];
-        auto weights = [&](uint32_t* v) {  // P of 64 columns, every fourth pair by polynomial
-#pragma unroll
-          for (int x = 0; x < 64; x += 2) {
-            float2 a = fma_f32x2(make_float2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])), make_float2(sl2, sl2),
-                                 make_float2(nl, nl));
-            if ((x & 7) == 6) {
-              a = ex2_poly(a);
-            } else {
-              a.x = ex2_approx(a.x);
-              a.y = ex2_approx(a.y);
-            }
-            v[x] = __float_as_uint(a.x);
-            v[x + 1] = __float_as_uint(a.y);
-          }
-        };
-        tmem_load_64_start(tR, s);
-        tmem_load_64_wait(s);
-        tmem_load_64_start(tR + 64, s + 64);
-        weights(s);
-        tmem_load_64_wait(s + 64);
+        uint32_t s[64];
+        tmem_load_32_start(tR, s);
+        tmem_load_32_start(tR + 32, s + 32);
+        tmem_load_32_wait(s);
+        tmem_load_32_wait(s + 32);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[kBqSRead0 + t]);
-        weights(s + 64);
+#pragma unroll
+        for (int x = 0; x < 64; x += 2) {
+          float2 a = fma_f32x2(make_float2(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), make_float2(sl2, sl2),
+                               make_float2(nl, nl));
+          a = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+          s[x] = __float_as_uint(a.x);
+          s[x + 1] = __float_as_uint(a.y);
+        }
         if (!mbar_wait(&bar[kBqXFull0 + t], ns & 1, ctx, 321)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
+        for (int q = 0; q < 4; ++q) {
           uint32_t dp[16], e[8];
           tmem_load_16(tR + 16 * q, dp);
 #pragma unroll
@@ -641,9 +641,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           }
           tmem_store_8(tR + 8 * q, e);
         }
-        if (u.n - j * kTile < kTile) {
+        const int left = u.n - j * kTile - 64 * c;
+        if (left > 0 && left < 64) {
           tmem_store_wait();
-          clear_ds(tR, u.n - j * kTile);
+          clear_ds(tR, left);
         }
         tmem_store_wait();
         tc_fence_before();
@@ -652,16 +653,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     }
   } else {
-    // ---- dQ: thread = row of each tile in turn; warp 8 also clears the last
-    // K tile behind the last key, for the issuers that wait for it
-    regs_lower<kBwdOtherRegs>();
+    // ---- dQ: thread = row of each tile in turn; one warp also clears the
+    // last K tile behind the last key, for the issuers that wait for it
+    regs_lower<kDqOtherRegs>();
     const int r = threadIdx.x & 127;
     const float out_mul = p.scale * pow2(-ds_exponent<T, D>(p, lane));
     int na0 = 0, na1 = 0, g = 0;
     uint32_t tail_turns = 0;
     while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 329, ok)) {
       g += u.hi - u.lo;
-      if (warp == 8 && has_tail(u.n, u.hi)) {
+      if (warp == kStoreWarp && has_tail(u.n, u.hi)) {
         const int slot = (g - 1) % SK;
         if (!mbar_wait(&bar[kBqTail0 + slot], tail_turns >> slot & 1, ctx, 331)) ok = false;
         tail_turns ^= 1u << slot;
@@ -682,9 +683,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
         int m, g, s;
         const bool real = p.rows.row(tile, r, m, g, s);
-        T* out = real ? p.dQ.at(u.b, u.hk * p.rows.G + g, m) : nullptr;
-        store_sums<T, D>(tmem + 256 + D * t + (static_cast<uint32_t>(r & 96) << 16), out, out_mul,
-                         u.slot < 0 ? nullptr : p.part + ((static_cast<int64_t>(u.slot) * 2 + t) * kTile + r) * D, lane);
+        float* part = p.part + ((static_cast<int64_t>(u.slot) * 2 + t) * kTile + r) * D;
+        uint8_t* out = u.slot >= 0 ? reinterpret_cast<uint8_t*>(part)
+                       : real      ? reinterpret_cast<uint8_t*>(p.dQ.at(u.b, u.hk * p.rows.G + g, m))
+                                   : nullptr;
+        store_sums<T, D>(tmem + 256 + D * t + (static_cast<uint32_t>(r & 96) << 16), u.slot >= 0, out,
+                         u.slot >= 0 ? 1.f : out_mul);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[kBqAccEmpty0 + t]);
@@ -695,7 +699,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0) publish_failure(*abort_flag, p.status);
-  if (warp == 13) {
+  if (warp == kMmaWarp0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -709,16 +713,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // The warps form dS^T during dV and S^T of the next tile, and its P^T during
 // dK and the next dP^T.
 //
-// Shared memory (D = 128): K, V 64 KB, Q x2, dO x2 128 KB, lse2 and delta.
-// TMEM: S^T [0, 128), dP^T [128, 256), dV, dK behind. Warps 0-7 form P and dS:
-// lane quarter warp % 4, rows 64 c .. 64 c + 63 of the row tile, c = warp / 4;
-// the 16-bit halves lie in columns [64 c, 64 c + 32).
+// Shared memory (D = 128): K, V 64 KB, Q x3, dO x2 160 KB, nlse2 and ndelta.
+// (With two Q slots, S^T waited some 700 cycles a step for its Q: the slot is
+// free only when dK of two steps before is done.) TMEM: S^T [0, 128), dP^T
+// [128, 256), dV, dK behind.
 template <int D>
 struct DkvCfg2 {
   static constexpr int kTileBytes = (D / kBoxCols) * kBoxBytes;
   static constexpr int kOffK = 0, kOffV = kTileBytes;
-  static constexpr int kOffQ = 2 * kTileBytes, kOffdO = 4 * kTileBytes;  // two slots each
-  static constexpr int kOffL = 6 * kTileBytes;                          // [2 slots][lse2, delta][128]
+  static constexpr int kOffQ = 2 * kTileBytes, kOffdO = 5 * kTileBytes;  // three and two slots
+  static constexpr int kOffL = 7 * kTileBytes;                          // [dO slot][nlse2, ndelta][128]
   static constexpr int kOffRing = kOffL + 2 * 2 * kTile * 4;
   static constexpr int kOffBar = kOffRing + sizeof(UnitRing);
   static constexpr int kSmemBytes = kOffBar + 256;
@@ -727,23 +731,24 @@ struct DkvCfg2 {
 };
 
 enum DkvBar2 : int {
-  kBkKV = 0,
-  kBkKVEmpty = 1,
-  kBkQFull0 = 2,   // + slot: Q, lse2, delta
-  kBkQEmpty0 = 4,
-  kBkOFull0 = 6,   // + slot: dO
-  kBkOEmpty0 = 8,
-  kBkSFull = 10,
-  kBkPFull = 11,   // 8 warps
-  kBkXFull = 12,
-  kBkDSFull = 13,  // 8 warps
-  kBkAcc = 14,
-  kBkAccEmpty = 15, // 4 warps
-  kBkDrain0 = 16,   // + issuer
-  kBkUnitFull0 = 18,
-  kBkUnitEmpty0 = 22,
-  kNumBkBars = 26,
+  kBkKVFull0 = 28,  // K, V
+  kBkKVEmpty0 = 0,  // the unit's last S^T, its last dP^T are done
+  kBkQFull0 = 2,   // + slot (3)
+  kBkQEmpty0 = 5,  // dK is done with it
+  kBkOFull0 = 8,   // + slot (2): dO, nlse2, ndelta
+  kBkOEmpty0 = 10, // dV is done with dO, and dK of the step (so the warps with ndelta)
+  kBkSFull = 12,
+  kBkPFull = 13,   // 16 warps
+  kBkXFull = 14,
+  kBkDSFull = 15,  // 16 warps
+  kBkAcc = 16,     // both issuers
+  kBkAccEmpty = 17, // 4 warps
+  kBkDrain0 = 18,  // + issuer
+  kBkUnitFull0 = 20,
+  kBkUnitEmpty0 = 24,
+  kNumBkBars = 30,
 };
+static_assert(kNumBkBars * 8 + 8 <= 256, "barrier area");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
@@ -769,23 +774,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (int i = 0; i < kNumBkBars; ++i)
       {
       int count = 1;
-      if (i == kBkKVEmpty || i == kBkOEmpty0 || i == kBkOEmpty0 + 1 || i == kBkAcc) count = 2;
-      if (i == kBkPFull || i == kBkDSFull) count = 8;
+      if (i == kBkOEmpty0 || i == kBkOEmpty0 + 1 || i == kBkAcc) count = 2;
+      if (i == kBkPFull || i == kBkDSFull) count = 16;
       if (i == kBkAccEmpty) count = 4;
-      if (i >= kBkUnitEmpty0) count = kUnitReaders;
+      if (i >= kBkUnitEmpty0 && i < kBkKVFull0) count = kBwdReaders;
       mbar_init(&bar[i], count);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 13) {
+  if (warp == kMmaWarp0) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   // rows of the Q and dO slots that no box fills are summed over with P = dS = 0
   const int box_rows = p.rows.Mt * p.rows.Gt;
   if (box_rows < kTile) {
-    for (int i = threadIdx.x; i < 4 * Cfg::kTileBytes / 16; i += kBwdThreads)
+    for (int i = threadIdx.x; i < 5 * Cfg::kTileBytes / 16; i += kBwdThreads)
       *reinterpret_cast<uint4*>(smem + Cfg::kOffQ + 16 * i) = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
   }
@@ -795,16 +800,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t tmem = *tmem_slot;
   WaitCtx ctx{abort_flag, p.timeout_ns};
   uint64_t *unit_full = &bar[kBkUnitFull0], *unit_empty = &bar[kBkUnitEmpty0];
-  BwdUnit u;
+  BwdUnit u{};
   int k = 0;
   bool ok = true;
   // The launch before (attn_dq_kernel) let this one start after its own wait
   // for attn_delta_kernel, whose rows are thus there; attn_dq_kernel itself is
   // waited for at the end, for the launches after.
 
-  if (warp >= 12) {
-    regs_lower<kBwdOtherRegs>();
-    if (warp == 12) {
+  if (warp >= kLoadWarp) {
+    if (warp == kLoadWarp) {
       // ---- TMA producer
       if (elect_one()) {
         tma_prefetch_desc(&tm_Q);
@@ -815,49 +819,51 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const uint32_t q_bytes = static_cast<uint32_t>(box_rows) * 128u * (D / kBoxCols);
         int nu = 0, n = 0, no = 0;
         while (take_unit<false>(ring, unit_full, unit_empty, k, u, ctx, 400, ok)) {
-          if (nu > 0 && !(ok = mbar_wait(&bar[kBkKVEmpty], (nu - 1) & 1, ctx, 401))) break;
-          mbar_arrive_expect_tx(&bar[kBkKV], 2 * Cfg::kTileBytes);
+#pragma unroll 1
+          for (int y = 0; y < 2; ++y) {  // K, V
+            if (nu > 0 && !(ok = mbar_wait(&bar[kBkKVEmpty0 + y], (nu - 1) & 1, ctx, 401))) break;
+            mbar_arrive_expect_tx(&bar[kBkKVFull0 + y], Cfg::kTileBytes);
 #pragma unroll
-          for (int x = 0; x < D / kBoxCols; ++x) {
-            tma_load_4d(smem + Cfg::kOffK + x * kBoxBytes, &tm_K, &bar[kBkKV], x * kBoxCols, u.idx * kTile, u.hk, u.b,
-                        pol_kv);
-            tma_load_4d(smem + Cfg::kOffV + x * kBoxBytes, &tm_V, &bar[kBkKV], x * kBoxCols, u.idx * kTile, u.hk, u.b,
-                        pol_kv);
+            for (int x = 0; x < D / kBoxCols; ++x)
+              tma_load_4d(smem + y * Cfg::kTileBytes + x * kBoxBytes, y == 0 ? &tm_K : &tm_V, &bar[kBkKVFull0 + y],
+                          x * kBoxCols, u.idx * kTile, u.hk, u.b, pol_kv);
           }
+          if (!ok) break;
           ++nu;
           for (int i = u.lo; i < u.hi; ++i) {
-            const int s = n & 1;
+            const int s = n % 3, so = n & 1;
             const int m0 = i % p.rows.nm * p.rows.Mt, h0 = u.hk * p.rows.G + i / p.rows.nm * p.rows.Gt;
             const int64_t row = ((static_cast<int64_t>(u.b) * p.Hkv + u.hk) * q_tiles + i) * kTile;
-            if (n >= 2 && !(ok = mbar_wait(&bar[kBkQEmpty0 + s], ((n >> 1) - 1) & 1, ctx, 402))) break;
-            mbar_arrive_expect_tx(&bar[kBkQFull0 + s], q_bytes + 2 * kTile * 4);
+            if (n >= 3 && !(ok = mbar_wait(&bar[kBkQEmpty0 + s], (n / 3 - 1) & 1, ctx, 402))) break;
+            mbar_arrive_expect_tx(&bar[kBkQFull0 + s], q_bytes);
 #pragma unroll
             for (int x = 0; x < D / kBoxCols; ++x)
               tma_load_4d(smem + Cfg::kOffQ + s * Cfg::kTileBytes + x * kBoxBytes, &tm_Q, &bar[kBkQFull0 + s],
                           x * kBoxCols, m0, h0, u.b, pol_q);
-            bulk_load(smem + Cfg::kOffL + s * 2 * kTile * 4, p.lse2 + row, kTile * 4, &bar[kBkQFull0 + s]);
-            bulk_load(smem + Cfg::kOffL + (s * 2 + 1) * kTile * 4, p.delta + row, kTile * 4, &bar[kBkQFull0 + s]);
             ++n;
-            if (no >= 2 && !(ok = mbar_wait(&bar[kBkOEmpty0 + s], ((no >> 1) - 1) & 1, ctx, 403))) break;
-            mbar_arrive_expect_tx(&bar[kBkOFull0 + s], q_bytes);
+            if (no >= 2 && !(ok = mbar_wait(&bar[kBkOEmpty0 + so], ((no >> 1) - 1) & 1, ctx, 403))) break;
+            mbar_arrive_expect_tx(&bar[kBkOFull0 + so], q_bytes + 2 * kTile * 4);
 #pragma unroll
             for (int x = 0; x < D / kBoxCols; ++x)
-              tma_load_4d(smem + Cfg::kOffdO + s * Cfg::kTileBytes + x * kBoxBytes, &tm_dO, &bar[kBkOFull0 + s],
+              tma_load_4d(smem + Cfg::kOffdO + so * Cfg::kTileBytes + x * kBoxBytes, &tm_dO, &bar[kBkOFull0 + so],
                           x * kBoxCols, m0, h0, u.b, pol_q);
+            bulk_load(smem + Cfg::kOffL + so * 2 * kTile * 4, p.nlse2 + row, kTile * 4, &bar[kBkOFull0 + so]);
+            bulk_load(smem + Cfg::kOffL + (so * 2 + 1) * kTile * 4, p.ndelta + row, kTile * 4, &bar[kBkOFull0 + so]);
             ++no;
           }
           if (!ok) break;
         }
         if (*abort_flag) {  // every copy in flight ends before the block does
-          if (nu > 0) mbar_wait_drain(&bar[kBkKV], (nu - 1) & 1, p.timeout_ns);
-          for (int i = (n > 2 ? n - 2 : 0); i < n; ++i)
-            mbar_wait_drain(&bar[kBkQFull0 + (i & 1)], (i >> 1) & 1, p.timeout_ns);
+          for (int y = 0; y < 2; ++y)
+            if (nu > 0) mbar_wait_drain(&bar[kBkKVFull0 + y], (nu - 1) & 1, p.timeout_ns);
+          for (int i = (n > 3 ? n - 3 : 0); i < n; ++i)
+            mbar_wait_drain(&bar[kBkQFull0 + i % 3], (i / 3) & 1, p.timeout_ns);
           for (int i = (no > 2 ? no - 2 : 0); i < no; ++i)
             mbar_wait_drain(&bar[kBkOFull0 + (i & 1)], (i >> 1) & 1, p.timeout_ns);
         }
       }
       __syncwarp();
-    } else if (warp == 14) {
+    } else if (warp == kUnitWarp) {
       if (lane == 0) {
         feed_units<T, false>(p, ring, unit_full, unit_empty, ctx, 405);
       } else if (p.lens) {
@@ -873,10 +879,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       __syncwarp();
     } else {
-      // ---- MMA issuers: warp 13 dV and S^T of the next row tile (TMEM S, P),
-      // warp 15 dK and dP^T of the next (TMEM X), so that neither chain's
+      // ---- MMA issuers: the first dV and S^T of the next row tile (TMEM S, P),
+      // the second dK and dP^T of the next (TMEM X), so that neither chain's
       // waits hold up the other's products.
-      const int w = warp == 13 ? 0 : 1;
+      const int w = warp == kMmaWarp0 ? 0 : 1;
       if (elect_one()) {
         constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
         constexpr uint32_t id_A = make_idesc_f16<kB>(kTile, D, false, true);
@@ -887,36 +893,41 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const uint32_t tR = tmem + (w == 0 ? Cfg::kColS : Cfg::kColX), tA = tmem + (w == 0 ? Cfg::kColdV : Cfg::kColdK);
         uint64_t* landed = &bar[w == 0 ? kBkQFull0 : kBkOFull0];
         uint64_t* formed = &bar[w == 0 ? kBkPFull : kBkDSFull];
-        int n = 0, nu = 0;
+        const int slots1 = w == 0 ? 3 : 2, slots2 = w == 0 ? 2 : 3;
+        int n = 0, nu = 0, s1 = 0, turn1 = 0, s2 = 0;  // steps and units; slots of `first` and `second`
         while (take_unit<false>(ring, unit_full, unit_empty, k, u, ctx, 409 + 10 * w, ok)) {
-          if (!(ok = mbar_wait(&bar[kBkKV], nu & 1, ctx, 410 + 10 * w))) break;
+          if (!(ok = mbar_wait(&bar[kBkKVFull0 + w], nu & 1, ctx, 410 + 10 * w))) break;
           for (int i = u.lo - 1; i < u.hi; ++i) {
             if (i >= u.lo) {
               if (i == u.lo && nu > 0 && !(ok = mbar_wait(&bar[kBkAccEmpty], (nu - 1) & 1, ctx, 413 + 10 * w))) break;
               if (!(ok = mbar_wait(formed, n & 1, ctx, 414 + 10 * w))) break;
               tc_fence_after();
-              const uint64_t db = make_sw128_desc(second + (n & 1) * Cfg::kTileBytes, kBoxBytes, 1024);
+              const uint64_t db = make_sw128_desc(second + s2 * Cfg::kTileBytes, kBoxBytes, 1024);
 #pragma unroll
               for (int x = 0; x < kTile / 16; ++x)
-                umma_f16_ts(tA, tR + (x >> 2) * 64 + (x & 3) * 8, desc_advance(db, x * 2048), id_A,
+                umma_f16_ts(tA, tR + (x >> 1) * 32 + (x & 1) * 8, desc_advance(db, x * 2048), id_A,
                             x > 0 || i > u.lo ? 1u : 0u);
-              umma_commit(&bar[(w == 0 ? kBkOEmpty0 : kBkQEmpty0) + (n & 1)]);
+              umma_commit(&bar[kBkOEmpty0 + (n & 1)]);
+              if (w == 1) umma_commit(&bar[kBkQEmpty0 + s2]);
               if (i + 1 == u.hi) umma_commit(&bar[kBkAcc]);
+              if (++s2 == slots2) s2 = 0;
               ++n;
             }
             if (i + 1 < u.hi) {
-              if (!(ok = mbar_wait(landed + (n & 1), (n >> 1) & 1, ctx, 411 + 10 * w))) break;
+              if (!(ok = mbar_wait(landed + s1, turn1, ctx, 411 + 10 * w))) break;
               tc_fence_after();
-              const uint64_t db = make_sw128_desc(first + (n & 1) * Cfg::kTileBytes, 16, 1024);
+              const uint64_t db = make_sw128_desc(first + s1 * Cfg::kTileBytes, 16, 1024);
 #pragma unroll
               for (int x = 0; x < D / 16; ++x) {
                 const uint32_t off = (x >> 2) * kBoxBytes + (x & 3) * 32;
                 umma_f16_ss(tR, desc_advance(da, off), desc_advance(db, off), id_S, x > 0 ? 1u : 0u);
               }
               umma_commit(&bar[w == 0 ? kBkSFull : kBkXFull]);
-              // dO has two readers that do not wait for one another; Q's second, dK, waits for its first
-              if (w == 1) umma_commit(&bar[kBkOEmpty0 + (n & 1)]);
-              if (i + 2 == u.hi) umma_commit(&bar[kBkKVEmpty]);
+              if (i + 2 == u.hi) umma_commit(&bar[kBkKVEmpty0 + w]);
+              if (++s1 == slots1) {
+                s1 = 0;
+                turn1 ^= 1;
+              }
             }
           }
           if (!ok) break;
@@ -929,42 +940,38 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       __syncwarp();
     }
-  } else if (warp < 8) {
-    // ---- P^T and dS^T
-    regs_raise<kBwdComputeRegs>();
-    const int c = warp >> 2, r = threadIdx.x & 127;  // r: key within the tile (TMEM lane)
+  } else if (warp < kStoreWarp) {
+    // ---- P^T and dS^T: thread = key (TMEM lane), rows 32 c to 32 c + 31 of the
+    // row tile; the 16-bit values lie in columns [32 c, 32 c + 16)
+    const int c = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(r & 96) << 16;
-    const uint32_t tS = tmem + Cfg::kColS + 64 * c + lanes, tX = tmem + Cfg::kColX + 64 * c + lanes;
-    const float sl2 = p.scale * kLog2e;
+    const uint32_t tS = tmem + Cfg::kColS + 32 * c + lanes, tX = tmem + Cfg::kColX + 32 * c + lanes;
+    const float2 sl2 = make_float2(p.scale * kLog2e, p.scale * kLog2e);
     const float ds_mul = pow2(ds_exponent<T, D>(p, lane) - kPBias);
     int n = 0;
     while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 419, ok)) {
       // a key that does not count gets P = dS = 0, whatever K and V hold
       const bool valid = u.idx * kTile + r < u.n;
       for (int i = u.lo; i < u.hi; ++i, ++n) {
-        const float4* lse = reinterpret_cast<const float4*>(smem + Cfg::kOffL + (n & 1) * 2 * kTile * 4) + 16 * c;
-        const float4* del = lse + kTile / 4;
-        if (!mbar_wait(&bar[kBkQFull0 + (n & 1)], (n >> 1) & 1, ctx, 420)) { ok = false; break; }
+        const float4* nl = reinterpret_cast<const float4*>(smem + Cfg::kOffL + (n & 1) * 2 * kTile * 4) + 8 * c;
+        const float4* nd = nl + kTile / 4;
+        if (!mbar_wait(&bar[kBkOFull0 + (n & 1)], (n >> 1) & 1, ctx, 420)) { ok = false; break; }
         if (!mbar_wait(&bar[kBkSFull], n & 1, ctx, 421)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
-        uint32_t s[64], e[32];
-        tmem_load_64(tS, s);
+        uint32_t s[32], e[16];
+        tmem_load_32(tS, s);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const float4 l = lse[x];
-          float2 a = fma_f32x2(make_float2(__uint_as_float(s[4 * x]), __uint_as_float(s[4 * x + 1])),
-                               make_float2(sl2, sl2), make_float2(kPBias - l.x, kPBias - l.y));
-          float2 b = fma_f32x2(make_float2(__uint_as_float(s[4 * x + 2]), __uint_as_float(s[4 * x + 3])),
-                               make_float2(sl2, sl2), make_float2(kPBias - l.z, kPBias - l.w));
-          a.x = ex2_approx(a.x);
-          a.y = ex2_approx(a.y);
-          if (x & 1) {
-            b = ex2_poly(b);
-          } else {
-            b.x = ex2_approx(b.x);
-            b.y = ex2_approx(b.y);
-          }
+        for (int x = 0; x < 8; ++x) {
+          const float4 l = nl[x];
+          float2 a = fma_f32x2(make_float2(__uint_as_float(s[4 * x]), __uint_as_float(s[4 * x + 1])), sl2,
+                               make_float2(l.x, l.y));
+          float2 b = fma_f32x2(make_float2(__uint_as_float(s[4 * x + 2]), __uint_as_float(s[4 * x + 3])), sl2,
+                               make_float2(l.z, l.w));
+          if (x % 4 < 1) a = ex2_poly<false>(a);
+          else a = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+          if (x % 4 < 1) b = ex2_poly<false>(b);
+          else b = make_float2(ex2_approx(b.x), ex2_approx(b.y));
           s[4 * x] = __float_as_uint(a.x);
           s[4 * x + 1] = __float_as_uint(a.y);
           s[4 * x + 2] = __float_as_uint(b.x);
@@ -974,10 +981,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         if (!valid) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) e[x] = 0u;
+          for (int x = 0; x < 16; ++x) e[x] = 0u;
         }
         __syncwarp();
-        tmem_store_32(tS, e);
+        tmem_store_16(tS, e);
         tmem_store_wait();
         tc_fence_before();
         __syncwarp();
@@ -985,34 +992,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!mbar_wait(&bar[kBkXFull], n & 1, ctx, 422)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
+        uint32_t dp[32];
+        tmem_load_32(tX, dp);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t dp[32];
-          tmem_load_32(tX + 32 * q, dp);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const float4 d = del[8 * q + x];
-            const uint32_t* sp = s + 32 * q + 4 * x;
-            float2 a = add_f32x2(make_float2(__uint_as_float(dp[4 * x]), __uint_as_float(dp[4 * x + 1])),
-                                 make_float2(-d.x, -d.y));
-            float2 b = add_f32x2(make_float2(__uint_as_float(dp[4 * x + 2]), __uint_as_float(dp[4 * x + 3])),
-                                 make_float2(-d.z, -d.w));
-            if (!kB) {
-              a = mul_f32x2(a, make_float2(ds_mul, ds_mul));
-              b = mul_f32x2(b, make_float2(ds_mul, ds_mul));
-            }
-            a = mul_f32x2(a, make_float2(__uint_as_float(sp[0]), __uint_as_float(sp[1])));
-            b = mul_f32x2(b, make_float2(__uint_as_float(sp[2]), __uint_as_float(sp[3])));
-            e[16 * q + 2 * x] = Elem<T>::pack(a.x, a.y);
-            e[16 * q + 2 * x + 1] = Elem<T>::pack(b.x, b.y);
+        for (int x = 0; x < 8; ++x) {
+          const float4 d = nd[x];
+          float2 a = add_f32x2(make_float2(__uint_as_float(dp[4 * x]), __uint_as_float(dp[4 * x + 1])), make_float2(d.x, d.y));
+          float2 b =
+              add_f32x2(make_float2(__uint_as_float(dp[4 * x + 2]), __uint_as_float(dp[4 * x + 3])), make_float2(d.z, d.w));
+          if (!kB) {
+            a = mul_f32x2(a, make_float2(ds_mul, ds_mul));
+            b = mul_f32x2(b, make_float2(ds_mul, ds_mul));
           }
+          a = mul_f32x2(a, make_float2(__uint_as_float(s[4 * x]), __uint_as_float(s[4 * x + 1])));
+          b = mul_f32x2(b, make_float2(__uint_as_float(s[4 * x + 2]), __uint_as_float(s[4 * x + 3])));
+          e[2 * x] = Elem<T>::pack(a.x, a.y);
+          e[2 * x + 1] = Elem<T>::pack(b.x, b.y);
         }
         if (!valid) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) e[x] = 0u;
+          for (int x = 0; x < 16; ++x) e[x] = 0u;
         }
         __syncwarp();
-        tmem_store_32(tX, e);
+        tmem_store_16(tX, e);
         tmem_store_wait();
         tc_fence_before();
         __syncwarp();
@@ -1021,7 +1023,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
   } else {
     // ---- dV and dK: thread = key
-    regs_lower<kBwdOtherRegs>();
     const int r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(r & 96) << 16;
     const float dk_mul = p.scale * pow2(-ds_exponent<T, D>(p, lane)), dv_mul = pow2(-kPBias);
@@ -1035,10 +1036,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll 1
       for (int which = 0; which < 2; ++which) {
         const View<T>& v = which == 0 ? p.dV : p.dK;
-        store_sums<T, D>(tmem + (which == 0 ? Cfg::kColdV : Cfg::kColdK) + lanes,
-                         key < p.N ? v.at(u.b, u.hk, key) : nullptr,
-                         which == 0 ? dv_mul : dk_mul,
-                         u.slot < 0 ? nullptr : p.part + ((static_cast<int64_t>(u.slot) * 2 + which) * kTile + r) * D, lane);
+        float* part = p.part + ((static_cast<int64_t>(u.slot) * 2 + which) * kTile + r) * D;
+        uint8_t* out = u.slot >= 0   ? reinterpret_cast<uint8_t*>(part)
+                       : key < p.N ? reinterpret_cast<uint8_t*>(v.at(u.b, u.hk, key))
+                                   : nullptr;
+        store_sums<T, D>(tmem + (which == 0 ? Cfg::kColdV : Cfg::kColdK) + lanes, u.slot >= 0, out,
+                         u.slot >= 0 ? 1.f : (which == 0 ? dv_mul : dk_mul));
       }
       tc_fence_before();
       __syncwarp();
@@ -1049,7 +1052,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0) publish_failure(*abort_flag, p.status);
-  if (warp == 13) {
+  if (warp == kMmaWarp0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

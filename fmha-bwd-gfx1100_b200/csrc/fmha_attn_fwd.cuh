@@ -37,27 +37,31 @@ namespace fmha_sm100 {
 constexpr float kLn2 = 0.6931471805599453f;
 
 // 2^x of two values on the FMA pipe instead of the SFU, whose 16 results a
-// clock bound these kernels: x = n + f with n the nearest integer (taken from
-// the low mantissa bits of x + 1.5 2^23) and 2^f on [-1/2, 1/2] by the
+// clock would bound these kernels: x = n + f with n the nearest integer (taken
+// from the low mantissa bits of x + 1.5 2^23) and 2^f on [-1/2, 1/2] by the
 // polynomial of degree 5 with the least largest relative error there (found by
 // Remez exchange): 7.5e-8, 2.4e-7 as evaluated in fp32, like ex2.approx. Below
-// 2^-126 the result stays there; NaN stays NaN.
+// 2^-126 the result stays there. With kNaN, NaN stays NaN; else it may come
+// out as anything.
+template <bool kNaN>
 __device__ __forceinline__ float2 ex2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
-  const float2 magic = make_float2(12582912.f, 12582912.f);
-  const float2 t = add_f32x2(x, magic);
-  const float2 n = add_f32x2(t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = fma_f32x2(n, make_float2(-1.f, -1.f), x);
+  if (kNaN) {
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  } else {
+    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  }
   auto both = [](float c) { return make_float2(c, c); };
+  const float2 t = add_f32x2(x, both(12582912.f));
+  const float2 f = fma_f32x2(add_f32x2(t, both(-12582912.f)), both(-1.f), x);
   float2 p = fma_f32x2(both(1.3276472e-3f), f, both(9.675541e-3f));
   p = fma_f32x2(p, f, both(5.550713e-2f));
   p = fma_f32x2(p, f, both(0.24022120f));
   p = fma_f32x2(p, f, both(0.69314694f));
   p = fma_f32x2(p, f, both(1.0000001f));
-  const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
-                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
-  return mul_f32x2(p, scale);
+  const uint32_t nx = __float_as_uint(t.x) << 23, ny = __float_as_uint(t.y) << 23;
+  if (kNaN) return mul_f32x2(p, make_float2(__uint_as_float(nx + 0x3f800000u), __uint_as_float(ny + 0x3f800000u)));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + nx), __uint_as_float(__float_as_uint(p.y) + ny));
 }
 
 // Units of work that one warp of a CTA works out and the others take from a
@@ -241,36 +245,6 @@ __device__ __forceinline__ void clear_tail(uint8_t* tile, int left, int lane) {
 }
 __device__ __forceinline__ bool has_tail(int n, int hi) { return hi * kTile > n && (n & 15) != 0; }
 
-// 16-byte chunks of 16-bit output rows held one row per lane, stored so that
-// each instruction writes whole row segments (the transpose of
-// store_rows_coalesced), each row at its own address; null rows are skipped.
-template <int S>
-__device__ __forceinline__ void store_rows_anywhere(uint4 (&c)[S], uint8_t* row, int lane) {
-#pragma unroll
-  for (int m = 1; m < S; m <<= 1) {
-    const bool hi = (lane & m) != 0;
-#pragma unroll
-    for (int j = 0; j < S; ++j) {
-      if (j & m) continue;
-      const uint4 snd = hi ? c[j] : c[j ^ m];
-      uint4 rcv;
-      rcv.x = __shfl_xor_sync(0xffffffffu, snd.x, m);
-      rcv.y = __shfl_xor_sync(0xffffffffu, snd.y, m);
-      rcv.z = __shfl_xor_sync(0xffffffffu, snd.z, m);
-      rcv.w = __shfl_xor_sync(0xffffffffu, snd.w, m);
-      if (hi) c[j] = rcv;
-      else c[j ^ m] = rcv;
-    }
-  }
-  const int g0 = lane & ~(S - 1), i = lane & (S - 1);
-#pragma unroll
-  for (int k = 0; k < S; ++k) {
-    uint8_t* at = reinterpret_cast<uint8_t*>(
-        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), g0 + k));
-    if (at) *reinterpret_cast<uint4*>(at + 16 * i) = c[k];
-  }
-}
-
 // 8 fp32 accumulators times `mul` as eight 16-bit values.
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const uint32_t* a, float mul) {
@@ -280,24 +254,26 @@ __device__ __forceinline__ uint4 pack8(const uint32_t* a, float mul) {
                     Elem<T>::pack(mul * __uint_as_float(a[6]), mul * __uint_as_float(a[7])));
 }
 
-// Columns [32 x, 32 x + 32) of each lane's row, times `mul`, as fp32 or as
-// 16-bit with the warp's rows transposed for whole segments a store.
-template <typename T>
-__device__ __forceinline__ void store_row_32(bool fp32, uint8_t* row, int x, uint32_t (&v)[32], float mul, int lane, T) {
-  if (fp32) {
-    if (row) {
+// This thread's row of D sums in TMEM, times `mul`, to its output row, fp32 or
+// 16-bit (null: no row).
+template <typename T, int D>
+__device__ __forceinline__ void store_sums(uint32_t taddr, bool fp32, uint8_t* row, float mul) {
+#pragma unroll 1
+  for (int x = 0; x < D / 16; ++x) {
+    uint32_t v[16];
+    __syncwarp();
+    tmem_load_16(taddr + 16 * x, v);
+    if (row == nullptr) continue;
+    if (fp32) {
 #pragma unroll
-      for (int y = 0; y < 8; ++y)
-        reinterpret_cast<float4*>(row + 128 * x)[y] =
+      for (int y = 0; y < 4; ++y)
+        reinterpret_cast<float4*>(row + 64 * x)[y] =
             make_float4(mul * __uint_as_float(v[4 * y]), mul * __uint_as_float(v[4 * y + 1]),
                         mul * __uint_as_float(v[4 * y + 2]), mul * __uint_as_float(v[4 * y + 3]));
+    } else {
+      reinterpret_cast<uint4*>(row + 32 * x)[0] = pack8<T>(v, mul);
+      reinterpret_cast<uint4*>(row + 32 * x)[1] = pack8<T>(v + 8, mul);
     }
-    __syncwarp();
-  } else {
-    uint4 ch[4];
-#pragma unroll
-    for (int y = 0; y < 4; ++y) ch[y] = pack8<T>(v + 8 * y, mul);
-    store_rows_anywhere<4>(ch, row ? row + 64 * x : nullptr, lane);
   }
 }
 
@@ -319,21 +295,15 @@ __device__ __forceinline__ void mask_columns(uint32_t taddr, int left) {
   tmem_store_wait();
 }
 
-// 32 weights of a row: p = 2^(s sl2 - m), every fourth pair by polynomial,
-// summed into l and packed. (The polynomial makes 2^-126 of a masked -inf: in
-// the sum that is nothing, and the products do not reach its key or find 0 in V.)
+// 32 weights of a row: p = 2^(s sl2 - m), summed into l and packed.
 template <typename T>
 __device__ __forceinline__ void weights_32(const uint32_t* s, float2 sc, float2 nm, float2& l0, float2& l1,
                                            uint32_t (&e)[16]) {
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
     float2 a = fma_f32x2(make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), sc, nm);
-    if ((x & 3) == 3) {
-      a = ex2_poly(a);
-    } else {
-      a.x = ex2_approx(a.x);
-      a.y = ex2_approx(a.y);
-    }
+    a.x = ex2_approx(a.x);
+    a.y = ex2_approx(a.y);
     if (x & 1) l1 = add_f32x2(l1, a);
     else l0 = add_f32x2(l0, a);
     e[x] = Elem<T>::pack(a.x, a.y);
@@ -450,7 +420,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
       }
       __syncwarp();
     } else if (warp == 14) {
-      if (elect_one()) feed_fwd(p, ring, unit_full, unit_empty, ctx);
+      if (lane == 0) feed_fwd(p, ring, unit_full, unit_empty, ctx);
       __syncwarp();
     } else {
       // ---- MMA issuer of tile t: S_(j+1) behind PV_j, for each item in turn.
@@ -610,7 +580,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     // last V tile behind the last key, for the issuers that wait for it.
     regs_lower<Cfg::kOtherRegs>();
     const int r = threadIdx.x & 127;
-    int nst[2] = {0, 0}, no[2] = {0, 0}, g = 0;
+    int nst0 = 0, nst1 = 0, no0 = 0, no1 = 0, g = 0;
     const int64_t all_rows = static_cast<int64_t>(p.B) * p.rows.S * p.Hkv * p.rows.G * p.rows.M;
     uint32_t tail_turns = 0;  // a bit for each slot
     while (get_unit<true>(ring, unit_full, unit_empty, k, ua, ub, ctx, 240, ok)) {
@@ -628,18 +598,20 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
           if (ok && lane == 0) mbar_arrive(&bar[kFwKVFull0 + slot]);
         }
       }
-#pragma unroll
+#pragma unroll 1
       for (int t = 0; t < 2; ++t) {
         if (t == 1 && !it.two) continue;
-        if (ok && !mbar_wait(&bar[kFwStFull0 + t], nst[t] & 1, ctx, 242)) ok = false;
+        if (ok && !mbar_wait(&bar[kFwStFull0 + t], (t == 0 ? nst0 : nst1) & 1, ctx, 242)) ok = false;
         if (!ok) break;
-        ++nst[t];
+        if (t == 0) ++nst0;
+        else ++nst1;
         const float2 ml = stat[128 * t + r];
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[kFwStEmpty0 + t]);
         if (keys) {
-          if (!mbar_wait(&bar[kFwOFull0 + t], no[t] & 1, ctx, 243)) { ok = false; break; }
-          ++no[t];
+          if (!mbar_wait(&bar[kFwOFull0 + t], (t == 0 ? no0 : no1) & 1, ctx, 243)) { ok = false; break; }
+          if (t == 0) ++no0;
+          else ++no1;
         }
         __syncwarp();
         tc_fence_after();
@@ -656,13 +628,11 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         uint8_t* out = reinterpret_cast<uint8_t*>(p.partial ? reinterpret_cast<void*>(p.part_o + (it.split * all_rows + row) * D)
                                                             : reinterpret_cast<void*>(p.O.at(b, h, m)));
         if (!real) out = nullptr;
-#pragma unroll 1
-        for (int x = 0; x < D / 32; ++x) {
-          uint32_t o[32];
-#pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = 0u;
-          if (keys) tmem_load_32(tO + 32 * x, o);
-          store_row_32(p.partial, out, x, o, inv, lane, T());
+        if (keys) {
+          store_sums<T, D>(tO, p.partial, out, inv);
+        } else if (out) {  // zeros
+          const int chunks = D / (p.partial ? 4 : 8);
+          for (int x = 0; x < chunks; ++x) reinterpret_cast<uint4*>(out)[x] = make_uint4(0, 0, 0, 0);
         }
         tc_fence_before();
         __syncwarp();

@@ -274,9 +274,9 @@ int enqueue_bwd(const fmha_attn_t& a, int device, cudaStream_t stream) {
       !encode_map4(&mK, kBF16, a.K, a.K_dim, a.N, a.kv_heads, a.batch, kTile, 1, 1) ||
       !encode_map4(&mV, kBF16, a.V, a.K_dim, a.N, a.kv_heads, a.batch, kTile, 1, 1))
     return set_error(kErrInvalidArgument, "tensor map encoding failed");
-  float* lse2 = static_cast<float*>(a.workspace);
-  float* delta = lse2 + f.packed_rows;
-  float2* amax = reinterpret_cast<float2*>(delta + f.packed_rows);
+  float* nlse2 = static_cast<float*>(a.workspace);
+  float* ndelta = nlse2 + f.packed_rows;
+  float2* amax = reinterpret_cast<float2*>(ndelta + f.packed_rows);
   BwdParams<T> q;
   q.rows = f.rows;
   q.B = a.batch;
@@ -287,8 +287,8 @@ int enqueue_bwd(const fmha_attn_t& a, int device, cudaStream_t stream) {
   q.dQ = view_of<T>(a.dQ);
   q.dK = view_of<T>(a.dK);
   q.dV = view_of<T>(a.dV);
-  q.lse2 = lse2;
-  q.delta = delta;
+  q.nlse2 = nlse2;
+  q.ndelta = ndelta;
   q.amax = amax;
   q.amax_count = f.delta_blocks;
   q.part = reinterpret_cast<float*>(amax + (f.delta_blocks + 1) / 2 * 2);
@@ -302,7 +302,7 @@ int enqueue_bwd(const fmha_attn_t& a, int device, cudaStream_t stream) {
     allow_smem<attn_dq_kernel<T, D>>(DqCfg2<D>::kSmemBytes, device);
     allow_smem<attn_dkv_kernel<T, D>>(DkvCfg2<D>::kSmemBytes, device);
     attn_delta_kernel<T, D><<<f.delta_blocks, 256, 0, stream>>>(view_of<T>(a.dO), view_of<T>(a.O), view_of<T>(a.V),
-                                                               a.LSE, q, lse2, delta, amax);
+                                                               a.LSE, q, nlse2, ndelta, amax);
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
