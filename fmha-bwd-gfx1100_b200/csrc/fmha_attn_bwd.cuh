@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint8_t* out = u.slot >= 0 ? reinterpret_cast<uint8_t*>(part)
                        : real      ? reinterpret_cast<uint8_t*>(p.dQ.at(u.b, u.hk * p.rows.G + g, m))
                                    : nullptr;
-        store_sums<T, D>(tmem + 256 + D * t + (static_cast<uint32_t>(r & 96) << 16), u.slot >= 0, out,
+        store_sums<T, D, 16>(tmem + 256 + D * t + (static_cast<uint32_t>(r & 96) << 16), u.slot >= 0, out,
                          u.slot >= 0 ? 1.f : out_mul);
         tc_fence_before();
         __syncwarp();
@@ -1040,7 +1040,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint8_t* out = u.slot >= 0   ? reinterpret_cast<uint8_t*>(part)
                        : key < p.N ? reinterpret_cast<uint8_t*>(v.at(u.b, u.hk, key))
                                    : nullptr;
-        store_sums<T, D>(tmem + (which == 0 ? Cfg::kColdV : Cfg::kColdK) + lanes, u.slot >= 0, out,
+        store_sums<T, D, 32>(tmem + (which == 0 ? Cfg::kColdV : Cfg::kColdK) + lanes, u.slot >= 0, out,
                          u.slot >= 0 ? 1.f : (which == 0 ? dv_mul : dk_mul));
       }
       tc_fence_before();

@@ -175,14 +175,14 @@ struct FwdCfg {
   // * 184 + 2 * 128 * 72 registers, the 512 * 128 of the launch
   static constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
   static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs == 4 * 128, "register split");
-  static constexpr int kReaders = 15;  // of a unit: warps 0-13 and 15
+  static constexpr int kReaders = 14;  // of a unit: warps 0-13
 };
 
 enum FwdBar : int {
   kFwQFull0 = 0,    // + tile
   kFwQEmpty0 = 2,   // + tile: the item's last S of the tile is done
   kFwKVFull0 = 4,   // + slot (up to 8)
-  kFwKVEmpty0 = 12, // + slot: both MMA issuers are done with it
+  kFwKVEmpty0 = 12, // + slot
   kFwTail0 = 20,    // + slot: a last V tile has landed, its rows behind the keys not yet cleared
   kFwSFull0 = 28,   // + tile
   kFwPFull0 = 30,   // + tile: the first 96 columns of p written (4 warps)
@@ -193,8 +193,8 @@ enum FwdBar : int {
   kFwStEmpty0 = 40, // + tile: and read (4 warps)
   kFwUnitFull0 = 42,
   kFwUnitEmpty0 = 46,
-  kFwDrain0 = 50,   // + tile
-  kNumFwdBars = 52,
+  kFwDrain = 50,
+  kNumFwdBars = 51,
 };
 static_assert(kNumFwdBars * 8 + 8 <= 512, "barrier area");
 
@@ -254,25 +254,40 @@ __device__ __forceinline__ uint4 pack8(const uint32_t* a, float mul) {
                     Elem<T>::pack(mul * __uint_as_float(a[6]), mul * __uint_as_float(a[7])));
 }
 
+// 32 bytes of one thread's row: one store where the row allows it.
+__device__ __forceinline__ void store_32_bytes(uint8_t* at, const uint4& a, const uint4& b) {
+  if ((reinterpret_cast<uintptr_t>(at) & 31u) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(a.x), "r"(a.y), "r"(a.z),
+                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(at)[0] = a;
+    reinterpret_cast<uint4*>(at)[1] = b;
+  }
+}
+
 // This thread's row of D sums in TMEM, times `mul`, to its output row, fp32 or
-// 16-bit (null: no row).
-template <typename T, int D>
+// 16-bit (null: no row), C columns at a time.
+template <typename T, int D, int C>
 __device__ __forceinline__ void store_sums(uint32_t taddr, bool fp32, uint8_t* row, float mul) {
 #pragma unroll 1
-  for (int x = 0; x < D / 16; ++x) {
-    uint32_t v[16];
+  for (int x = 0; x < D; x += C) {
+    uint32_t v[C];
     __syncwarp();
-    tmem_load_16(taddr + 16 * x, v);
+    if constexpr (C == 32) tmem_load_32(taddr + x, v);
+    else tmem_load_16(taddr + x, v);
     if (row == nullptr) continue;
     if (fp32) {
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
-        reinterpret_cast<float4*>(row + 64 * x)[y] =
-            make_float4(mul * __uint_as_float(v[4 * y]), mul * __uint_as_float(v[4 * y + 1]),
-                        mul * __uint_as_float(v[4 * y + 2]), mul * __uint_as_float(v[4 * y + 3]));
+      for (int y = 0; y < C; ++y) v[y] = __float_as_uint(mul * __uint_as_float(v[y]));
+#pragma unroll
+      for (int y = 0; y < C; y += 8)
+        store_32_bytes(row + 4 * (x + y), make_uint4(v[y], v[y + 1], v[y + 2], v[y + 3]),
+                       make_uint4(v[y + 4], v[y + 5], v[y + 6], v[y + 7]));
     } else {
-      reinterpret_cast<uint4*>(row + 32 * x)[0] = pack8<T>(v, mul);
-      reinterpret_cast<uint4*>(row + 32 * x)[1] = pack8<T>(v + 8, mul);
+#pragma unroll
+      for (int y = 0; y < C; y += 16)
+        store_32_bytes(row + 2 * (x + y), pack8<T>(v + y, mul), pack8<T>(v + y + 8, mul));
     }
   }
 }
@@ -334,9 +349,8 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kNumFwdBars; ++i) {
       int count = 1;
-      if (i >= kFwKVEmpty0 && i < kFwTail0) count = 2;
       if ((i >= kFwPFull0 && i < kFwOFull0) || (i >= kFwOEmpty0 && i < kFwUnitFull0)) count = 4;
-      if (i >= kFwUnitEmpty0 && i < kFwDrain0) count = Cfg::kReaders;
+      if (i >= kFwUnitEmpty0 && i < kFwDrain) count = Cfg::kReaders;
       mbar_init(&bar[i], count);
     }
     *abort_flag = 0;
@@ -422,68 +436,84 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     } else if (warp == 14) {
       if (lane == 0) feed_fwd(p, ring, unit_full, unit_empty, ctx);
       __syncwarp();
-    } else {
-      // ---- MMA issuer of tile t: S_(j+1) behind PV_j, for each item in turn.
-      // The pipe takes only about a product ahead, so a thread for each tile
-      // keeps one tile's wait from holding up the other's products.
-      const int t = warp == 13 ? 0 : 1;
+    } else if (warp == 13) {
+      // ---- MMA. Per step, for each tile in turn: O += p V_j, then S of the
+      // next step (of the next item, after the last one), which keeps the two
+      // tiles half a step apart: with an issuer for each tile they drifted
+      // into step and fought for the SFU and the tensor core by turns (357
+      // against 327 us at 16384 rows, 1024 keys, 40 heads of 128).
       if (elect_one()) {
         constexpr uint32_t id_S = make_idesc_f16<kB>(kTile, kTile, false, false);
         constexpr uint32_t id_O = make_idesc_f16<kB>(kTile, D, false, true);
-        const uint32_t sKV = smem_u32(smem + Cfg::kOffKV);
-        const uint64_t dq = make_sw128_desc(smem_u32(smem + Cfg::kOffQ + t * Cfg::kTileBytes), 16, 1024);
-        const uint32_t tS = tmem + Cfg::kColS + 128 * t, tO = tmem + Cfg::kColO + D * t;
-        int slot = 0, turn = 0, nq = 0, np = 0;
-        auto advance = [&](int n) {
-          slot += n;
-          while (slot >= kSlots) {
-            slot -= kSlots;
+        const uint32_t sKV = smem_u32(smem + Cfg::kOffKV), sQ = smem_u32(smem + Cfg::kOffQ);
+        int slot = 0, turn = 0;
+        uint32_t turns = 0;  // bits: Q 0, 1; p 2, 3; O 4, 5; whether O was used 6, 7
+        auto advance = [&] {
+          if (++slot == kSlots) {
+            slot = 0;
             turn ^= 1;
           }
         };
-        auto done_with = [&](bool alone) {
-          umma_commit(&bar[kFwKVEmpty0 + slot]);
-          if (alone) umma_commit(&bar[kFwKVEmpty0 + slot]);
-          advance(1);
-        };
-        while (get_unit<false>(ring, unit_full, unit_empty, k, ua, ub, ctx, 210 + 10 * t, ok)) {
-          const FwdItem it = fwd_item(ua, ub);
-          if (it.lo == it.hi) continue;
-          if (t == 1 && !it.two) {
-            advance(2 * (it.hi - it.lo));
-            continue;
+        auto next_item = [&](FwdItem& it) {
+          while (get_unit<false>(ring, unit_full, unit_empty, k, ua, ub, ctx, 210, ok)) {
+            it = fwd_item(ua, ub);
+            if (it.lo < it.hi) return true;
           }
-          ok = mbar_wait(&bar[kFwQFull0 + t], nq & 1, ctx, 211 + 10 * t);
-          for (int j = it.lo - 1; ok && j < it.hi; ++j) {
-            if (j >= it.lo) {  // O += p V_j
-              if (!(ok = mbar_wait(&bar[kFwKVFull0 + slot], turn, ctx, 212 + 10 * t))) break;
-              if (j == it.lo && nq > 0 && !(ok = mbar_wait(&bar[kFwOEmpty0 + t], (nq - 1) & 1, ctx, 213 + 10 * t))) break;
-              if (!(ok = mbar_wait(&bar[kFwPFull0 + t], np & 1, ctx, 214 + 10 * t))) break;
+          return false;
+        };
+        FwdItem cur{}, nxt;
+        bool more = next_item(cur);
+        nxt = cur;
+        int j = cur.lo - 1;  // the step before the first has no p V
+        while (more && ok) {
+          const bool start = j < cur.lo, last = j + 1 == cur.hi;
+          if (last) more = next_item(nxt);
+          if (!ok) break;
+          const int jn = last ? nxt.lo : j + 1, vslot = slot;
+          if (!start) {
+            if (!(ok = mbar_wait(&bar[kFwKVFull0 + slot], turn, ctx, 212))) break;
+            advance();
+          }
+          if (more && !(ok = mbar_wait(&bar[kFwKVFull0 + slot], turn, ctx, 216))) break;
+#pragma unroll 1
+          for (int t = 0; t < 2; ++t) {
+            const uint32_t tS = tmem + Cfg::kColS + 128 * t, tO = tmem + Cfg::kColO + D * t;
+            if (!start && (t == 0 || cur.two)) {
+              if (j == cur.lo) {
+                if ((turns >> (6 + t) & 1) && !(ok = mbar_wait(&bar[kFwOEmpty0 + t], (turns >> (4 + t) & 1) ^ 1, ctx, 213))) break;
+                turns = (turns ^ (1u << (4 + t))) | 1u << (6 + t);
+              }
+              const uint32_t par = turns >> (2 + t) & 1, keep = j > cur.lo ? 1u : 0u;
+              if (!(ok = mbar_wait(&bar[kFwPFull0 + t], par, ctx, 214))) break;
               tc_fence_after();
-              const uint64_t dv = make_sw128_desc(sKV + slot * Cfg::kTileBytes, kBoxBytes, 1024);
-              const uint32_t keep = j > it.lo ? 1u : 0u;
-              const int left = it.n - j * kTile;
+              const uint64_t dv = make_sw128_desc(sKV + vslot * Cfg::kTileBytes, kBoxBytes, 1024);
+              const int left = cur.n - j * kTile;
               if (left >= kTile) {
 #pragma unroll
                 for (int x = 0; x < 6; ++x)
                   umma_f16_ts(tO, tS + x * 8, desc_advance(dv, x * 2048), id_O, x > 0 ? 1u : keep);
-                if (!(ok = mbar_wait(&bar[kFwPRest0 + t], np & 1, ctx, 215 + 10 * t))) break;
+                if (!(ok = mbar_wait(&bar[kFwPRest0 + t], par, ctx, 215))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int x = 6; x < 8; ++x) umma_f16_ts(tO, tS + x * 8, desc_advance(dv, x * 2048), id_O, 1u);
               } else {
-                if (!(ok = mbar_wait(&bar[kFwPRest0 + t], np & 1, ctx, 215 + 10 * t))) break;
+                if (!(ok = mbar_wait(&bar[kFwPRest0 + t], par, ctx, 215))) break;
                 tc_fence_after();
+#pragma unroll 1
                 for (int x = 0; x < (left + 15) / 16; ++x)
                   umma_f16_ts(tO, tS + x * 8, desc_advance(dv, x * 2048), id_O, x > 0 ? 1u : keep);
               }
-              ++np;
-              done_with(!it.two);
-              if (j + 1 == it.hi) umma_commit(&bar[kFwOFull0 + t]);
+              turns ^= 4u << t;
+              if (last) umma_commit(&bar[kFwOFull0 + t]);
             }
-            if (j + 1 < it.hi) {  // S = Q K_(j+1)^T
-              if (!(ok = mbar_wait(&bar[kFwKVFull0 + slot], turn, ctx, 216 + 10 * t))) break;
+            if (t == 1 && !start) umma_commit(&bar[kFwKVEmpty0 + vslot]);
+            if (more && (t == 0 || nxt.two)) {
+              if (jn == nxt.lo) {
+                if (!(ok = mbar_wait(&bar[kFwQFull0 + t], turns >> t & 1, ctx, 211))) break;
+                turns ^= 1u << t;
+              }
               tc_fence_after();
+              const uint64_t dq = make_sw128_desc(sQ + t * Cfg::kTileBytes, 16, 1024);
               const uint64_t dk = make_sw128_desc(sKV + slot * Cfg::kTileBytes, 16, 1024);
 #pragma unroll
               for (int x = 0; x < D / 16; ++x) {
@@ -491,15 +521,18 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
                 umma_f16_ss(tS, desc_advance(dq, off), desc_advance(dk, off), id_S, x > 0 ? 1u : 0u);
               }
               umma_commit(&bar[kFwSFull0 + t]);
-              if (j + 2 == it.hi) umma_commit(&bar[kFwQEmpty0 + t]);
-              done_with(!it.two);
+              if (jn + 1 == nxt.hi) umma_commit(&bar[kFwQEmpty0 + t]);
             }
+            if (t == 1 && more) umma_commit(&bar[kFwKVEmpty0 + slot]);
           }
-          ++nq;
+          if (!ok) break;
+          if (more) advance();
+          cur = nxt;
+          j = jn;
         }
         if (!ok) {
-          umma_commit(&bar[kFwDrain0 + t]);
-          mbar_wait_drain(&bar[kFwDrain0 + t], 0, p.timeout_ns);
+          umma_commit(&bar[kFwDrain]);
+          mbar_wait_drain(&bar[kFwDrain], 0, p.timeout_ns);
         }
       }
       __syncwarp();
@@ -629,7 +662,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
                                                             : reinterpret_cast<void*>(p.O.at(b, h, m)));
         if (!real) out = nullptr;
         if (keys) {
-          store_sums<T, D>(tO, p.partial, out, inv);
+          store_sums<T, D, 32>(tO, p.partial, out, inv);
         } else if (out) {  // zeros
           const int chunks = D / (p.partial ? 4 : 8);
           for (int x = 0; x < chunks; ++x) reinterpret_cast<uint4*>(out)[x] = make_uint4(0, 0, 0, 0);
