@@ -62,8 +62,8 @@ struct BwdUnit {
 // Steps that a division by steps has to save, as its partial sums cost about
 // as much, and the least number of steps of a CTA under it.
 constexpr int kBwdSpare = 8, kBwdLeast = 4;
-__host__ __device__ inline bool bwd_by_steps(int64_t items, int64_t most, int64_t total, int64_t grid) {
-  return (items + grid - 1) / grid * most > (total + grid - 1) / grid + kBwdSpare;
+__host__ __device__ inline bool bwd_by_steps(int64_t whole, int64_t total, int64_t grid) {
+  return whole > (total + grid - 1) / grid + kBwdSpare;
 }
 __host__ __device__ inline int bwd_parts(int64_t total, int grid) {
   const int64_t most = (total + kBwdLeast - 1) / kBwdLeast;
@@ -91,20 +91,24 @@ struct BwdSchedule {
 
   __device__ BwdSchedule(const BwdParams<T>& params, int g, int c) : p(params), grid(g), cta(c) {
     total = items = 0;
-    int most = 0;
+    // steps of the busiest CTA with whole items: all of them as long as the
+    // longest, or the entries one after another, whichever bounds it better
+    int most = 0, apart = 0;
     if (!p.lens) {
-      most = key_tiles(0);
-      items = items_of(most) * p.B;
-      total = items * len_of(most);
+      most = len_of(key_tiles(0));
+      items = items_of(key_tiles(0)) * p.B;
+      total = items * most;
+      apart = (items + grid - 1) / grid * most;
     } else {
       for (int e = 0; e < p.B; ++e) {
-        const int nt = key_tiles(e);
-        most = max(most, nt);
-        items += items_of(nt);
-        total += items_of(nt) * len_of(nt);
+        const int nt = key_tiles(e), n = items_of(nt), len = len_of(nt);
+        most = max(most, len);
+        items += n;
+        total += n * len;
+        apart += (n + grid - 1) / grid * len;
       }
     }
-    by_steps = bwd_by_steps(items, len_of(most), total, grid);
+    by_steps = bwd_by_steps(min((items + grid - 1) / grid * most, apart), total, grid);
     parts = bwd_parts(total, grid);
     pos = by_steps ? mark(c) : c;
     end = by_steps ? mark(c + 1) : items;

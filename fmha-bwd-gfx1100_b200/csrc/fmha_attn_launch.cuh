@@ -251,8 +251,8 @@ inline BwdPlan plan_bwd(const fmha_attn_t& a) {
   f.grid_q = static_cast<int>(std::min<int64_t>(kPlanSms, heads * f.pairs * nt));
   f.grid_k = static_cast<int>(std::min<int64_t>(kPlanSms, heads * f.rows.tiles * nt));
   f.join = a.kv_lens != nullptr ||
-           bwd_by_steps(heads * f.pairs, nt, heads * f.pairs * nt, f.grid_q) ||
-           bwd_by_steps(heads * nt, f.rows.tiles, heads * nt * f.rows.tiles, f.grid_k);
+           bwd_by_steps((heads * f.pairs + f.grid_q - 1) / f.grid_q * nt, heads * f.pairs * nt, f.grid_q) ||
+           bwd_by_steps((heads * nt + f.grid_k - 1) / f.grid_k * f.rows.tiles, heads * nt * f.rows.tiles, f.grid_k);
   f.packed_rows = heads * f.rows.tiles * kTile;
   f.delta_blocks = static_cast<int>(std::min<int64_t>(6 * kPlanSms, heads * std::max<int64_t>(f.rows.tiles, nt)));
   f.slot_floats = 2 * static_cast<int64_t>(kTile) * a.K_dim;
