@@ -120,34 +120,71 @@ int enqueue_fwd(const fmha_attn_t& a, const FwdPlan& f, const fmha_tensor_t& K, 
   return kOk;
 }
 
-// How few-row attention divides its work: 8 or 16 rows a block, and the
-// number of blocks that share a kv head's keys.
+// How few-row attention divides its work: 8 or 16 rows a block, and either a
+// cluster of `splits` blocks to a kv head's keys or, `blocks` > 0, that many
+// blocks to equal runs of the whole batch (see DecodeParams).
 struct DecodePlan {
-  int R, row_tiles, splits;
+  int R, row_tiles, splits, blocks, side, sub;
   int64_t tasks;
+  uint64_t ws_bytes;
 };
 
-// Of 1 to 16 blocks a tile of rows, the number with the least estimated time:
-// waves of blocks (kDecodeSlots on the GPU at a time) times a block's steps of
-// 64 keys plus its fixed costs, which measure like kDecodeFixed such steps.
-constexpr int kDecodeSlots = 4 * kPlanSms, kDecodeFixed = 4;
-inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N) {
+// Stream: evens out lengths and reads at 6.1 TB/s, but costs a second launch
+// and some 15 us in all to fill, drain and join, so from kStreamBytes of keys
+// and values on. Clusters read at 4.9 (D = 128) and 6.5 TB/s (D = 64) at 7 us:
+// at 64 columns they stay ahead (71 against 79 us for 64 x 1500 keys of 16
+// heads) until the lengths can differ much (kStreamKeys); at 128 columns 16 x
+// 4000 keys of 8 heads take 63 us in clusters and 51 us streamed. Blocks of a
+// cluster: of 1 to 16 a tile of rows, the number with the least estimated time:
+// waves of blocks times a block's steps of 64 keys plus its fixed costs, which
+// measure like kDecodeFixed such steps. `parts`: the caller's parts join in the
+// cluster's launch.
+constexpr int kDecodeFixed = 4, kStreamKeys = 8192;
+constexpr int64_t kStreamBytes = 96ll << 20;
+inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N, int D, bool parts) {
   DecodePlan d;
   const int64_t rows = static_cast<int64_t>(G) * M;
   d.R = rows <= 8 ? 1 : 2;
   d.row_tiles = static_cast<int>((rows + 8 * d.R - 1) / (8 * d.R));
   d.tasks = static_cast<int64_t>(B) * Hkv * d.row_tiles;
-  const int64_t steps = (N + 16 * kDecodeWarps - 1) / (16 * kDecodeWarps);
-  d.splits = 1;
+  d.splits = d.side = d.sub = 1;
+  d.blocks = 0;
+  d.ws_bytes = 0;
+  const int64_t tiles = (static_cast<int64_t>(N) + 15) / 16;
+  if (!parts && d.tasks * N * D * 4 >= kStreamBytes && (D == 128 || N >= kStreamKeys) && d.tasks * tiles < (1ll << 30)) {
+    const int warps = D == 128 ? (d.R == 1 ? StreamCfg<128, 1>::kWarps : StreamCfg<128, 2>::kWarps)
+                               : (d.R == 1 ? StreamCfg<64, 1>::kWarps : StreamCfg<64, 2>::kWarps);
+    // as many items side by side as leave the fewest warps without one
+    const int items = Hkv * d.row_tiles;
+    int best = warps;
+    for (int side = warps; side >= 1; --side) {
+      if (warps % side != 0) continue;
+      const int idle = (items + side - 1) / side * side - items;
+      const int64_t spent = static_cast<int64_t>(items + idle) * ((tiles + warps / side - 1) / (warps / side)) * (warps / side);
+      const int64_t least = static_cast<int64_t>((items + best - 1) / best * best) *
+                            ((tiles + warps / best - 1) / (warps / best)) * (warps / best);
+      if (spent < least) best = side;
+    }
+    d.side = best;
+    d.sub = warps / best;
+    d.blocks = kPlanSms;
+    d.ws_bytes = 2ull * d.blocks * d.side * 8 * d.R * (D * 4 + 8);
+    return d;
+  }
+  const int64_t steps = (static_cast<int64_t>(N) + 63) / 64;
+  const int64_t slots = (D == 128 ? (d.R == 1 ? 3 : 2) : (d.R == 1 ? 5 : 4)) * kPlanSms;  // by registers
   int64_t best = 0;
-  for (int s = 1; s <= 16 && s <= steps; s *= 2) {
-    const int64_t cost = (d.tasks * s + kDecodeSlots - 1) / kDecodeSlots * ((steps + s - 1) / s + kDecodeFixed);
+  for (int s = 1; s <= kMostSplits && s <= steps; s *= 2) {
+    const int64_t cost = (d.tasks * s + slots - 1) / slots * ((steps + s - 1) / s + kDecodeFixed);
     if (s == 1 || cost < best) {
       best = cost;
       d.splits = s;
     }
   }
   return d;
+}
+inline DecodePlan plan_decode(const fmha_attn_t& a, bool parts) {
+  return plan_decode(a.M, a.q_heads / a.kv_heads, a.batch, a.kv_heads, a.N, a.K_dim, parts);
 }
 
 // Up to this many query rows a kv head go through attn_decode_kernel.
@@ -162,7 +199,7 @@ inline bool is_decode(const fmha_attn_t& a) {
 template <typename T>
 int enqueue_decode(const fmha_attn_t& a, bool prefix, int parts, int64_t all_rows, int device, cudaStream_t stream) {
   const int G = a.q_heads / a.kv_heads;
-  const DecodePlan d = plan_decode(a.M, G, a.batch, a.kv_heads, a.N);
+  const DecodePlan d = plan_decode(a, prefix);
   DecodeParams<T> p;
   p.Q = view_of<T>(a.Q);
   p.K = view_of<T>(a.K);
@@ -183,6 +220,22 @@ int enqueue_decode(const fmha_attn_t& a, bool prefix, int parts, int64_t all_row
   p.all_rows = all_rows;
   p.part_o = parts > 0 ? static_cast<const float*>(a.workspace) : nullptr;
   p.part_lse = parts > 0 ? p.part_o + parts * all_rows * a.K_dim : nullptr;
+  CUtensorMap mK, mV;
+  if (d.blocks > 0) {
+    if (!encode_fn()) return set_error(kErrNoDriver, "cuTensorMapEncodeTiled is unavailable");
+    p.status = attn_status(device);
+    if (!p.status) return kErrOutOfMemory;
+    p.timeout_ns = effective_timeout_ns();
+    constexpr bool kBF16 = Elem<T>::kBF16;
+    if (!encode_map4(&mK, kBF16, a.K, a.K_dim, a.N, a.kv_heads, a.batch, 16, 1, 1) ||
+        !encode_map4(&mV, kBF16, a.V, a.K_dim, a.N, a.kv_heads, a.batch, 16, 1, 1))
+      return set_error(kErrInvalidArgument, "tensor map encoding failed");
+  }
+  p.blocks = d.blocks;
+  p.side = d.side;
+  p.sub = d.sub;
+  p.run_o = static_cast<float*>(a.workspace);
+  p.run_ml = reinterpret_cast<float2*>(p.run_o + 2ll * d.blocks * d.side * 8 * d.R * a.K_dim);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(d.tasks * d.splits));
   cfg.blockDim = dim3(32 * kDecodeWarps);
@@ -202,6 +255,17 @@ int enqueue_decode(const fmha_attn_t& a, bool prefix, int parts, int64_t all_row
   cfg.attrs = at;
   auto go = [&](auto dim, auto r) {
     constexpr int D = decltype(dim)::value, R = decltype(r)::value;
+    if (d.blocks > 0) {
+      using Cfg = StreamCfg<D, R>;
+      allow_smem<attn_decode_stream_kernel<T, D, R>>(Cfg::kSmemBytes, device);
+      attn_decode_stream_kernel<T, D, R><<<d.blocks, 32 * Cfg::kWarps, Cfg::kSmemBytes, stream>>>(mK, mV, p);
+      cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.q_heads * a.M));
+      cfg.blockDim = dim3(D);
+      at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.numAttrs = 1;
+      return cudaLaunchKernelEx(&cfg, attn_decode_join_kernel<T, D, R>, p);
+    }
     constexpr auto kernel = attn_decode_kernel<T, D, R>;
     static std::atomic<bool> done[64];
     if (device >= 64 || !done[device].load()) {
@@ -336,7 +400,7 @@ inline int attn_workspace(const fmha_attn_t& a, AttnOp op, uint64_t* bytes) {
   const int rc = check_attn_sizes(a, op);
   if (rc != kOk) return rc;
   *bytes = 0;
-  if (op == AttnOp::kCrossFwd && !is_decode(a)) *bytes = cross_plan(a).ws_bytes;
+  if (op == AttnOp::kCrossFwd) *bytes = is_decode(a) ? plan_decode(a, false).ws_bytes : cross_plan(a).ws_bytes;
   if (op == AttnOp::kPrefix) *bytes = prefix_plan(a).ws_bytes;
   if (op == AttnOp::kCrossBwd) *bytes = plan_bwd(a).ws_bytes;
   return kOk;

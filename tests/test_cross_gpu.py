@@ -93,6 +93,31 @@ def test_forward(F, B, Hq, Hkv, M, N, d, name, lens, layout, std):
     assert O.dtype == Q.dtype and LSE.dtype == torch.float32
 
 
+# single tokens over caches large enough to be read as one stream: items that do
+# and do not divide among a block's warps, 8 and 16 rows, empty and short entries
+# between long ones, several entries to a block and several blocks to an entry
+LONG = [
+    (3, 20, 4, 1, 16400, 128, "bf16", [16400, 0, 9000]),
+    (5, 10, 10, 1, 8200, 64, "fp16", [8200, 1, 0, 4097, 8191]),
+    (2, 55, 5, 1, 25000, 128, "fp16", [24999, 16]),
+    (1, 13, 13, 1, 40000, 64, "bf16", None),
+    (40, 7, 1, 2, 5000, 128, "bf16", [5000 - 131 * i for i in range(38)] + [0, 5000]),
+    (2, 11, 11, 1, 9000, 128, "fp16", [3, 17]),
+    (1, 1, 1, 1, 200000, 128, "bf16", [199999]),
+]
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,M,N,d,name,lens", LONG)
+def test_long_caches(F, B, Hq, Hkv, M, N, d, name, lens):
+    Q, K, V, n = make(B, Hq, Hkv, M, N, d, name, lens, seed=18)
+    O, LSE = F.cross_attn_fwd(Q, K, V, n)
+    ref, lse, bound, lse_bound = R.forward(Q, K, V, n, d ** -0.5)
+    R.check("O", O, ref, bound)
+    R.check("LSE", LSE, lse, lse_bound)
+    again = F.cross_attn_fwd(Q, K, V, n)
+    assert torch.equal(O, again[0]) and torch.equal(LSE, again[1])
+
+
 def saved(Q, K, V, n, scale):
     """O and LSE of a right forward, rounded to their types."""
     ref, lse, _, _ = R.forward(Q, K, V, n, scale)
