@@ -272,14 +272,16 @@ __device__ __forceinline__ void decode_output(const DecodeParams<T>& p, int b, i
 }
 
 // ------------------------------------------------------------------- clusters
-constexpr int kMostSplits = 16, kDecodeWarps = 4;
+constexpr int kMostSplits = 16, kDecodeWarps = 4, kMostParts = 160;
+// Blocks that an SM holds at a time.
+__host__ __device__ constexpr int decode_blocks(int D, int R) { return D == 128 ? (R == 1 ? 3 : 2) : (R == 1 ? 5 : 4); }
 
 template <typename T, int D, int R>
-__global__ void __launch_bounds__(32 * kDecodeWarps) attn_decode_kernel(const __grid_constant__ DecodeParams<T> p) {
+__global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R)) attn_decode_kernel(const __grid_constant__ DecodeParams<T> p) {
   constexpr int kRows = 8 * R, W = kDecodeWarps, kThreads = 32 * W;
   __shared__ __align__(16) float sum_o[W][kRows][D];
   __shared__ float warp_m[W][kRows], warp_l[W][kRows], block_m[kRows], block_l[kRows];
-  __shared__ float weight[kMostSplits][kRows], total[kRows], top_of[kRows];
+  __shared__ float weight[kMostSplits][kRows], total[kRows], top_of[kRows], part_weight[kMostParts][kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % p.splits;
@@ -403,42 +405,56 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) attn_decode_kernel(const __
     }
     __syncthreads();
   }
-  if (p.part_o) asm volatile("griddepcontrol.wait;" ::: "memory");  // the launch that wrote the parts
+  if (p.splits == 1 && threadIdx.x < kRows) {
+    top_of[threadIdx.x] = block_m[threadIdx.x];
+    total[threadIdx.x] = block_l[threadIdx.x];
+    weight[0][threadIdx.x] = 1.f;
+  }
+  if (p.parts > 0) {
+    // the parts' LSE, a thread each, then their weights. A part is normalised:
+    // its sum is 1 at the reference LSE log2e.
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the launch that wrote them
+    for (int e = threadIdx.x; e < p.parts * real; e += kThreads) {
+      const int q = row0 + e % real;
+      const int64_t id = (static_cast<int64_t>(b) * p.Hkv * p.G + hk * p.G + q / p.M) * p.M + q % p.M;
+      part_weight[e / real][e % real] = __ldcg(p.part_lse + e / real * p.all_rows + id) * kLog2e;
+    }
+    __syncthreads();
+    if (threadIdx.x < real) {
+      const int row = threadIdx.x;
+      float top = top_of[row];
+      for (int y = 0; y < p.parts; ++y) top = fmaxf(top, part_weight[y][row]);
+      const float keep = ex2_approx(top_of[row] - top);
+      float sum = keep * total[row];
+      for (int y = 0; y < p.parts; ++y) {
+        const float f = ex2_approx(part_weight[y][row] - top);
+        part_weight[y][row] = f;
+        sum += f;
+      }
+      for (int y = 0; y < p.splits; ++y) weight[y][row] *= keep;
+      top_of[row] = top;
+      total[row] = sum;
+    }
+  }
+  __syncthreads();
   // ---- the blocks' sums, and the parts: each block finishes a share
   for (int e = threadIdx.x * p.splits + split; e < real * (D / 4); e += p.splits * kThreads) {
     const int row = e / (D / 4), c = e % (D / 4);
     const int q = row0 + row;
-    float m, sum;
-    float4 acc;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.splits == 1) {
-      m = block_m[row];
-      sum = block_l[row];
-      acc = sum4(row, c);
+      add_weighted(acc, weight[0][row], sum4(row, c));
     } else {
-      m = top_of[row];
-      sum = total[row];
-      acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (int y = 0; y < p.splits; ++y) add_weighted(acc, weight[y][row], load_cluster4(&sum_o[0][row][4 * c], y));
     }
     if (p.parts > 0) {
-      // a part is normalised: its sum is 1 at the reference LSE log2e
       const int64_t id = (static_cast<int64_t>(b) * p.Hkv * p.G + hk * p.G + q / p.M) * p.M + q % p.M;
-      float top = m;
-#pragma unroll 4
-      for (int y = 0; y < p.parts; ++y) top = fmaxf(top, __ldcg(p.part_lse + y * p.all_rows + id) * kLog2e);
-      const float keep = ex2_approx(m - top);
-      m = top;
-      sum *= keep;
-      acc = make_float4(keep * acc.x, keep * acc.y, keep * acc.z, keep * acc.w);
-#pragma unroll 4
-      for (int y = 0; y < p.parts; ++y) {
-        const float f = ex2_approx(fmaf(__ldcg(p.part_lse + y * p.all_rows + id), kLog2e, -top));
-        sum += f;
-        add_weighted(acc, f, __ldcg(reinterpret_cast<const float4*>(p.part_o + (y * p.all_rows + id) * D) + c));
-      }
+      const float4* at = reinterpret_cast<const float4*>(p.part_o + id * D) + c;
+#pragma unroll 6
+      for (int y = 0; y < p.parts; ++y) add_weighted(acc, part_weight[y][row], __ldcg(at + y * p.all_rows * (D / 4)));
     }
-    decode_output(p, b, hk, q, c, m, sum, acc);
+    decode_output(p, b, hk, q, c, top_of[row], total[row], acc);
   }
   if (p.splits > 1) cluster_sync();  // no block leaves while its sums are read
 }

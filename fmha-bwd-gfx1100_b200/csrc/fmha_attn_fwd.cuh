@@ -292,6 +292,31 @@ __device__ __forceinline__ void store_sums(uint32_t taddr, bool fp32, uint8_t* r
   }
 }
 
+// O and LSE of row `tok` of head g and entry s of an item's tile, from the
+// sums in TMEM at taddr, their total l and its reference m; or a part of them.
+template <typename T, int D>
+__device__ __forceinline__ void store_tile(const FwdParams<T>& p, const FwdItem& it, uint32_t taddr, int tok, int g, int s,
+                                           bool real, float m, float l) {
+  const bool keys = it.lo < it.hi;
+  const int64_t all_rows = static_cast<int64_t>(p.B) * p.rows.S * p.Hkv * p.rows.G * p.rows.M;
+  const int b = it.b * p.rows.S + s, h = it.hk * p.rows.G + g;
+  // a sum of 0 has no keys behind it, or scores of -inf alone
+  const float inv = keys && l != 0.f ? 1.f / l : 0.f;
+  const float lse = keys ? (m + log2f(l)) * kLn2 : -INFINITY;
+  const int64_t row = (static_cast<int64_t>(b) * p.Hkv * p.rows.G + h) * p.rows.M + tok;
+  if (real) *(p.partial ? p.part_lse + it.split * all_rows + row : p.LSE + row) = lse;
+  // bytes of this row's output, fp32 or 16-bit; null where there is no row
+  uint8_t* out = reinterpret_cast<uint8_t*>(p.partial ? reinterpret_cast<void*>(p.part_o + (it.split * all_rows + row) * D)
+                                                      : reinterpret_cast<void*>(p.O.at(b, h, tok)));
+  if (!real) out = nullptr;
+  if (keys) {
+    store_sums<T, D, 32>(taddr, p.partial, out, inv);
+  } else if (out) {  // zeros
+    const int chunks = D / (p.partial ? 4 : 8);
+    for (int x = 0; x < chunks; ++x) reinterpret_cast<uint4*>(out)[x] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // The instruction caches hold little next to these kernels' unrolled loops, and
 // straight-line code that runs once an item is fetched at some 50 cycles a
 // line: what is not the inner loop is kept short and rolled.
@@ -545,7 +570,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     const uint32_t tS = tmem + Cfg::kColS + 128 * t + (static_cast<uint32_t>(r & 96) << 16);
     const uint32_t tO = tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16);
     const float sl2 = p.scale * kLog2e;
-    int ns = 0, nst = 0;
+    int ns = 0, nst = 0, no = 0;
     while (get_unit<true>(ring, unit_full, unit_empty, k, ua, ub, ctx, 230, ok)) {
       const FwdItem it = fwd_item(ua, ub);
       if (t == 1 && !it.two) continue;
@@ -602,6 +627,22 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         }
       }
       if (!ok) continue;
+      if (p.partial) {
+        // parts: few items a CTA, so nothing to get on with meanwhile
+        if (it.lo < it.hi) {
+          if (!mbar_wait(&bar[kFwOFull0 + t], no & 1, ctx, 233)) { ok = false; continue; }
+          ++no;
+        }
+        __syncwarp();
+        tc_fence_after();
+        int tok, g, s;
+        const bool real = p.rows.row(it.tile0 + t, r, tok, g, s);
+        store_tile<T, D>(p, it, tO, tok, g, s, real, m, (l0.x + l0.y) + (l1.x + l1.y));
+        tc_fence_before();
+        __syncwarp();
+        if (it.lo < it.hi && lane == 0) mbar_arrive(&bar[kFwOEmpty0 + t]);
+        continue;
+      }
       if (nst > 0 && !mbar_wait(&bar[kFwStEmpty0 + t], (nst - 1) & 1, ctx, 232)) { ok = false; continue; }
       stat[128 * t + r] = make_float2(m, (l0.x + l0.y) + (l1.x + l1.y));
       ++nst;
@@ -614,7 +655,6 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     regs_lower<Cfg::kOtherRegs>();
     const int r = threadIdx.x & 127;
     int nst0 = 0, nst1 = 0, no0 = 0, no1 = 0, g = 0;
-    const int64_t all_rows = static_cast<int64_t>(p.B) * p.rows.S * p.Hkv * p.rows.G * p.rows.M;
     uint32_t tail_turns = 0;  // a bit for each slot
     while (get_unit<true>(ring, unit_full, unit_empty, k, ua, ub, ctx, 240, ok)) {
       const FwdItem it = fwd_item(ua, ub);
@@ -633,7 +673,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
       }
 #pragma unroll 1
       for (int t = 0; t < 2; ++t) {
-        if (t == 1 && !it.two) continue;
+        if ((t == 1 && !it.two) || p.partial) continue;
         if (ok && !mbar_wait(&bar[kFwStFull0 + t], (t == 0 ? nst0 : nst1) & 1, ctx, 242)) ok = false;
         if (!ok) break;
         if (t == 0) ++nst0;
@@ -650,23 +690,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         tc_fence_after();
         int m, g, s;
         const bool real = p.rows.row(it.tile0 + t, r, m, g, s);
-        const int b = it.b * p.rows.S + s, h = it.hk * p.rows.G + g;
-        // a sum of 0 has no keys behind it, or scores of -inf alone
-        const float inv = keys && ml.y != 0.f ? 1.f / ml.y : 0.f;
-        const float lse = keys ? (ml.x + log2f(ml.y)) * kLn2 : -INFINITY;
-        const int64_t row = (static_cast<int64_t>(b) * p.Hkv * p.rows.G + h) * p.rows.M + m;
-        const uint32_t tO = tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16);
-        if (real) *(p.partial ? p.part_lse + it.split * all_rows + row : p.LSE + row) = lse;
-        // bytes of this row's output, 16-bit or fp32; null where there is no row
-        uint8_t* out = reinterpret_cast<uint8_t*>(p.partial ? reinterpret_cast<void*>(p.part_o + (it.split * all_rows + row) * D)
-                                                            : reinterpret_cast<void*>(p.O.at(b, h, m)));
-        if (!real) out = nullptr;
-        if (keys) {
-          store_sums<T, D, 32>(tO, p.partial, out, inv);
-        } else if (out) {  // zeros
-          const int chunks = D / (p.partial ? 4 : 8);
-          for (int x = 0; x < chunks; ++x) reinterpret_cast<uint4*>(out)[x] = make_uint4(0, 0, 0, 0);
-        }
+        store_tile<T, D>(p, it, tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16), m, g, s, real, ml.x, ml.y);
         tc_fence_before();
         __syncwarp();
         if (keys && lane == 0) mbar_arrive(&bar[kFwOEmpty0 + t]);

@@ -69,6 +69,7 @@ inline FwdPlan plan_fwd(int M, int G, int S, int B, int Hkv, int N, int D, int s
   f.splits = 1;
   if (base < sms) f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / base, nt / 2)));
   f.items = static_cast<int>(base * f.splits);
+  static_assert(kPlanSms <= kMostParts, "parts that attn_decode_kernel joins");
   f.all_rows = static_cast<int64_t>(B) * S * Hkv * G * M;
   f.ws_bytes = partial || f.splits > 1 ? static_cast<uint64_t>(f.splits) * f.all_rows * (D + 1) * 4 : 0;
   return f;
@@ -172,7 +173,7 @@ inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N, int D, bool p
     return d;
   }
   const int64_t steps = (static_cast<int64_t>(N) + 63) / 64;
-  const int64_t slots = (D == 128 ? (d.R == 1 ? 3 : 2) : (d.R == 1 ? 5 : 4)) * kPlanSms;  // by registers
+  const int64_t slots = decode_blocks(D, d.R) * kPlanSms;
   int64_t best = 0;
   for (int s = 1; s <= kMostSplits && s <= steps; s *= 2) {
     const int64_t cost = (d.tasks * s + slots - 1) / slots * ((steps + s - 1) / s + kDecodeFixed);
