@@ -399,16 +399,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kNumBqBars; ++i) {
-      int count = 1;
-      if ((i >= kBqKEmpty0 && i < kBqVFull0) || (i >= kBqVEmpty0 && i < kBqSFull0)) count = 2;
-      if ((i >= kBqSRead0 && i < kBqXFull0) || (i >= kBqDSFull0 && i < kBqAcc0)) count = 8;
-      if (i >= kBqAccEmpty0 && i < kBqDrain0) count = 4;
-      if (i >= kBqUnitEmpty0 && i < kBqTail0) count = kBwdReaders;
-      mbar_init(&bar[i], count);
-    }
-    *abort_flag = 0;
+  if (threadIdx.x < kNumBqBars) {
+    const int i = threadIdx.x;
+    int count = 1;
+    if ((i >= kBqKEmpty0 && i < kBqVFull0) || (i >= kBqVEmpty0 && i < kBqSFull0)) count = 2;
+    if ((i >= kBqSRead0 && i < kBqXFull0) || (i >= kBqDSFull0 && i < kBqAcc0)) count = 8;
+    if (i >= kBqAccEmpty0 && i < kBqDrain0) count = 4;
+    if (i >= kBqUnitEmpty0 && i < kBqTail0) count = kBwdReaders;
+    mbar_init(&bar[i], count);
+    if (i == 0) *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp0) {
@@ -774,17 +773,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_tiles = p.rows.tiles;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kNumBkBars; ++i)
-      {
-      int count = 1;
-      if (i == kBkOEmpty0 || i == kBkOEmpty0 + 1 || i == kBkAcc) count = 2;
-      if (i == kBkPFull || i == kBkDSFull) count = 16;
-      if (i == kBkAccEmpty) count = 4;
-      if (i >= kBkUnitEmpty0 && i < kBkKVFull0) count = kBwdReaders;
-      mbar_init(&bar[i], count);
-    }
-    *abort_flag = 0;
+  if (threadIdx.x < kNumBkBars) {
+    const int i = threadIdx.x;
+    int count = 1;
+    if (i == kBkOEmpty0 || i == kBkOEmpty0 + 1 || i == kBkAcc) count = 2;
+    if (i == kBkPFull || i == kBkDSFull) count = 16;
+    if (i == kBkAccEmpty) count = 4;
+    if (i >= kBkUnitEmpty0 && i < kBkKVFull0) count = kBwdReaders;
+    mbar_init(&bar[i], count);
+    if (i == 0) *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp0) {

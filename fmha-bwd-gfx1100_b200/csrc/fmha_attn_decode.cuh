@@ -22,12 +22,12 @@
 // same bias in fp16).
 //
 // Two kernels share this:
-//   * attn_decode_kernel, for small calls and behind a shared prefix: a cluster
-//     of blocks splits one kv head's keys and meets in each other's shared
-//     memory. One launch, no workspace; pieces go straight to registers, one
-//     tile ahead. With `parts`, O and LSE of other keys (the prefix) join at
-//     the end.
-//   * attn_decode_stream_kernel, for large ones: every block takes an equal run
+//   * attn_decode_kernel: a block to a tile of rows of a kv head; with few of
+//     those, a cluster of blocks splits the keys and meets in each other's
+//     shared memory. One launch, no workspace; pieces go straight to registers,
+//     one tile ahead. Behind a shared prefix it leaves its O and LSE as one
+//     part more for attn_join_kernel.
+//   * attn_decode_stream_kernel, for long caches: every block takes an equal run
 //     of the keys of the whole batch, counted on the device from the lengths,
 //     its warps side by side in neighbouring heads (and tiles): those lie
 //     together in a [token][head] cache, whose 128-byte rows otherwise come one
@@ -107,12 +107,11 @@ struct DecodeParams {
   int B, Hkv, G, M, N;
   int row_tiles;    // tiles of 8 R query rows of a kv head
   int splits;       // blocks (a cluster) that share a tile's keys
+  int d16;          // D / 16
   bool causal;      // token m reads lens - (M - 1 - m) keys
   float scale;
-  const float* part_o;  // null, or [parts][row][D] and [parts][row] to join
-  const float* part_lse;
-  int parts;
-  int64_t all_rows;
+  float* part_o;    // null, or where O and LSE go as a part: [row][D], normalised, and
+  float* part_lse;  // [row]
   int blocks;         // stream: blocks,
   int side;           // items (tiles of rows of a kv head) that a block has side by side,
   int sub;            // warps to an item (side * sub warps a block)
@@ -264,24 +263,28 @@ template <typename T>
 __device__ __forceinline__ void decode_output(const DecodeParams<T>& p, int b, int hk, int q, int c, float m, float sum,
                                               const float4& acc) {
   const int head = hk * p.G + q / p.M, tok = q % p.M;
+  const int64_t row = (static_cast<int64_t>(b) * p.Hkv * p.G + head) * p.M + tok;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<uint2*>(p.O.at(b, head, tok) + 4 * c) =
-      make_uint2(Elem<T>::pack(inv * acc.x, inv * acc.y), Elem<T>::pack(inv * acc.z, inv * acc.w));
-  if (c == 0)
-    p.LSE[(static_cast<int64_t>(b) * p.Hkv * p.G + head) * p.M + tok] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+  if (p.part_o)
+    reinterpret_cast<float4*>(p.part_o + row * (16 * p.d16))[c] = make_float4(inv * acc.x, inv * acc.y, inv * acc.z, inv * acc.w);
+  else
+    *reinterpret_cast<uint2*>(p.O.at(b, head, tok) + 4 * c) =
+        make_uint2(Elem<T>::pack(inv * acc.x, inv * acc.y), Elem<T>::pack(inv * acc.z, inv * acc.w));
+  if (c == 0) (p.part_o ? p.part_lse : p.LSE)[row] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
 }
 
 // ------------------------------------------------------------------- clusters
-constexpr int kMostSplits = 16, kDecodeWarps = 4, kMostParts = 160;
+constexpr int kMostSplits = 16, kDecodeWarps = 4;
 // Blocks that an SM holds at a time.
 __host__ __device__ constexpr int decode_blocks(int D, int R) { return D == 128 ? (R == 1 ? 3 : 2) : (R == 1 ? 5 : 4); }
 
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R)) attn_decode_kernel(const __grid_constant__ DecodeParams<T> p) {
   constexpr int kRows = 8 * R, W = kDecodeWarps, kThreads = 32 * W;
+  if (p.part_o) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ __align__(16) float sum_o[W][kRows][D];
   __shared__ float warp_m[W][kRows], warp_l[W][kRows], block_m[kRows], block_l[kRows];
-  __shared__ float weight[kMostSplits][kRows], total[kRows], top_of[kRows], part_weight[kMostParts][kRows];
+  __shared__ float weight[kMostSplits][kRows], total[kRows], top_of[kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % p.splits;
@@ -405,58 +408,23 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R)) attn_d
     }
     __syncthreads();
   }
-  if (p.splits == 1 && threadIdx.x < kRows) {
-    top_of[threadIdx.x] = block_m[threadIdx.x];
-    total[threadIdx.x] = block_l[threadIdx.x];
-    weight[0][threadIdx.x] = 1.f;
-  }
-  if (p.parts > 0) {
-    // the parts' LSE, a thread each, then their weights. A part is normalised:
-    // its sum is 1 at the reference LSE log2e.
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the launch that wrote them
-    for (int e = threadIdx.x; e < p.parts * real; e += kThreads) {
-      const int q = row0 + e % real;
-      const int64_t id = (static_cast<int64_t>(b) * p.Hkv * p.G + hk * p.G + q / p.M) * p.M + q % p.M;
-      part_weight[e / real][e % real] = __ldcg(p.part_lse + e / real * p.all_rows + id) * kLog2e;
-    }
-    __syncthreads();
-    if (threadIdx.x < real) {
-      const int row = threadIdx.x;
-      float top = top_of[row];
-      for (int y = 0; y < p.parts; ++y) top = fmaxf(top, part_weight[y][row]);
-      const float keep = ex2_approx(top_of[row] - top);
-      float sum = keep * total[row];
-      for (int y = 0; y < p.parts; ++y) {
-        const float f = ex2_approx(part_weight[y][row] - top);
-        part_weight[y][row] = f;
-        sum += f;
-      }
-      for (int y = 0; y < p.splits; ++y) weight[y][row] *= keep;
-      top_of[row] = top;
-      total[row] = sum;
-    }
-  }
-  __syncthreads();
-  // ---- the blocks' sums, and the parts: each block finishes a share
+  // ---- the blocks' sums: each block finishes a share
   for (int e = threadIdx.x * p.splits + split; e < real * (D / 4); e += p.splits * kThreads) {
     const int row = e / (D / 4), c = e % (D / 4);
     const int q = row0 + row;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.splits == 1) {
-      add_weighted(acc, weight[0][row], sum4(row, c));
+      acc = sum4(row, c);
     } else {
 #pragma unroll 4
       for (int y = 0; y < p.splits; ++y) add_weighted(acc, weight[y][row], load_cluster4(&sum_o[0][row][4 * c], y));
     }
-    if (p.parts > 0) {
-      const int64_t id = (static_cast<int64_t>(b) * p.Hkv * p.G + hk * p.G + q / p.M) * p.M + q % p.M;
-      const float4* at = reinterpret_cast<const float4*>(p.part_o + id * D) + c;
-#pragma unroll 6
-      for (int y = 0; y < p.parts; ++y) add_weighted(acc, part_weight[y][row], __ldcg(at + y * p.all_rows * (D / 4)));
-    }
-    decode_output(p, b, hk, q, c, top_of[row], total[row], acc);
+    decode_output(p, b, hk, q, c, p.splits == 1 ? block_m[row] : top_of[row], p.splits == 1 ? block_l[row] : total[row],
+                  acc);
   }
   if (p.splits > 1) cluster_sync();  // no block leaves while its sums are read
+  // behind a prefix: the launch before this one, for the join
+  if (p.part_o) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // --------------------------------------------------------------------- stream
@@ -743,16 +711,6 @@ __global__ void __launch_bounds__(32 * StreamCfg<D, R>::kWarps, 1)
     for (int x = done; x < loads; ++x) mbar_wait_drain(&bar[x % S], (x / S) & 1, p.timeout_ns);
   __syncthreads();
   if (threadIdx.x == 0) publish_failure(*abort_flag, p.status);
-  // entries without keys: O = 0, LSE = -inf
-  if (p.lens)
-    for (int b = 0; b < p.B; ++b) {
-      if (valid_rows(p.lens, b, p.N) > 0) continue;
-      const int rows = p.G * p.M;
-      for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < static_cast<int64_t>(p.Hkv) * rows * (D / 4);
-           e += static_cast<int64_t>(gridDim.x) * blockDim.x)
-        decode_output(p, b, static_cast<int>(e / (D / 4) / rows), static_cast<int>(e / (D / 4) % rows),
-                      static_cast<int>(e % (D / 4)), 0.f, 0.f, make_float4(0.f, 0.f, 0.f, 0.f));
-    }
 }
 
 // Joins the partial sums of one row (a block each; a thread takes 4 columns,
@@ -767,7 +725,11 @@ __global__ void __launch_bounds__(D) attn_decode_join_kernel(const __grid_consta
   const int item = hk * p.row_tiles + q / kRows, row = q % kRows;
   const DecodeLine<T> line(p);
   const int steps = line.steps_of(b);
-  if (steps == 0) return;
+  const int c = threadIdx.x % (D / 4), quarter = threadIdx.x / (D / 4);
+  if (steps == 0) {  // an entry without keys: O = 0, LSE = -inf
+    if (quarter == 0) decode_output(p, b, hk, q, c, 0.f, 0.f, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
   const int start = line.before_entry(b) + item / p.side * steps;
   const int c0 = line.block_of(start), c1 = line.block_of(start + steps - 1);
   const int count = c1 - c0 + 1;
@@ -777,7 +739,6 @@ __global__ void __launch_bounds__(D) attn_decode_join_kernel(const __grid_consta
     return ((2ll * (c0 + k) + (k == 0 ? skip : 0)) * p.side + item % p.side) * kRows + row;
   };
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = threadIdx.x % (D / 4), quarter = threadIdx.x / (D / 4);
   float top = kNoMax, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   // kMost sums at a time: references and sums first, a thread each, then O

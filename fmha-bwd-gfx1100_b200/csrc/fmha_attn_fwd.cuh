@@ -99,25 +99,40 @@ __device__ __forceinline__ bool get_unit(const UnitRing* ring, uint64_t* full, u
   return b.w != 0;
 }
 
+// Quotient and remainder; most divisors here are 1 in most calls.
+__device__ __forceinline__ void div_mod(int x, int d, int& q, int& r) {
+  q = x;
+  r = 0;
+  if (d != 1) {
+    q = static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(d));
+    r = x - q * d;
+  }
+}
+
 // How query rows fall into tiles (see above).
 struct RowPack {
   int M, G, S;     // tokens, query heads of a kv head, batch entries that share keys
   int Mt, Gt, St;  // the box
   int nm, ng, ns;  // boxes along each
   int tiles;       // nm * ng * ns
+  // tile t's box along each
+  __device__ __forceinline__ void box(int t, int& im, int& ig, int& is) const {
+    int u;
+    div_mod(t, nm, u, im);
+    div_mod(u, ng, is, ig);
+  }
   // token, head within the group and entry of row r of tile t; false if there is no such row
   __device__ __forceinline__ bool row(int t, int r, int& m, int& g, int& s) const {
-    const int im = t % nm, u = t / nm;
-    int rm = r, rg = 0, rs = 0;
+    int im, ig, is, rm = r, rg = 0, rs = 0;
+    box(t, im, ig, is);
     if (Mt < 128) {
-      rm = r % Mt;
-      const int v = r / Mt;
-      rg = v % Gt;
-      rs = v / Gt;
+      int v;
+      div_mod(r, Mt, v, rm);
+      div_mod(v, Gt, rs, rg);
     }
     m = im * Mt + rm;
-    g = (u % ng) * Gt + rg;
-    s = (u / ng) * St + rs;
+    g = ig * Gt + rg;
+    s = is * St + rs;
     return m < M && rg < Gt && g < G && rs < St && s < S;
   }
 };
@@ -152,6 +167,7 @@ struct FwdParams {
   float* part_o;      // splits > 1 or partial: [split][row][D], normalised
   float* part_lse;    // [split][row]
   bool partial;
+  bool in_turn;       // partial, an item to a CTA: the softmax warps store it, a tile each warpgroup
   float scale;
   KernelStatus* status;
   uint64_t timeout_ns;
@@ -212,20 +228,28 @@ __device__ __forceinline__ FwdItem fwd_item(const int4& a, const int4& b) {
 // The items of this CTA. kv heads lie innermost: with the usual [token][head]
 // layouts of Q and O, the CTAs then read and write neighbouring memory.
 template <typename T>
-__device__ void feed_fwd(const FwdParams<T>& p, UnitRing* ring, uint64_t* full, uint64_t* empty, const WaitCtx& ctx) {
+__device__ __forceinline__ void fwd_unit(const FwdParams<T>& p, int t, int4& a, int4& b) {
+  int hk, pair, split, e;
+  div_mod(t, p.Hkv, t, hk);
+  div_mod(t, p.pairs, t, pair);
+  div_mod(t, p.splits, e, split);
+  const int n = valid_rows(p.lens, e, p.N), nt = (n + kTile - 1) / kTile;
+  int lo, hi, rest;
+  // up to 2^23 tiles times 2 * 148 parts: 32 bits without a sign
+  div_mod(static_cast<int>(static_cast<uint32_t>(nt) * split), p.splits, lo, rest);
+  div_mod(static_cast<int>(static_cast<uint32_t>(nt) * (split + 1)), p.splits, hi, rest);
+  a = make_int4(e, hk, split, 2 * pair);
+  b = make_int4(lo, hi, n, 2 * pair + 1 < p.rows.tiles ? 2 : 1);
+}
+// a, b: the first of them.
+template <typename T>
+__device__ void feed_fwd(const FwdParams<T>& p, int4 a, int4 b, UnitRing* ring, uint64_t* full, uint64_t* empty,
+                         const WaitCtx& ctx) {
   int k = 0;
-  for (int t = blockIdx.x; t < p.items; t += gridDim.x, ++k) {
-    const int hk = t % p.Hkv;
-    int u = t / p.Hkv;
-    const int pair = u % p.pairs;
-    u /= p.pairs;
-    const int split = u % p.splits, b = u / p.splits;
-    const int n = valid_rows(p.lens, b, p.N), nt = (n + kTile - 1) / kTile;
-    const int lo = static_cast<int>(static_cast<int64_t>(nt) * split / p.splits);
-    const int hi = static_cast<int>(static_cast<int64_t>(nt) * (split + 1) / p.splits);
-    if (!put_unit(ring, full, empty, k, make_int4(b, hk, split, 2 * pair),
-                  make_int4(lo, hi, n, 2 * pair + 1 < p.rows.tiles ? 2 : 1), ctx, 205))
-      return;
+  for (int t = blockIdx.x; t < p.items; ++k) {
+    if (!put_unit(ring, full, empty, k, a, b, ctx, 205)) return;
+    t += gridDim.x;
+    if (t < p.items) fwd_unit(p, t, a, b);
   }
   put_unit(ring, full, empty, k, make_int4(0, 0, 0, 0), make_int4(0, 0, 0, 0), ctx, 205);
 }
@@ -321,10 +345,11 @@ __device__ __forceinline__ void store_tile(const FwdParams<T>& p, const FwdItem&
 // straight-line code that runs once an item is fetched at some 50 cycles a
 // line: what is not the inner loop is kept short and rolled.
 
-// Overwrites columns [left, 128) of the warp's rows of S with -inf.
-__device__ __forceinline__ void mask_columns(uint32_t taddr, int left) {
+// Overwrites columns [left, 128) of this thread's row of S with -inf; none of
+// the warp's rows has a left below `least`.
+__device__ __forceinline__ void mask_columns(uint32_t taddr, int left, int least) {
 #pragma unroll 1
-  for (int c = left & ~15; c < 128; c += 16) {
+  for (int c = max(least, 0) & ~15; c < 128; c += 16) {
     uint32_t v[16];
     tmem_load_16(taddr + c, v);
 #pragma unroll
@@ -350,7 +375,10 @@ __device__ __forceinline__ void weights_32(const uint32_t* s, float2 sc, float2 
   }
 }
 
-template <typename T, int D>
+// kOwn: the keys of an entry's own tokens, behind a prefix: token m reads n - (M
+// - 1 - m) of them. It starts before the launch before it has ended, and waits
+// for that at its end.
+template <typename T, int D, bool kOwn>
 __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_Q, const __grid_constant__ CUtensorMap tm_K,
                     const __grid_constant__ CUtensorMap tm_V, const __grid_constant__ FwdParams<T> p) {
@@ -371,27 +399,33 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kNumFwdBars; ++i) {
-      int count = 1;
-      if ((i >= kFwPFull0 && i < kFwOFull0) || (i >= kFwOEmpty0 && i < kFwUnitFull0)) count = 4;
-      if (i >= kFwUnitEmpty0 && i < kFwDrain) count = Cfg::kReaders;
-      mbar_init(&bar[i], count);
-    }
-    *abort_flag = 0;
+  int4 ua, ub;
+  if (threadIdx.x < kNumFwdBars) {
+    const int i = threadIdx.x;
+    int count = 1;
+    if ((i >= kFwPFull0 && i < kFwOFull0) || (i >= kFwOEmpty0 && i < kFwUnitFull0)) count = 4;
+    if (i >= kFwUnitEmpty0 && i < kFwDrain) count = Cfg::kReaders;
+    mbar_init(&bar[i], count);
+    if (i == 0) *abort_flag = 0;
     fence_mbar_init();
   }
+  if (warp == 12 && elect_one()) {
+    tma_prefetch_desc(&tm_Q);
+    tma_prefetch_desc(&tm_K);
+    tma_prefetch_desc(&tm_V);
+  }
+  __syncwarp();
   if (warp == 13) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if (warp == 14) fwd_unit(p, blockIdx.x, ua, ub);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   WaitCtx ctx{abort_flag, p.timeout_ns};
   uint64_t *unit_full = &bar[kFwUnitFull0], *unit_empty = &bar[kFwUnitEmpty0];
-  int4 ua, ub;
   int k = 0;
   bool ok = true;
   // a launch that joins the parts may start, and waits for them itself
@@ -403,22 +437,18 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
       if (elect_one()) {
         // ---- TMA producer. Ring order: K_lo, then V_j, K_(j+1) in turn, the
         // order in which the MMA issuers use them.
-        tma_prefetch_desc(&tm_Q);
-        tma_prefetch_desc(&tm_K);
-        tma_prefetch_desc(&tm_V);
         const uint64_t pol_q = l2_policy_evict_first(), pol_kv = l2_policy_evict_last();
         const uint32_t q_bytes = static_cast<uint32_t>(p.rows.Mt * p.rows.Gt * p.rows.St) * 128u * (D / kBoxCols);
         int nq0 = 0, nq1 = 0, g = 0, slot = 0, turn = 0, tails = 0;
         auto load_q = [&](const FwdItem& it, int t, int& n) {
           if (n > 0 && !mbar_wait(&bar[kFwQEmpty0 + t], (n - 1) & 1, ctx, 201)) return false;
-          const int tile = it.tile0 + t;
-          const int im = tile % p.rows.nm, u = tile / p.rows.nm;
+          int im, ig, is;
+          p.rows.box(it.tile0 + t, im, ig, is);
           mbar_arrive_expect_tx(&bar[kFwQFull0 + t], q_bytes);
 #pragma unroll
           for (int x = 0; x < D / kBoxCols; ++x)
             tma_load_4d(smem + Cfg::kOffQ + t * Cfg::kTileBytes + x * kBoxBytes, &tm_Q, &bar[kFwQFull0 + t], x * kBoxCols,
-                        im * p.rows.Mt, it.hk * p.rows.G + (u % p.rows.ng) * p.rows.Gt,
-                        it.b * p.rows.S + (u / p.rows.ng) * p.rows.St, pol_q);
+                        im * p.rows.Mt, it.hk * p.rows.G + ig * p.rows.Gt, it.b * p.rows.S + is * p.rows.St, pol_q);
           ++n;
           return true;
         };
@@ -459,7 +489,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
       }
       __syncwarp();
     } else if (warp == 14) {
-      if (lane == 0) feed_fwd(p, ring, unit_full, unit_empty, ctx);
+      if (lane == 0) feed_fwd(p, ua, ub, ring, unit_full, unit_empty, ctx);
       __syncwarp();
     } else if (warp == 13) {
       // ---- MMA. Per step, for each tile in turn: O += p V_j, then S of the
@@ -580,7 +610,13 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         if (!mbar_wait(&bar[kFwSFull0 + t], ns & 1, ctx, 231)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
-        if (it.n - j * kTile < kTile) mask_columns(tS, it.n - j * kTile);
+        if constexpr (!kOwn) {
+          if (it.n - j * kTile < kTile) mask_columns(tS, it.n - j * kTile, it.n - j * kTile);
+        } else if (const int least = it.n - (p.rows.M - 1) - j * kTile; least < kTile) {
+          int tok, g, s;
+          p.rows.row(it.tile0 + t, r, tok, g, s);
+          mask_columns(tS, least + min(tok, p.rows.M - 1), least);
+        }
         uint32_t s[128];
         tmem_load_64_start(tS, s);
         tmem_load_64_wait(s);
@@ -627,8 +663,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         }
       }
       if (!ok) continue;
-      if (p.partial) {
-        // parts: few items a CTA, so nothing to get on with meanwhile
+      if (p.in_turn) {
         if (it.lo < it.hi) {
           if (!mbar_wait(&bar[kFwOFull0 + t], no & 1, ctx, 233)) { ok = false; continue; }
           ++no;
@@ -673,7 +708,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
       }
 #pragma unroll 1
       for (int t = 0; t < 2; ++t) {
-        if ((t == 1 && !it.two) || p.partial) continue;
+        if ((t == 1 && !it.two) || p.in_turn) continue;
         if (ok && !mbar_wait(&bar[kFwStFull0 + t], (t == 0 ? nst0 : nst1) & 1, ctx, 242)) ok = false;
         if (!ok) break;
         if (t == 0) ++nst0;
@@ -705,39 +740,61 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (kOwn) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+constexpr int kJoinAhead = 4;
 // Joins the parts of split keys: with weights w_i = exp(LSE_i - max LSE),
 // O = sum w_i O_i / sum w_i and LSE = max LSE + log sum w_i, parts in order.
-// One thread per 4 columns.
+// D / 4 lanes to a row: they hold the parts' weights, and take 4 columns each.
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
     attn_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, int parts, int64_t rows,
                      View<T> O, float* __restrict__ LSE, int Hq, int M) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row = i / (D / 4);
-  const int c = static_cast<int>(i % (D / 4));
-  if (row >= rows) return;
+  constexpr int L = D / 4;
+  static_assert(L % kJoinAhead == 0, "a row's lanes hold whole batches of weights");
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
+  const int lane = threadIdx.x % L;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const bool real = at < rows;
+  const int64_t row = real ? at : rows - 1;  // whole warps shuffle
+  const float4* base = reinterpret_cast<const float4*>(part_o + row * D) + lane;
+  const int64_t stride = rows * L;
+  float4 v[kJoinAhead];  // the next parts' O, asked for before the weights are known
+  auto load = [&](int from) {
+#pragma unroll
+    for (int k = 0; k < kJoinAhead; ++k)
+      if (from + k < parts) v[k] = __ldcg(base + (from + k) * stride);
+  };
+  load(0);
   float top = -INFINITY;
-  for (int k = 0; k < parts; ++k) top = fmaxf(top, part_lse[k * rows + row]);
-  float sum = 0.f;
+  for (int k = lane; k < parts; k += L) top = fmaxf(top, __ldcg(part_lse + k * rows + row));
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (top == -INFINITY) top = 0.f;  // no part has a key: all weights are 0
+  float sum = 0.f, mine = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (top > -INFINITY) {
-    for (int k = 0; k < parts; ++k) {
-      const float w = ex2_approx((part_lse[k * rows + row] - top) * kLog2e);
-      const float4 o = reinterpret_cast<const float4*>(part_o + (k * rows + row) * D)[c];
+  for (int from = 0; from < parts; from += kJoinAhead) {
+    if (from % L == 0)
+      mine = from + lane < parts ? ex2_approx((__ldcg(part_lse + (from + lane) * rows + row) - top) * kLog2e) : 0.f;
+    if (from > 0) load(from);
+#pragma unroll
+    for (int k = 0; k < kJoinAhead; ++k) {
+      if (from + k >= parts) break;
+      const float w = __shfl_sync(0xffffffffu, mine, (from + k) % L, L);
       sum += w;
-      acc.x = fmaf(w, o.x, acc.x);
-      acc.y = fmaf(w, o.y, acc.y);
-      acc.z = fmaf(w, o.z, acc.z);
-      acc.w = fmaf(w, o.w, acc.w);
+      acc.x = fmaf(w, v[k].x, acc.x);
+      acc.y = fmaf(w, v[k].y, acc.y);
+      acc.z = fmaf(w, v[k].z, acc.z);
+      acc.w = fmaf(w, v[k].w, acc.w);
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  if (!real) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;  // NaN stays
   const int m = static_cast<int>(row % M), h = static_cast<int>(row / M % Hq), b = static_cast<int>(row / M / Hq);
-  const uint2 v = make_uint2(Elem<T>::pack(inv * acc.x, inv * acc.y), Elem<T>::pack(inv * acc.z, inv * acc.w));
-  *reinterpret_cast<uint2*>(O.at(b, h, m) + 4 * c) = v;
-  if (c == 0) LSE[row] = sum > 0.f ? top + logf(sum) : -INFINITY;
+  *reinterpret_cast<uint2*>(O.at(b, h, m) + 4 * lane) =
+      make_uint2(Elem<T>::pack(inv * acc.x, inv * acc.y), Elem<T>::pack(inv * acc.z, inv * acc.w));
+  if (lane == 0) LSE[row] = sum == 0.f ? -INFINITY : top + logf(sum);
 }
 
 }  // namespace fmha_sm100

@@ -50,6 +50,30 @@ void allow_smem(int bytes, int device) {
 // than this would split finer than its workspace allows, so plans use it too.
 constexpr int kPlanSms = 148;
 
+inline int launched(cudaError_t e) {
+  if (e == cudaSuccess) return kOk;
+  cudaGetLastError();
+  return set_error(kErrLaunch, "launch failed: %s", cudaGetErrorString(e));
+}
+
+// Launches `kernel`; with `early`, as soon as the launch before it on the
+// stream lets it (griddepcontrol), which it then waits for itself.
+template <typename... P, typename... A>
+cudaError_t launch_after(bool early, void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t stream,
+                         const A&... args) {
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &at;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // How a forward over `B` key batches divides its work.
 struct FwdPlan {
   RowPack rows;
@@ -58,18 +82,18 @@ struct FwdPlan {
   uint64_t ws_bytes;
 };
 
-// Parts of the keys: with fewer items than SMs, as many parts as still leave
-// each two key tiles, so that the loads of one item spread over idle SMs.
-inline FwdPlan plan_fwd(int M, int G, int S, int B, int Hkv, int N, int D, int sms, bool partial) {
+// Parts of the keys: with fewer items than `want`, as many parts as still leave
+// each two key tiles (one for a small call), so that the loads of one item
+// spread over idle SMs.
+inline FwdPlan plan_fwd(int M, int G, int S, int B, int Hkv, int N, int D, int want, bool partial) {
   FwdPlan f;
   f.rows = pack_rows(M, G, S);
   f.pairs = (f.rows.tiles + 1) / 2;
   const int64_t base = static_cast<int64_t>(f.pairs) * B * Hkv;
   const int nt = (N + kTile - 1) / kTile;
   f.splits = 1;
-  if (base < sms) f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / base, nt / 2)));
+  if (base < want) f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want / base, nt >= 16 ? nt / 2 : nt)));
   f.items = static_cast<int>(base * f.splits);
-  static_assert(kPlanSms <= kMostParts, "parts that attn_decode_kernel joins");
   f.all_rows = static_cast<int64_t>(B) * S * Hkv * G * M;
   f.ws_bytes = partial || f.splits > 1 ? static_cast<uint64_t>(f.splits) * f.all_rows * (D + 1) * 4 : 0;
   return f;
@@ -77,7 +101,7 @@ inline FwdPlan plan_fwd(int M, int G, int S, int B, int Hkv, int N, int D, int s
 
 template <typename T>
 int enqueue_fwd(const fmha_attn_t& a, const FwdPlan& f, const fmha_tensor_t& K, const fmha_tensor_t& V, int B, int N,
-                const int* lens, bool partial, int device, int sms, cudaStream_t stream) {
+                const int* lens, float* part_o, float* part_lse, bool own, int device, int sms, cudaStream_t stream) {
   constexpr bool kBF16 = Elem<T>::kBF16;
   if (!encode_fn()) return set_error(kErrNoDriver, "cuTensorMapEncodeTiled is unavailable");
   KernelStatus* st = attn_status(device);
@@ -98,27 +122,40 @@ int enqueue_fwd(const fmha_attn_t& a, const FwdPlan& f, const fmha_tensor_t& K, 
   p.items = f.items;
   p.O = view_of<T>(a.O);
   p.LSE = a.LSE;
-  p.partial = partial || f.splits > 1;
-  p.part_o = static_cast<float*>(a.workspace);
-  p.part_lse = p.part_o + static_cast<int64_t>(f.splits) * f.all_rows * a.K_dim;
+  p.partial = part_o != nullptr;
+  p.in_turn = p.partial && f.items <= sms;
+  p.part_o = part_o;
+  p.part_lse = part_lse;
   p.scale = a.softmax_scale;
   p.status = st;
   p.timeout_ns = effective_timeout_ns();
   const unsigned grid = static_cast<unsigned>(std::min(f.items, sms));
-  auto go = [&](auto dim) {
+  auto go = [&](auto dim, auto kind) {
     constexpr int D = decltype(dim)::value;
+    constexpr bool kOwn = decltype(kind)::value;
     using Cfg = FwdCfg<D>;
-    allow_smem<attn_fwd_kernel<T, D>>(Cfg::kSmemBytes, device);
-    attn_fwd_kernel<T, D><<<grid, Cfg::kThreads, Cfg::kSmemBytes, stream>>>(mQ, mK, mV, p);
-    if (f.splits > 1 && !partial) {
-      const int64_t threads = f.all_rows * (D / 4);
-      attn_join_kernel<T, D><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, stream>>>(
-          p.part_o, p.part_lse, f.splits, f.all_rows, p.O, p.LSE, a.q_heads, a.M);
-    }
+    allow_smem<attn_fwd_kernel<T, D, kOwn>>(Cfg::kSmemBytes, device);
+    return launch_after(kOwn, attn_fwd_kernel<T, D, kOwn>, dim3(grid), Cfg::kThreads, Cfg::kSmemBytes, stream, mQ, mK, mV,
+                        p);
   };
-  if (a.K_dim == 128) go(std::integral_constant<int, 128>{});
-  else go(std::integral_constant<int, 64>{});
-  return kOk;
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  return launched(a.K_dim == 128 ? (own ? go(D128{}, std::true_type{}) : go(D128{}, std::false_type{}))
+                                 : (own ? go(D64{}, std::true_type{}) : go(D64{}, std::false_type{})));
+}
+
+// O and LSE from `parts` parts of every row, behind the launches that write
+// them. Launched `early` behind one whose blocks all run at once: otherwise its
+// blocks would take the place of some that have work (64 entries behind 8192
+// keys: 54.1 against 51.8 us).
+template <typename T>
+int enqueue_join(const fmha_attn_t& a, const float* part_o, const float* part_lse, int parts, int64_t rows, bool early,
+                 cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((rows * (a.K_dim / 4) + 255) / 256));
+  return launched(a.K_dim == 128 ? launch_after(early, attn_join_kernel<T, 128>, grid, 256, 0, stream, part_o, part_lse,
+                                                parts, rows, view_of<T>(a.O), a.LSE, a.q_heads, a.M)
+                                 : launch_after(early, attn_join_kernel<T, 64>, grid, 256, 0, stream, part_o, part_lse,
+                                                parts, rows, view_of<T>(a.O), a.LSE, a.q_heads, a.M));
 }
 
 // How few-row attention divides its work: 8 or 16 rows a block, and either a
@@ -131,18 +168,17 @@ struct DecodePlan {
 };
 
 // Stream: evens out lengths and reads at 6.1 TB/s, but costs a second launch
-// and some 15 us in all to fill, drain and join, so from kStreamBytes of keys
-// and values on. Clusters read at 4.9 (D = 128) and 6.5 TB/s (D = 64) at 7 us:
-// at 64 columns they stay ahead (71 against 79 us for 64 x 1500 keys of 16
-// heads) until the lengths can differ much (kStreamKeys); at 128 columns 16 x
-// 4000 keys of 8 heads take 63 us in clusters and 51 us streamed. Blocks of a
-// cluster: of 1 to 16 a tile of rows, the number with the least estimated time:
-// waves of blocks times a block's steps of 64 keys plus its fixed costs, which
-// measure like kDecodeFixed such steps. `parts`: the caller's parts join in the
-// cluster's launch.
-constexpr int kDecodeFixed = 4, kStreamKeys = 8192;
+// and some 15 us in all to fill, drain and join. A block to a tile of rows
+// needs enough of them: 512 (64 entries of 8 heads of 128, up to 512 keys) take
+// 19 us, 34 streamed; 1024 of 1500 keys of 64 columns 72 and 79 us. With fewer
+// than the GPU holds at a time, clusters divide the keys (some 9 ns a block for
+// the launch): 16 x 4000 keys of 8 heads of 128 take 63 us that way, 51
+// streamed. So streamed are calls of kStreamBytes of keys and values whose
+// tiles of rows do not fill the GPU, or whose lengths can differ much
+// (kStreamKeys). `part`: the output goes to a join anyway, behind a prefix.
+constexpr int kStreamKeys = 8192;
 constexpr int64_t kStreamBytes = 96ll << 20;
-inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N, int D, bool parts) {
+inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N, int D, bool part) {
   DecodePlan d;
   const int64_t rows = static_cast<int64_t>(G) * M;
   d.R = rows <= 8 ? 1 : 2;
@@ -152,7 +188,8 @@ inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N, int D, bool p
   d.blocks = 0;
   d.ws_bytes = 0;
   const int64_t tiles = (static_cast<int64_t>(N) + 15) / 16;
-  if (!parts && d.tasks * N * D * 4 >= kStreamBytes && (D == 128 || N >= kStreamKeys) && d.tasks * tiles < (1ll << 30)) {
+  const int64_t slots = decode_blocks(D, d.R) * kPlanSms;
+  if (!part && d.tasks * N * D * 4 >= kStreamBytes && (d.tasks < slots || N >= kStreamKeys) && d.tasks * tiles < (1ll << 30)) {
     const int warps = D == 128 ? (d.R == 1 ? StreamCfg<128, 1>::kWarps : StreamCfg<128, 2>::kWarps)
                                : (d.R == 1 ? StreamCfg<64, 1>::kWarps : StreamCfg<64, 2>::kWarps);
     // as many items side by side as leave the fewest warps without one
@@ -172,20 +209,11 @@ inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N, int D, bool p
     d.ws_bytes = 2ull * d.blocks * d.side * 8 * d.R * (D * 4 + 8);
     return d;
   }
-  const int64_t steps = (static_cast<int64_t>(N) + 63) / 64;
-  const int64_t slots = decode_blocks(D, d.R) * kPlanSms;
-  int64_t best = 0;
-  for (int s = 1; s <= kMostSplits && s <= steps; s *= 2) {
-    const int64_t cost = (d.tasks * s + slots - 1) / slots * ((steps + s - 1) / s + kDecodeFixed);
-    if (s == 1 || cost < best) {
-      best = cost;
-      d.splits = s;
-    }
-  }
+  while (d.splits < kMostSplits && 2 * d.splits * d.tasks <= slots && 64ll * 2 * d.splits <= N) d.splits *= 2;
   return d;
 }
-inline DecodePlan plan_decode(const fmha_attn_t& a, bool parts) {
-  return plan_decode(a.M, a.q_heads / a.kv_heads, a.batch, a.kv_heads, a.N, a.K_dim, parts);
+inline DecodePlan plan_decode(const fmha_attn_t& a, bool part) {
+  return plan_decode(a.M, a.q_heads / a.kv_heads, a.batch, a.kv_heads, a.N, a.K_dim, part);
 }
 
 // Up to this many query rows a kv head go through attn_decode_kernel.
@@ -194,13 +222,12 @@ inline bool is_decode(const fmha_attn_t& a) {
   return static_cast<int64_t>(a.M) * (a.q_heads / a.kv_heads) <= kDecodeRows;
 }
 
-// `parts` > 0: joins that many parts of every row in the workspace, which the
-// launch before this one on the stream writes; token m then reads its entry's
-// keys up to itself.
+// With part_o and part_lse, O and LSE go there as a part, behind a prefix:
+// token m then reads its entry's keys up to itself.
 template <typename T>
-int enqueue_decode(const fmha_attn_t& a, bool prefix, int parts, int64_t all_rows, int device, cudaStream_t stream) {
+int enqueue_decode(const fmha_attn_t& a, float* part_o, float* part_lse, int device, cudaStream_t stream) {
   const int G = a.q_heads / a.kv_heads;
-  const DecodePlan d = plan_decode(a, prefix);
+  const DecodePlan d = plan_decode(a, part_o != nullptr);
   DecodeParams<T> p;
   p.Q = view_of<T>(a.Q);
   p.K = view_of<T>(a.K);
@@ -215,12 +242,11 @@ int enqueue_decode(const fmha_attn_t& a, bool prefix, int parts, int64_t all_row
   p.N = a.N;
   p.row_tiles = d.row_tiles;
   p.splits = d.splits;
-  p.causal = prefix;
+  p.causal = part_o != nullptr;
+  p.d16 = a.K_dim / 16;
   p.scale = a.softmax_scale;
-  p.parts = parts;
-  p.all_rows = all_rows;
-  p.part_o = parts > 0 ? static_cast<const float*>(a.workspace) : nullptr;
-  p.part_lse = parts > 0 ? p.part_o + parts * all_rows * a.K_dim : nullptr;
+  p.part_o = part_o;
+  p.part_lse = part_lse;
   CUtensorMap mK, mV;
   if (d.blocks > 0) {
     if (!encode_fn()) return set_error(kErrNoDriver, "cuTensorMapEncodeTiled is unavailable");
@@ -237,64 +263,60 @@ int enqueue_decode(const fmha_attn_t& a, bool prefix, int parts, int64_t all_row
   p.sub = d.sub;
   p.run_o = static_cast<float*>(a.workspace);
   p.run_ml = reinterpret_cast<float2*>(p.run_o + 2ll * d.blocks * d.side * 8 * d.R * a.K_dim);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(d.tasks * d.splits));
-  cfg.blockDim = dim3(32 * kDecodeWarps);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[2];
-  if (d.splits > 1) {
-    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    at[cfg.numAttrs].val.clusterDim.x = d.splits;
-    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
-    ++cfg.numAttrs;
-  }
-  if (parts > 0) {  // starts while the parts are still being written
-    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
-  cfg.attrs = at;
   auto go = [&](auto dim, auto r) {
     constexpr int D = decltype(dim)::value, R = decltype(r)::value;
     if (d.blocks > 0) {
       using Cfg = StreamCfg<D, R>;
       allow_smem<attn_decode_stream_kernel<T, D, R>>(Cfg::kSmemBytes, device);
-      attn_decode_stream_kernel<T, D, R><<<d.blocks, 32 * Cfg::kWarps, Cfg::kSmemBytes, stream>>>(mK, mV, p);
-      cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.q_heads * a.M));
-      cfg.blockDim = dim3(D);
-      at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      at[0].val.programmaticStreamSerializationAllowed = 1;
-      cfg.numAttrs = 1;
-      return cudaLaunchKernelEx(&cfg, attn_decode_join_kernel<T, D, R>, p);
+      const cudaError_t e = launch_after(false, attn_decode_stream_kernel<T, D, R>, dim3(d.blocks), 32 * Cfg::kWarps,
+                                         Cfg::kSmemBytes, stream, mK, mV, p);
+      if (e != cudaSuccess) return e;
+      const int64_t rows = static_cast<int64_t>(a.batch) * a.q_heads * a.M;
+      return launch_after(true, attn_decode_join_kernel<T, D, R>, dim3(static_cast<unsigned>(rows)), D, 0, stream, p);
     }
+    const dim3 grid(static_cast<unsigned>(d.tasks * d.splits));
+    if (d.splits == 1)
+      return launch_after(part_o != nullptr, attn_decode_kernel<T, D, R>, grid, 32 * kDecodeWarps, 0, stream, p);
     constexpr auto kernel = attn_decode_kernel<T, D, R>;
     static std::atomic<bool> done[64];
     if (device >= 64 || !done[device].load()) {
       cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (device < 64) done[device].store(true);
     }
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = d.splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(32 * kDecodeWarps);
+    cfg.stream = stream;
+    cfg.attrs = at;
+    cfg.numAttrs = part_o ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, p);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;
   using R1 = std::integral_constant<int, 1>;
   using R2 = std::integral_constant<int, 2>;
-  const cudaError_t e = a.K_dim == 128 ? (d.R == 1 ? go(D128{}, R1{}) : go(D128{}, R2{}))
-                                       : (d.R == 1 ? go(D64{}, R1{}) : go(D64{}, R2{}));
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return set_error(kErrLaunch, "launch failed: %s", cudaGetErrorString(e));
-  }
-  return kOk;
+  return launched(a.K_dim == 128 ? (d.R == 1 ? go(D128{}, R1{}) : go(D128{}, R2{}))
+                                 : (d.R == 1 ? go(D64{}, R1{}) : go(D64{}, R2{})));
 }
 
 inline FwdPlan cross_plan(const fmha_attn_t& a) {
   return plan_fwd(a.M, a.q_heads / a.kv_heads, 1, a.batch, a.kv_heads, a.N, a.K_dim, kPlanSms, false);
 }
-
+// Parts of the prefix: twice as many with several, which can differ in length.
 inline FwdPlan prefix_plan(const fmha_attn_t& a) {
   return plan_fwd(a.M, a.q_heads / a.kv_heads, a.batch / a.prefixes, a.prefixes, a.kv_heads, a.N_prefix, a.K_dim,
-                  kPlanSms, true);
+                  a.prefixes > 1 ? 2 * kPlanSms : kPlanSms, true);
+}
+// Behind a prefix: the entries' own keys, where they have too many rows for
+// attn_decode_kernel.
+inline FwdPlan own_plan(const fmha_attn_t& a) {
+  return plan_fwd(a.M, a.q_heads / a.kv_heads, 1, a.batch, a.kv_heads, a.N, a.K_dim, kPlanSms, true);
 }
 
 // How a backward divides its work, and its workspace: packed LSE and D, the
@@ -368,33 +390,17 @@ int enqueue_bwd(const fmha_attn_t& a, int device, cudaStream_t stream) {
     allow_smem<attn_dkv_kernel<T, D>>(DkvCfg2<D>::kSmemBytes, device);
     attn_delta_kernel<T, D><<<f.delta_blocks, 256, 0, stream>>>(view_of<T>(a.dO), view_of<T>(a.O), view_of<T>(a.V),
                                                                a.LSE, q, nlse2, ndelta, amax);
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.stream = stream;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3(f.grid_q);
-    cfg.blockDim = dim3(kBwdThreads);
-    cfg.dynamicSmemBytes = DqCfg2<D>::kSmemBytes;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, attn_dq_kernel<T, D>, mQ, mK, mV, mdO, q);
-    if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3(f.grid_k);
-    cfg.dynamicSmemBytes = DkvCfg2<D>::kSmemBytes;
-    e = cudaLaunchKernelEx(&cfg, attn_dkv_kernel<T, D>, mQ, mK, mV, mdO, k);
+    cudaError_t e = launch_after(true, attn_dq_kernel<T, D>, dim3(f.grid_q), kBwdThreads, DqCfg2<D>::kSmemBytes, stream, mQ,
+                                 mK, mV, mdO, q);
+    if (e == cudaSuccess)
+      e = launch_after(true, attn_dkv_kernel<T, D>, dim3(f.grid_k), kBwdThreads, DkvCfg2<D>::kSmemBytes, stream, mQ, mK, mV,
+                       mdO, k);
     const int marks = std::max(f.grid_q, f.grid_k) - 1;
     if (e == cudaSuccess && f.join && marks > 0)
       attn_bwd_join_kernel<T, D><<<dim3(kJoinBlocks, marks, 2), 256, 0, stream>>>(q, k, f.grid_q, f.grid_k);
     return e;
   };
-  const cudaError_t e =
-      a.K_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{});
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return set_error(kErrLaunch, "launch failed: %s", cudaGetErrorString(e));
-  }
-  return kOk;
+  return launched(a.K_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{}));
 }
 
 inline int attn_workspace(const fmha_attn_t& a, AttnOp op, uint64_t* bytes) {
@@ -402,7 +408,11 @@ inline int attn_workspace(const fmha_attn_t& a, AttnOp op, uint64_t* bytes) {
   if (rc != kOk) return rc;
   *bytes = 0;
   if (op == AttnOp::kCrossFwd) *bytes = is_decode(a) ? plan_decode(a, false).ws_bytes : cross_plan(a).ws_bytes;
-  if (op == AttnOp::kPrefix) *bytes = prefix_plan(a).ws_bytes;
+  if (op == AttnOp::kPrefix) {
+    const FwdPlan f = prefix_plan(a);
+    const int parts = f.splits + (is_decode(a) ? 1 : own_plan(a).splits);
+    *bytes = static_cast<uint64_t>(parts) * f.all_rows * (a.K_dim + 1) * 4;
+  }
   if (op == AttnOp::kCrossBwd) *bytes = plan_bwd(a).ws_bytes;
   return kOk;
 }
@@ -423,13 +433,30 @@ int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
   int device = 0, sms = 0;
   if ((rc = attn_device(device, sms)) != kOk) return rc;
   if (op == AttnOp::kCrossFwd && is_decode(a)) {
-    rc = enqueue_decode<T>(a, false, 0, 0, device, stream);
-  } else if (op == AttnOp::kPrefix) {
-    const FwdPlan f = prefix_plan(a);
-    rc = enqueue_fwd<T>(a, f, a.Kp, a.Vp, a.prefixes, a.N_prefix, a.prefix_lens, true, device, sms, stream);
-    if (rc == kOk) rc = enqueue_decode<T>(a, true, f.splits, f.all_rows, device, stream);
+    rc = enqueue_decode<T>(a, nullptr, nullptr, device, stream);
   } else if (op == AttnOp::kCrossFwd) {
-    rc = enqueue_fwd<T>(a, cross_plan(a), a.K, a.V, a.batch, a.N, a.kv_lens, false, device, sms, stream);
+    const FwdPlan f = cross_plan(a);
+    float* part_o = f.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
+    float* part_lse = f.splits > 1 ? part_o + f.splits * f.all_rows * a.K_dim : nullptr;
+    rc = enqueue_fwd<T>(a, f, a.K, a.V, a.batch, a.N, a.kv_lens, part_o, part_lse, false, device, sms, stream);
+    if (rc == kOk && f.splits > 1) rc = enqueue_join<T>(a, part_o, part_lse, f.splits, f.all_rows, true, stream);
+  } else if (op == AttnOp::kPrefix) {
+    // parts of the prefix, parts of the entries' own keys, and their join; the
+    // second launch needs nothing of the first, and the third waits for both
+    const FwdPlan f = prefix_plan(a), g = own_plan(a);
+    const int parts = f.splits + (is_decode(a) ? 1 : g.splits);
+    float* part_o = static_cast<float*>(a.workspace);
+    float* part_lse = part_o + parts * f.all_rows * a.K_dim;
+    float* own_o = part_o + f.splits * f.all_rows * a.K_dim;
+    float* own_lse = part_lse + f.splits * f.all_rows;
+    rc = enqueue_fwd<T>(a, f, a.Kp, a.Vp, a.prefixes, a.N_prefix, a.prefix_lens, part_o, part_lse, false, device, sms,
+                        stream);
+    if (rc == kOk)
+      rc = is_decode(a) ? enqueue_decode<T>(a, own_o, own_lse, device, stream)
+                        : enqueue_fwd<T>(a, g, a.K, a.V, a.batch, a.N, a.kv_lens, own_o, own_lse, true, device, sms, stream);
+    const DecodePlan d = plan_decode(a, true);
+    if (rc == kOk)
+      rc = enqueue_join<T>(a, part_o, part_lse, parts, f.all_rows, !is_decode(a) || d.tasks * d.splits <= sms, stream);
   } else {
     rc = enqueue_bwd<T>(a, device, stream);
   }

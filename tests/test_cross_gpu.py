@@ -190,6 +190,10 @@ PREFIXES = [
     (1, 2, 2, 1, 130, 150, 200, 128, "bf16", [130, 150], None, "bnhd"),
     (2, 1, 4, 4, 1, 2000, 3000, 64, "fp16", [2000, 3], [2999, 64], "bnhd"),
     (1, 2, 2, 2, 1, 30, 20, 64, "bf16", [0, 30], [0], "bhnd"),        # entry 0 has no key at all
+    (1, 2, 4, 2, 300, 700, 260, 128, "bf16", [700, 120], None, "bnhd"),       # own tokens over several tiles
+    (2, 1, 3, 1, 150, 1000, 1100, 64, "fp16", [1000, 149], [0, 1100], "bnhd"),
+    (1, 2, 1, 1, 1, 20, 20000, 64, "bf16", None, None, "bnhd"),       # 78 parts of the prefix
+    (2, 40, 32, 4, 3, 100, 513, 128, "bf16", None, [513, 200], "bnhd"),       # more items than SMs
 ]
 
 
