@@ -46,6 +46,18 @@ void allow_smem(int bytes, int device) {
   if (device < 64) done[device].store(true);
 }
 
+// Shared memory's share of an SM for `kernel`, in percent, set once. Without a
+// word on it, a kernel that follows one with 227 KB of shared memory before its
+// SMs are idle runs with what that left of L1, in which too few loads find room
+// (64 entries behind 8192 keys: 52.4 against 41.4 us).
+template <auto kernel>
+void share_smem(int percent, int device) {
+  static std::atomic<bool> done[64];
+  if (device < 64 && done[device].load()) return;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, percent);
+  if (device < 64) done[device].store(true);
+}
+
 // The SM count that workspace sizes go by: a call on a device with more SMs
 // than this would split finer than its workspace allows, so plans use it too.
 constexpr int kPlanSms = 148;
@@ -150,12 +162,14 @@ int enqueue_fwd(const fmha_attn_t& a, const FwdPlan& f, const fmha_tensor_t& K, 
 // keys: 54.1 against 51.8 us).
 template <typename T>
 int enqueue_join(const fmha_attn_t& a, const float* part_o, const float* part_lse, int parts, int64_t rows, bool early,
-                 cudaStream_t stream) {
+                 int device, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>((rows * (a.K_dim / 4) + 255) / 256));
-  return launched(a.K_dim == 128 ? launch_after(early, attn_join_kernel<T, 128>, grid, 256, 0, stream, part_o, part_lse,
-                                                parts, rows, view_of<T>(a.O), a.LSE, a.q_heads, a.M)
-                                 : launch_after(early, attn_join_kernel<T, 64>, grid, 256, 0, stream, part_o, part_lse,
-                                                parts, rows, view_of<T>(a.O), a.LSE, a.q_heads, a.M));
+  auto go = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    return launch_after(early, attn_join_kernel<T, D>, grid, 256, 0, stream, part_o, part_lse, parts, rows, view_of<T>(a.O),
+                        a.LSE, a.q_heads, a.M);
+  };
+  return launched(a.K_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{}));
 }
 
 // How few-row attention divides its work: 8 or 16 rows a block, and either a
@@ -275,6 +289,9 @@ int enqueue_decode(const fmha_attn_t& a, float* part_o, float* part_lse, int dev
       return launch_after(true, attn_decode_join_kernel<T, D, R>, dim3(static_cast<unsigned>(rows)), D, 0, stream, p);
     }
     const dim3 grid(static_cast<unsigned>(d.tasks * d.splits));
+    // the blocks' sums, and 2 KB each for what is small or reserved
+    constexpr int kShare = decode_blocks(D, R) * (kDecodeWarps * 8 * R * D * 4 + 2048) * 100 / (228 * 1024) + 1;
+    share_smem<attn_decode_kernel<T, D, R>>(kShare, device);
     if (d.splits == 1)
       return launch_after(part_o != nullptr, attn_decode_kernel<T, D, R>, grid, 32 * kDecodeWarps, 0, stream, p);
     constexpr auto kernel = attn_decode_kernel<T, D, R>;
@@ -439,7 +456,7 @@ int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
     float* part_o = f.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
     float* part_lse = f.splits > 1 ? part_o + f.splits * f.all_rows * a.K_dim : nullptr;
     rc = enqueue_fwd<T>(a, f, a.K, a.V, a.batch, a.N, a.kv_lens, part_o, part_lse, false, device, sms, stream);
-    if (rc == kOk && f.splits > 1) rc = enqueue_join<T>(a, part_o, part_lse, f.splits, f.all_rows, true, stream);
+    if (rc == kOk && f.splits > 1) rc = enqueue_join<T>(a, part_o, part_lse, f.splits, f.all_rows, true, device, stream);
   } else if (op == AttnOp::kPrefix) {
     // parts of the prefix, parts of the entries' own keys, and their join; the
     // second launch needs nothing of the first, and the third waits for both
@@ -456,7 +473,7 @@ int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
                         : enqueue_fwd<T>(a, g, a.K, a.V, a.batch, a.N, a.kv_lens, own_o, own_lse, true, device, sms, stream);
     const DecodePlan d = plan_decode(a, true);
     if (rc == kOk)
-      rc = enqueue_join<T>(a, part_o, part_lse, parts, f.all_rows, !is_decode(a) || d.tasks * d.splits <= sms, stream);
+      rc = enqueue_join<T>(a, part_o, part_lse, parts, f.all_rows, !is_decode(a) || d.tasks * d.splits <= sms, device, stream);
   } else {
     rc = enqueue_bwd<T>(a, device, stream);
   }
