@@ -553,7 +553,11 @@ __global__ void __launch_bounds__(32 * StreamCfg<D, R>::kWarps, 1)
   const int items = p.Hkv * p.row_tiles, place = warp % p.side, part = warp / p.side;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar) + warp * S;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kOffBar + 8 * Cfg::kWarps * S);
-  if (threadIdx.x == 0) *abort_flag = 0;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_K);
+    tma_prefetch_desc(&tm_V);
+    *abort_flag = 0;
+  }
   if (lane == 0) {
     for (int x = 0; x < S; ++x) mbar_init(&bar[x], 1);
     fence_mbar_init();
@@ -719,7 +723,7 @@ template <typename T, int D, int R>
 __global__ void __launch_bounds__(D) attn_decode_join_kernel(const __grid_constant__ DecodeParams<T> p) {
   constexpr int kRows = 8 * R, kMost = 256;
   __shared__ float4 part[4][D / 4];
-  __shared__ float weight[kMost], reduce[2][D / 32];
+  __shared__ float weight[kMost], mass[kMost], reduce[2][D / 32];
   const int rows = p.G * p.M, q = blockIdx.x % rows;
   const int hk = blockIdx.x / rows % p.Hkv, b = blockIdx.x / rows / p.Hkv;
   const int item = hk * p.row_tiles + q / kRows, row = q % kRows;
@@ -728,17 +732,18 @@ __global__ void __launch_bounds__(D) attn_decode_join_kernel(const __grid_consta
   const int c = threadIdx.x % (D / 4), quarter = threadIdx.x / (D / 4);
   if (steps == 0) {  // an entry without keys: O = 0, LSE = -inf
     if (quarter == 0) decode_output(p, b, hk, q, c, 0.f, 0.f, make_float4(0.f, 0.f, 0.f, 0.f));
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // never done before the launch before it
     return;
   }
   const int start = line.before_entry(b) + item / p.side * steps;
   const int c0 = line.block_of(start), c1 = line.block_of(start + steps - 1);
   const int count = c1 - c0 + 1;
-  if (count == 1) return;
   const int skip = line.mark(c0) < start ? 1 : 0;  // a block that begins in the group has it in its first slot
   auto at = [&](int k) {  // the sum of block c0 + k
     return ((2ll * (c0 + k) + (k == 0 ? skip : 0)) * p.side + item % p.side) * kRows + row;
   };
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (count == 1) return;
   float top = kNoMax, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   // kMost sums at a time: references and sums first, a thread each, then O
@@ -746,7 +751,9 @@ __global__ void __launch_bounds__(D) attn_decode_join_kernel(const __grid_consta
     const int here = min(kMost, count - from);
     float most = top;
     for (int k = threadIdx.x; k < here; k += D) {
-      weight[k] = __ldcg(p.run_ml + at(from + k)).x;
+      const float2 ml = __ldcg(p.run_ml + at(from + k));
+      weight[k] = ml.x;
+      mass[k] = ml.y;
       most = fmaxf(most, weight[k]);
     }
 #pragma unroll
@@ -762,7 +769,7 @@ __global__ void __launch_bounds__(D) attn_decode_join_kernel(const __grid_consta
     float mine = 0.f;
     for (int k = threadIdx.x; k < here; k += D) {
       weight[k] = ex2_approx(weight[k] - top);
-      mine = fmaf(weight[k], __ldcg(p.run_ml + at(from + k)).y, mine);
+      mine = fmaf(weight[k], mass[k], mine);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);

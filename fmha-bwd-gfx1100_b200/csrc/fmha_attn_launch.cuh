@@ -473,7 +473,7 @@ int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
                         : enqueue_fwd<T>(a, g, a.K, a.V, a.batch, a.N, a.kv_lens, own_o, own_lse, true, device, sms, stream);
     const DecodePlan d = plan_decode(a, true);
     if (rc == kOk)
-      rc = enqueue_join<T>(a, part_o, part_lse, parts, f.all_rows, !is_decode(a) || d.tasks * d.splits <= sms, device, stream);
+      rc = enqueue_join<T>(a, part_o, part_lse, parts, f.all_rows, is_decode(a) && d.tasks * d.splits <= sms, device, stream);
   } else {
     rc = enqueue_bwd<T>(a, device, stream);
   }
