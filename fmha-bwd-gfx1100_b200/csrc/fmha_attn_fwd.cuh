@@ -36,34 +36,6 @@ namespace fmha_sm100 {
 
 constexpr float kLn2 = 0.6931471805599453f;
 
-// 2^x of two values on the FMA pipe instead of the SFU, whose 16 results a
-// clock would bound these kernels: x = n + f with n the nearest integer (taken
-// from the low mantissa bits of x + 1.5 2^23) and 2^f on [-1/2, 1/2] by the
-// polynomial of degree 5 with the least largest relative error there (found by
-// Remez exchange): 7.5e-8, 2.4e-7 as evaluated in fp32, like ex2.approx. Below
-// 2^-126 the result stays there. With kNaN, NaN stays NaN; else it may come
-// out as anything.
-template <bool kNaN>
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  if (kNaN) {
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
-  } else {
-    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  }
-  auto both = [](float c) { return make_float2(c, c); };
-  const float2 t = add_f32x2(x, both(12582912.f));
-  const float2 f = fma_f32x2(add_f32x2(t, both(-12582912.f)), both(-1.f), x);
-  float2 p = fma_f32x2(both(1.3276472e-3f), f, both(9.675541e-3f));
-  p = fma_f32x2(p, f, both(5.550713e-2f));
-  p = fma_f32x2(p, f, both(0.24022120f));
-  p = fma_f32x2(p, f, both(0.69314694f));
-  p = fma_f32x2(p, f, both(1.0000001f));
-  const uint32_t nx = __float_as_uint(t.x) << 23, ny = __float_as_uint(t.y) << 23;
-  if (kNaN) return mul_f32x2(p, make_float2(__uint_as_float(nx + 0x3f800000u), __uint_as_float(ny + 0x3f800000u)));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + nx), __uint_as_float(__float_as_uint(p.y) + ny));
-}
-
 // Units of work that one warp of a CTA works out and the others take from a
 // ring in shared memory: the divisions are done once, and the other roles hold
 // a unit's few numbers only. A unit is two int4; its last number is 0 behind

@@ -390,7 +390,7 @@ def cross_attn_fwd(Q, K, V, kv_lens=None, scale=None, *, out=None, stream=None, 
         _check_lse(out[1], dev, shape)
     return _run_attn(
         _CROSS_FWD, Q, dev, (Q, ..., K, V, None, None, None, None, None, None),
-        lambda: (torch.empty_like(Q), torch.empty(shape[:3], dtype=torch.float32, device=Q.device)), out, ..., kv_lens,
+        lambda: (torch.empty_like(Q), Q.new_empty((B, Hq, M), dtype=torch.float32)), out, ..., kv_lens,
         None, (B, Hq, kshape[1], M, kshape[2], d, 0, 0), d ** -0.5 if scale is None else float(scale), stream, sync)
 
 
@@ -445,7 +445,7 @@ def prefix_attn(Q, Kp, Vp, K, V, prefix_lens=None, kv_lens=None, scale=None, *, 
         _check_lse(out[1], dev, shape)
     return _run_attn(
         _PREFIX, Q, dev, (Q, ..., K, V, None, None, None, None, Kp, Vp),
-        lambda: (torch.empty_like(Q), torch.empty(shape[:3], dtype=torch.float32, device=Q.device)), out, ..., kv_lens,
+        lambda: (torch.empty_like(Q), Q.new_empty((B, Hq, M), dtype=torch.float32)), out, ..., kv_lens,
         prefix_lens, (B, Hq, Hkv, M, kshape[2], d, P, pshape[2]), d ** -0.5 if scale is None else float(scale), stream,
         sync)
 
