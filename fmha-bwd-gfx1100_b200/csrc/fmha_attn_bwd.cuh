@@ -890,10 +890,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (lane == 0) {
         feed_units<T, false>(p, ring, unit_full, unit_empty, ctx, 405);
       } else if (p.lens) {
-        // the other lanes: key tiles without a valid key have dK = dV = 0
+        // the other lanes: dK = dV = 0 behind the last key. (The sums of a
+        // tile would do if Q and dO held neither infinities nor NaN.)
         const int64_t thread = static_cast<int64_t>(blockIdx.x) * 31 + lane - 1, threads = 31ll * gridDim.x;
         for (int b = 0; b < p.B; ++b) {
-          const int from = (valid_rows(p.lens, b, p.N) + kTile - 1) / kTile * kTile;
+          const int from = valid_rows(p.lens, b, p.N);
           if (from < p.N) {
             zero_rows<T, D>(p.dK, b, p.Hkv, from, p.N, thread, threads);
             zero_rows<T, D>(p.dV, b, p.Hkv, from, p.N, thread, threads);
@@ -1060,8 +1061,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int which = 0; which < 2; ++which) {
         const View<T>& v = which == 0 ? p.dV : p.dK;
         float* part = p.part + ((static_cast<int64_t>(u.slot) * 2 + which) * kTile + r) * D;
-        uint8_t* out = u.slot >= 0   ? reinterpret_cast<uint8_t*>(part)
-                       : key < p.N ? reinterpret_cast<uint8_t*>(v.at(u.b, u.hk, key))
+        uint8_t* out = u.slot >= 0 ? reinterpret_cast<uint8_t*>(part)
+                       : key < u.n ? reinterpret_cast<uint8_t*>(v.at(u.b, u.hk, key))
                                    : nullptr;
         store_sums<T, D, 32>(tmem + (which == 0 ? Cfg::kColdV : Cfg::kColdK) + lanes, u.slot >= 0, out,
                          u.slot >= 0 ? 1.f : (which == 0 ? dv_mul : dk_mul));
@@ -1150,7 +1151,7 @@ __global__ void __launch_bounds__(256)
     } else {
       const int key = it.u.idx * kTile + row;
       if (which == 0) mul = Elem<T>::kBF16 ? 1.f : pow2(-10);
-      if (key < p.N) out = (which == 0 ? p.dV : p.dK).at(it.u.b, it.u.hk, key);
+      if (key < it.u.n) out = (which == 0 ? p.dV : p.dK).at(it.u.b, it.u.hk, key);
     }
     if (out)
       *reinterpret_cast<uint2*>(out + 4 * col) =

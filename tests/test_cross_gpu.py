@@ -178,6 +178,24 @@ def test_backward_against_differences(F, name, d):
             assert abs((got[i].double() * U).sum() - slope) <= tol, label
 
 
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("M", [1, 130])
+def test_nan_is_not_lost(F, name, M):
+    """A NaN in one query row: that row of O, LSE and dQ, and what sums over it."""
+    Q, K, V, n = make(1, 2, 1, M, 150, 64, name, [140], seed=15)
+    dO = tensor(torch.Generator(device="cuda").manual_seed(16), 1, 2, M, 64, Q.dtype)
+    Q[0, 0, M // 2, 3] = math.nan
+    O, LSE = F.cross_attn_fwd(Q, K, V, n)
+    dQ, dK, dV = F.cross_attn_bwd(Q, K, V, O, LSE, dO, n)
+    hit = torch.zeros(1, 2, M, dtype=torch.bool, device="cuda")
+    hit[0, 0, M // 2] = True
+    assert torch.equal(LSE.isnan(), hit)
+    for x in (O, dQ):
+        assert torch.equal(x.isfinite().all(-1), ~hit) and torch.equal(x.isfinite().any(-1), ~hit)
+    for x in (dK, dV):
+        assert not x[:, :, :140].isfinite().any() and (x[:, :, 140:] == 0).all()
+
+
 PREFIXES = [
     # (P, S, Hq, Hkv, M, N, Np, d, dtype, lens, prefix_lens, layout)
     (1, 1, 1, 1, 1, 1, 1, 64, "bf16", None, None, "bhnd"),
