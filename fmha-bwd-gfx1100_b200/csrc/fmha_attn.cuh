@@ -114,10 +114,13 @@ inline int check_attn(fmha_attn_t& a, AttnOp op) {
   }
   const void* read[] = {a.Q.ptr, a.K.ptr, a.V.ptr, bwd ? a.O.ptr : nullptr, bwd ? a.dO.ptr : nullptr,
                         op == AttnOp::kPrefix ? a.Kp.ptr : nullptr, op == AttnOp::kPrefix ? a.Vp.ptr : nullptr};
-  const void* written[] = {bwd ? a.dQ.ptr : a.O.ptr, bwd ? a.dK.ptr : nullptr, bwd ? a.dV.ptr : nullptr};
-  for (const void* r : read)
-    for (const void* w : written)
+  const void* written[] = {bwd ? a.dQ.ptr : a.O.ptr, bwd ? a.dK.ptr : a.LSE, bwd ? a.dV.ptr : nullptr};
+  for (const void* const& w : written) {
+    for (const void* r : read)
       if (r && r == w) return set_error(kErrInvalidArgument, "an output lies over an input");
+    for (const void* const& v : written)
+      if (&v != &w && v && v == w) return set_error(kErrInvalidArgument, "an output lies over another");
+  }
   if (!a.LSE) return set_error(kErrInvalidArgument, "null LSE argument");
   if ((reinterpret_cast<uintptr_t>(a.LSE) & 3u) != 0) return set_error(kErrMisaligned, "LSE must be 4-byte aligned");
   if ((reinterpret_cast<uintptr_t>(a.kv_lens) & 3u) != 0)

@@ -65,9 +65,11 @@ BAD = [
     (1, "scale", dict(softmax_scale=float("nan"))), (1, "scale", dict(softmax_scale=float("inf"))),
 ]
 BAD_OF = {
-    0: [(1, "overlap", dict(O__head=64)), (1, "input", dict(O__ptr=0x10000000))],
+    0: [(1, "overlap", dict(O__head=64)), (1, "input", dict(O__ptr=0x10000000)),
+        (1, "input", dict(LSE=0x10000000)), (1, "another", dict(LSE=0x20000000))],
     1: [(1, "dO", dict(dO__ptr=None)), (1, "overlap", dict(dK__batch=64)), (2, "dV", dict(dV__ptr=0x1004)),
-        (1, "input", dict(dQ__ptr=0x10000000))],
+        (1, "input", dict(dQ__ptr=0x10000000)), (1, "another", dict(dK__ptr=0x80000000)),
+        (1, "another", dict(dQ__ptr=0x70000000))],
     2: [(1, "Kp", dict(Kp__ptr=None)), (1, "prefixes", dict(prefixes=0)), (1, "multiple", dict(prefixes=3)),
         (1, "N_prefix", dict(N_prefix=0)), (2, "prefix_lens", dict(prefix_lens=0x1002)),
         (2, "Vp", dict(Vp__row=66))],
