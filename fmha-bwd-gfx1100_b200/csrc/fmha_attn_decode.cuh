@@ -25,8 +25,9 @@
 //   * attn_decode_kernel: a block to a tile of rows of a kv head; with few of
 //     those, a cluster of blocks splits the keys and meets in each other's
 //     shared memory. One launch, no workspace; pieces go straight to registers,
-//     one tile ahead. Behind a shared prefix it leaves its O and LSE as one
-//     part more for attn_join_kernel.
+//     one tile ahead. Behind a shared prefix it takes the prefix's keys along
+//     (few of them), or leaves its O and LSE as one part more for
+//     attn_join_kernel.
 //   * attn_decode_stream_kernel, for long caches: every block takes an equal run
 //     of the keys of the whole batch, counted on the device from the lengths,
 //     its warps side by side in neighbouring heads (and tiles): those lie
@@ -112,6 +113,9 @@ struct DecodeParams {
   float scale;
   float* part_o;    // null, or where O and LSE go as a part: [row][D], normalised, and
   float* part_lse;  // [row]
+  View<T> Kp, Vp;         // kBehind: the keys that `share` entries have before their own,
+  const int* prefix_lens; // [B / share] or null
+  int share, Np;
   int blocks;         // stream: blocks,
   int side;           // items (tiles of rows of a kv head) that a block has side by side,
   int sub;            // warps to an item (side * sub warps a block)
@@ -278,8 +282,10 @@ constexpr int kMostSplits = 16, kDecodeWarps = 4;
 // Blocks that an SM holds at a time.
 __host__ __device__ constexpr int decode_blocks(int D, int R) { return D == 128 ? (R == 1 ? 3 : 2) : (R == 1 ? 5 : 4); }
 
-template <typename T, int D, int R>
-__global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R)) attn_decode_kernel(const __grid_constant__ DecodeParams<T> p) {
+// kBehind: over a shared prefix's keys and an entry's own in one go.
+template <typename T, int D, int R, bool kBehind>
+__global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBehind && D == 64))
+    attn_decode_kernel(const __grid_constant__ DecodeParams<T> p) {
   constexpr int kRows = 8 * R, W = kDecodeWarps, kThreads = 32 * W;
   if (p.part_o) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ __align__(16) float sum_o[W][kRows][D];
@@ -294,27 +300,33 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R)) attn_d
   const int hk = u % p.Hkv, b = u / p.Hkv;
   const int rows = p.G * p.M, row0 = tile * kRows;
   const int n = valid_rows(p.lens, b, p.N);
-  const int tiles = (n + 15) / 16;
+  const int bp = kBehind ? b / p.share : 0, np = kBehind ? valid_rows(p.prefix_lens, bp, p.Np) : 0;
+  const int ahead = (np + 15) / 16;  // tiles of the prefix
+  const int tiles = ahead + (n + 15) / 16;
   const int lo = static_cast<int>(static_cast<int64_t>(tiles) * split / p.splits);
   const int hi = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / p.splits);
 
   uint4 kf[2][D / 32], vf[4][D / 64];
   auto load_k = [&](int i) {
+    const bool own = !kBehind || i >= ahead;
+    const int from = 16 * (own ? i - ahead : i), most = own ? n : np;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int key = 16 * i + g + 8 * x;
-      const T* at = p.K.at(b, hk, key) + 8 * t;
+      const int key = from + g + 8 * x;
+      const T* at = (own ? p.K.at(b, hk, key) : p.Kp.at(bp, hk, key)) + 8 * t;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) kf[x][c] = key < n ? load_stream(at + 32 * c) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < D / 32; ++c) kf[x][c] = key < most ? load_stream(at + 32 * c) : make_uint4(0, 0, 0, 0);
     }
   };
   auto load_v = [&](int i) {
+    const bool own = !kBehind || i >= ahead;
+    const int from = 16 * (own ? i - ahead : i), most = own ? n : np;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int key = 16 * i + 2 * t + (x & 1) + 8 * (x >> 1);
-      const T* at = p.V.at(b, hk, key) + 8 * g;
+      const int key = from + 2 * t + (x & 1) + 8 * (x >> 1);
+      const T* at = (own ? p.V.at(b, hk, key) : p.Vp.at(bp, hk, key)) + 8 * g;
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) vf[x][c] = key < n ? load_stream(at + 64 * c) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < D / 64; ++c) vf[x][c] = key < most ? load_stream(at + 64 * c) : make_uint4(0, 0, 0, 0);
     }
   };
   int i = lo + warp;
@@ -337,7 +349,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R)) attn_d
     w.scores(s, [&](int x, int c) { return kf[x][c]; });
     const bool more = i + W < hi;
     if (more) load_k(i + W);
-    w.weights(s, pt, 16 * i, limit, sl2);
+    if (!kBehind || i >= ahead) {
+      w.weights(s, pt, 16 * (i - ahead), limit, sl2);
+    } else {
+      int all[R][2];
+#pragma unroll
+      for (int r = 0; r < R; ++r) all[r][0] = all[r][1] = np;
+      w.weights(s, pt, 16 * i, all, sl2);
+    }
     w.values(pt, [&](int x, int c) { return vf[x][c]; });
     if (more) load_v(i + W);
   }

@@ -236,12 +236,30 @@ inline bool is_decode(const fmha_attn_t& a) {
   return static_cast<int64_t>(a.M) * (a.q_heads / a.kv_heads) <= kDecodeRows;
 }
 
-// With part_o and part_lse, O and LSE go there as a part, behind a prefix:
-// token m then reads its entry's keys up to itself.
+// Behind a prefix: whether one launch of attn_decode_kernel reads the prefix for
+// each entry anew, instead of parts and their join. It does for kTogetherBytes
+// of keys and values in all, read so (4 entries of 16 heads behind 1000 keys: 8.2
+// and 11.2 us; 8 of 8 heads behind 4 prefixes of 1000, 34 MB: 11 and 17; but 8
+// behind 2000, 66 MB: 15 and 13), unless they are few long caches, for which a
+// cluster is too little (kTogetherKeys: 23 us either way for one of 20000); and
+// for prefixes of one entry each, if there are many (64 caches of 8192 + 512
+// keys: 56 and 79 us).
+constexpr int64_t kTogetherBytes = 48ll << 20, kTogetherKeys = 20480, kTogetherTasks = 32;
+inline bool prefix_together(const fmha_attn_t& a) {
+  if (!is_decode(a)) return false;
+  const int64_t tasks = static_cast<int64_t>(a.batch) * a.kv_heads, keys = static_cast<int64_t>(a.N_prefix) + a.N;
+  if (a.prefixes == a.batch && tasks >= kTogetherTasks) return keys < (1 << 30);
+  return keys <= kTogetherKeys && tasks * keys * a.K_dim * 4 <= kTogetherBytes;
+}
+
+// kPrefix: token m reads its entry's keys up to itself, and with part_o and
+// part_lse O and LSE go there as a part, else the prefix's keys come along.
 template <typename T>
-int enqueue_decode(const fmha_attn_t& a, float* part_o, float* part_lse, int device, cudaStream_t stream) {
+int enqueue_decode(const fmha_attn_t& a, AttnOp op, float* part_o, float* part_lse, int device, cudaStream_t stream) {
   const int G = a.q_heads / a.kv_heads;
-  const DecodePlan d = plan_decode(a, part_o != nullptr);
+  const bool behind = op == AttnOp::kPrefix && !part_o;
+  const DecodePlan d = behind ? plan_decode(a.M, G, a.batch, a.kv_heads, a.N_prefix + a.N, a.K_dim, true)
+                              : plan_decode(a, op == AttnOp::kPrefix);
   DecodeParams<T> p;
   p.Q = view_of<T>(a.Q);
   p.K = view_of<T>(a.K);
@@ -256,11 +274,16 @@ int enqueue_decode(const fmha_attn_t& a, float* part_o, float* part_lse, int dev
   p.N = a.N;
   p.row_tiles = d.row_tiles;
   p.splits = d.splits;
-  p.causal = part_o != nullptr;
+  p.causal = op == AttnOp::kPrefix;
   p.d16 = a.K_dim / 16;
   p.scale = a.softmax_scale;
   p.part_o = part_o;
   p.part_lse = part_lse;
+  p.Kp = view_of<T>(a.Kp);
+  p.Vp = view_of<T>(a.Vp);
+  p.prefix_lens = a.prefix_lens;
+  p.share = behind ? a.batch / a.prefixes : 1;
+  p.Np = a.N_prefix;
   CUtensorMap mK, mV;
   if (d.blocks > 0) {
     if (!encode_fn()) return set_error(kErrNoDriver, "cuTensorMapEncodeTiled is unavailable");
@@ -277,7 +300,7 @@ int enqueue_decode(const fmha_attn_t& a, float* part_o, float* part_lse, int dev
   p.sub = d.sub;
   p.run_o = static_cast<float*>(a.workspace);
   p.run_ml = reinterpret_cast<float2*>(p.run_o + 2ll * d.blocks * d.side * 8 * d.R * a.K_dim);
-  auto go = [&](auto dim, auto r) {
+  auto go = [&](auto dim, auto r, auto kind) {
     constexpr int D = decltype(dim)::value, R = decltype(r)::value;
     if (d.blocks > 0) {
       using Cfg = StreamCfg<D, R>;
@@ -291,10 +314,10 @@ int enqueue_decode(const fmha_attn_t& a, float* part_o, float* part_lse, int dev
     const dim3 grid(static_cast<unsigned>(d.tasks * d.splits));
     // the blocks' sums, and 2 KB each for what is small or reserved
     constexpr int kShare = decode_blocks(D, R) * (kDecodeWarps * 8 * R * D * 4 + 2048) * 100 / (228 * 1024) + 1;
-    share_smem<attn_decode_kernel<T, D, R>>(kShare, device);
-    if (d.splits == 1)
-      return launch_after(part_o != nullptr, attn_decode_kernel<T, D, R>, grid, 32 * kDecodeWarps, 0, stream, p);
-    constexpr auto kernel = attn_decode_kernel<T, D, R>;
+    constexpr bool kBehind = decltype(kind)::value;
+    constexpr auto kernel = attn_decode_kernel<T, D, R, kBehind>;
+    share_smem<kernel>(kShare, device);
+    if (d.splits == 1) return launch_after(part_o != nullptr, kernel, grid, 32 * kDecodeWarps, 0, stream, p);
     static std::atomic<bool> done[64];
     if (device >= 64 || !done[device].load()) {
       cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -318,8 +341,11 @@ int enqueue_decode(const fmha_attn_t& a, float* part_o, float* part_lse, int dev
   using D128 = std::integral_constant<int, 128>;
   using R1 = std::integral_constant<int, 1>;
   using R2 = std::integral_constant<int, 2>;
-  return launched(a.K_dim == 128 ? (d.R == 1 ? go(D128{}, R1{}) : go(D128{}, R2{}))
-                                 : (d.R == 1 ? go(D64{}, R1{}) : go(D64{}, R2{})));
+  auto with = [&](auto kind) {
+    return a.K_dim == 128 ? (d.R == 1 ? go(D128{}, R1{}, kind) : go(D128{}, R2{}, kind))
+                          : (d.R == 1 ? go(D64{}, R1{}, kind) : go(D64{}, R2{}, kind));
+  };
+  return launched(behind ? with(std::true_type{}) : with(std::false_type{}));
 }
 
 inline FwdPlan cross_plan(const fmha_attn_t& a) {
@@ -425,7 +451,7 @@ inline int attn_workspace(const fmha_attn_t& a, AttnOp op, uint64_t* bytes) {
   if (rc != kOk) return rc;
   *bytes = 0;
   if (op == AttnOp::kCrossFwd) *bytes = is_decode(a) ? plan_decode(a, false).ws_bytes : cross_plan(a).ws_bytes;
-  if (op == AttnOp::kPrefix) {
+  if (op == AttnOp::kPrefix && !prefix_together(a)) {
     const FwdPlan f = prefix_plan(a);
     const int parts = f.splits + (is_decode(a) ? 1 : own_plan(a).splits);
     *bytes = static_cast<uint64_t>(parts) * f.all_rows * (a.K_dim + 1) * 4;
@@ -449,8 +475,8 @@ int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
   if (need > 0 && !aligned16(a.workspace)) return set_error(kErrMisaligned, "workspace must be 16-byte aligned");
   int device = 0, sms = 0;
   if ((rc = attn_device(device, sms)) != kOk) return rc;
-  if (op == AttnOp::kCrossFwd && is_decode(a)) {
-    rc = enqueue_decode<T>(a, nullptr, nullptr, device, stream);
+  if (op == AttnOp::kCrossFwd ? is_decode(a) : op == AttnOp::kPrefix && prefix_together(a)) {
+    rc = enqueue_decode<T>(a, op, nullptr, nullptr, device, stream);
   } else if (op == AttnOp::kCrossFwd) {
     const FwdPlan f = cross_plan(a);
     float* part_o = f.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
@@ -469,7 +495,7 @@ int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
     rc = enqueue_fwd<T>(a, f, a.Kp, a.Vp, a.prefixes, a.N_prefix, a.prefix_lens, part_o, part_lse, false, device, sms,
                         stream);
     if (rc == kOk)
-      rc = is_decode(a) ? enqueue_decode<T>(a, own_o, own_lse, device, stream)
+      rc = is_decode(a) ? enqueue_decode<T>(a, op, own_o, own_lse, device, stream)
                         : enqueue_fwd<T>(a, g, a.K, a.V, a.batch, a.N, a.kv_lens, own_o, own_lse, true, device, sms, stream);
     const DecodePlan d = plan_decode(a, true);
     if (rc == kOk)

@@ -210,7 +210,12 @@ PREFIXES = [
     (1, 2, 2, 2, 1, 30, 20, 64, "bf16", [0, 30], [0], "bhnd"),        # entry 0 has no key at all
     (1, 2, 4, 2, 300, 700, 260, 128, "bf16", [700, 120], None, "bnhd"),       # own tokens over several tiles
     (2, 1, 3, 1, 150, 1000, 1100, 64, "fp16", [1000, 149], [0, 1100], "bnhd"),
-    (1, 2, 1, 1, 1, 20, 20000, 64, "bf16", None, None, "bnhd"),       # 78 parts of the prefix
+    (1, 2, 1, 1, 1, 20, 20000, 64, "bf16", None, None, "bnhd"),
+    (1, 2, 1, 1, 1, 20, 30000, 64, "bf16", None, None, "bnhd"),       # 117 parts of the prefix
+    (1, 3, 4, 2, 2, 40, 20500, 128, "fp16", [40, 0, 1], None, "bnhd"),        # parts, and own keys or none
+    (2, 40, 8, 4, 1, 100, 513, 128, "bf16", None, [513, 100], "bnhd"),
+    (8, 1, 16, 4, 2, 300, 500, 64, "fp16", [300, 1, 2, 0, 17, 16, 299, 100], None, "bnhd"),   # nothing shared
+    (3, 2, 4, 4, 1, 17, 33, 128, "fp16", [0, 17, 16, 1, 0, 3], [33, 0, 16], "apart"),
     (2, 40, 32, 4, 3, 100, 513, 128, "bf16", None, [513, 200], "bnhd"),       # more items than SMs
 ]
 
