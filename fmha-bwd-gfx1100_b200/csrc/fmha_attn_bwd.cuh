@@ -60,13 +60,17 @@ struct BwdUnit {
 };
 
 // Steps that a division by steps has to save, as its partial sums cost about
-// as much, and the least number of steps of a CTA under it.
-constexpr int kBwdSpare = 8, kBwdLeast = 4;
+// as much, and the least number of steps of a CTA under it: of a query-major
+// step, which takes twice as long, half as many (with 4 of either 768 key-major
+// steps take 50 us, with 8 36; with 8 of either 16 items of 12 query-major ones
+// 55 instead of 42).
+constexpr int kBwdSpare = 8, kBwdLeastQ = 4, kBwdLeastK = 8;
 __host__ __device__ inline bool bwd_by_steps(int64_t whole, int64_t total, int64_t grid) {
   return whole > (total + grid - 1) / grid + kBwdSpare;
 }
-__host__ __device__ inline int bwd_parts(int64_t total, int grid) {
-  const int64_t most = (total + kBwdLeast - 1) / kBwdLeast;
+__host__ __device__ inline int bwd_parts(int64_t total, int grid, bool q_major) {
+  const int least = q_major ? kBwdLeastQ : kBwdLeastK;
+  const int64_t most = (total + least - 1) / least;
   return most < grid ? (most > 0 ? static_cast<int>(most) : 1) : grid;
 }
 
@@ -109,7 +113,7 @@ struct BwdSchedule {
       }
     }
     by_steps = bwd_by_steps(min((items + grid - 1) / grid * most, apart), total, grid);
-    parts = bwd_parts(total, grid);
+    parts = bwd_parts(total, grid, kQMajor);
     pos = by_steps ? mark(c) : c;
     end = by_steps ? mark(c + 1) : items;
     b = before = 0;
