@@ -494,14 +494,23 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         int j = cur.lo - 1;  // the step before the first has no p V
         while (more && ok) {
           const bool start = j < cur.lo, last = j + 1 == cur.hi;
-          if (last) more = next_item(nxt);
+          // Whether S of a next step goes ahead. Behind the last step that is
+          // of the next item, if this is not one without keys: to look for
+          // further ones first would wait for units that are only put once
+          // this item's O is done.
+          bool ahead = true;
+          if (last) {
+            more = get_unit<false>(ring, unit_full, unit_empty, k, ua, ub, ctx, 210, ok);
+            nxt = fwd_item(ua, ub);
+            ahead = more && nxt.lo < nxt.hi;
+          }
           if (!ok) break;
           const int jn = last ? nxt.lo : j + 1, vslot = slot;
           if (!start) {
             if (!(ok = mbar_wait(&bar[kFwKVFull0 + slot], turn, ctx, 212))) break;
             advance();
           }
-          if (more && !(ok = mbar_wait(&bar[kFwKVFull0 + slot], turn, ctx, 216))) break;
+          if (ahead && !(ok = mbar_wait(&bar[kFwKVFull0 + slot], turn, ctx, 216))) break;
 #pragma unroll 1
           for (int t = 0; t < 2; ++t) {
             const uint32_t tS = tmem + Cfg::kColS + 128 * t, tO = tmem + Cfg::kColO + D * t;
@@ -534,7 +543,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
               if (last) umma_commit(&bar[kFwOFull0 + t]);
             }
             if (t == 1 && !start) umma_commit(&bar[kFwKVEmpty0 + vslot]);
-            if (more && (t == 0 || nxt.two)) {
+            if (ahead && (t == 0 || nxt.two)) {
               if (jn == nxt.lo) {
                 if (!(ok = mbar_wait(&bar[kFwQFull0 + t], turns >> t & 1, ctx, 211))) break;
                 turns ^= 1u << t;
@@ -550,12 +559,13 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
               umma_commit(&bar[kFwSFull0 + t]);
               if (jn + 1 == nxt.hi) umma_commit(&bar[kFwQEmpty0 + t]);
             }
-            if (t == 1 && more) umma_commit(&bar[kFwKVEmpty0 + slot]);
+            if (t == 1 && ahead) umma_commit(&bar[kFwKVEmpty0 + slot]);
           }
           if (!ok) break;
-          if (more) advance();
+          if (ahead) advance();
+          else if (more) more = next_item(nxt);
           cur = nxt;
-          j = jn;
+          j = ahead ? jn : nxt.lo - 1;
         }
         if (!ok) {
           umma_commit(&bar[kFwDrain]);

@@ -196,6 +196,26 @@ def test_nan_is_not_lost(F, name, M):
         assert not x[:, :, :140].isfinite().any() and (x[:, :, 140:] == 0).all()
 
 
+@pytest.mark.parametrize("d,name", [(64, "fp16"), (128, "bf16")])
+def test_runs_of_entries_without_keys(F, d, name):
+    """More in a row than a CTA holds units of work ahead, between others."""
+    B, H, M, N = 120, 8, 20, 140
+    Q, K, V, n = make(B, H, H, M, N, d, name, [140] * 19 + [0] * 82 + [77] * 19, seed=17)
+    O, LSE = F.cross_attn_fwd(Q, K, V, n)
+    ref, lse, bound, lse_bound = R.forward(Q, K, V, n, d ** -0.5)
+    R.check("O", O, ref, bound)
+    R.check("LSE", LSE, lse, lse_bound)
+    dO = tensor(torch.Generator(device="cuda").manual_seed(18), B, H, M, d, Q.dtype)
+    grads = F.cross_attn_bwd(Q, K, V, O, LSE, dO, n)
+    for label, x, ref, bound in zip(("dQ", "dK", "dV"), grads, *R.backward(Q, K, V, O, LSE, dO, n, d ** -0.5)):
+        R.check(label, x, ref, bound)
+    _, Kp, Vp, np_ = make(B, H, H, 1, 130, d, name, [0] * 30 + [130] + [0] * 85 + [9] * 4, seed=19)
+    O, LSE = F.prefix_attn(Q, Kp, Vp, K, V, np_, n)
+    ref, lse, bound, lse_bound = R.prefix(Q, Kp, Vp, K, V, np_, n, d ** -0.5)
+    R.check("O", O, ref, bound)
+    R.check("LSE", LSE, lse, lse_bound)
+
+
 PREFIXES = [
     # (P, S, Hq, Hkv, M, N, Np, d, dtype, lens, prefix_lens, layout)
     (1, 1, 1, 1, 1, 1, 1, 64, "bf16", None, None, "bhnd"),
