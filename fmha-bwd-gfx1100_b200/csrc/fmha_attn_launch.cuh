@@ -94,9 +94,13 @@ struct FwdPlan {
   uint64_t ws_bytes;
 };
 
-// Parts of the keys: with fewer items than `want`, as many parts as still leave
-// each two key tiles (one for a small call), so that the loads of one item
-// spread over idle SMs.
+// Parts of the keys, so that one item's chain of key tiles is worked off by
+// several SMs. With fewer items than `want`, as many as still leave each two
+// key tiles (four above 32 parts: 19 against 22 us with 62 for 125 tiles). If a
+// join comes for their sake only, that has to be worth some 5 us, about five
+// tiles (24 heads of 512 x 512, d 128: 14.5 us whole, 20.5 in 3 parts; 16 of 77
+// x 1000, d 64: 15.9 and 10.7 in 4). `partial`: it comes anyway, and small
+// calls get a part for each tile.
 inline FwdPlan plan_fwd(int M, int G, int S, int B, int Hkv, int N, int D, int want, bool partial) {
   FwdPlan f;
   f.rows = pack_rows(M, G, S);
@@ -104,7 +108,11 @@ inline FwdPlan plan_fwd(int M, int G, int S, int B, int Hkv, int N, int D, int w
   const int64_t base = static_cast<int64_t>(f.pairs) * B * Hkv;
   const int nt = (N + kTile - 1) / kTile;
   f.splits = 1;
-  if (base < want) f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want / base, nt >= 16 ? nt / 2 : nt)));
+  if (base < want) {
+    const int most = partial && nt < 16 ? nt : std::min((nt + 1) / 2, std::max(32, nt / 4));
+    f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want / base, most)));
+    if (!partial && nt - (nt + f.splits - 1) / f.splits < 5) f.splits = 1;
+  }
   f.items = static_cast<int>(base * f.splits);
   f.all_rows = static_cast<int64_t>(B) * S * Hkv * G * M;
   f.ws_bytes = partial || f.splits > 1 ? static_cast<uint64_t>(f.splits) * f.all_rows * (D + 1) * 4 : 0;

@@ -80,6 +80,12 @@ SHAPES = [
     (1, 2, 1, 1, 20000, 64, "bf16", [19999], "bhnd", 1),
     (300, 1, 1, 1, 20, 64, "fp16", None, "bnhd", 1),
     (1, 6, 3, 64, 4000, 128, "fp16", [3999], "bnhd", 1),     # few rows, many keys
+    (2, 6, 3, 40, 2100, 64, "fp16", [2100, 0], "bnhd", 1),
+    (1, 2, 2, 130, 4200, 128, "bf16", [4199], "bnhd", 1),
+    (1, 4, 1, 700, 1000, 64, "bf16", None, "bnhd", 1),       # few items of many steps, both ways round
+    (1, 16, 2, 600, 77, 128, "bf16", [70], "bnhd", 1),
+    (3, 8, 8, 200, 900, 64, "fp16", [900, 3, 0], "apart", 1),
+    (1, 32, 4, 300, 900, 128, "bf16", None, "bnhd", 1),
 ]
 
 
