@@ -402,9 +402,12 @@ inline BwdPlan plan_bwd(const fmha_attn_t& a) {
     f.grid_q = std::min(f.grid_q, std::min(busy, kBesideQ));
     f.grid_k = std::min(f.grid_k, kPlanSms - f.grid_q);
   }
-  f.join = a.kv_lens != nullptr ||
-           bwd_by_steps((heads * f.pairs + f.grid_q - 1) / f.grid_q * nt, heads * f.pairs * nt, f.grid_q) ||
-           bwd_by_steps((heads * nt + f.grid_k - 1) / f.grid_k * f.rows.tiles, heads * nt * f.rows.tiles, f.grid_k);
+  // steps of the busiest CTA with whole items, no fewer than with any lengths
+  const int64_t whole_q = (heads * f.pairs + f.grid_q - 1) / f.grid_q * nt;
+  const int64_t whole_k = (heads * nt + f.grid_k - 1) / f.grid_k * f.rows.tiles;
+  f.join = a.kv_lens ? bwd_by_steps(std::max(whole_q, whole_k), 1, kPlanSms)
+                     : bwd_by_steps(whole_q, heads * f.pairs * nt, f.grid_q) ||
+                           bwd_by_steps(whole_k, heads * nt * f.rows.tiles, f.grid_k);
   f.packed_rows = heads * f.rows.tiles * kTile;
   f.delta_blocks = static_cast<int>(std::min<int64_t>(6 * kPlanSms, heads * std::max<int64_t>(f.rows.tiles, nt)));
   f.slot_floats = 2 * static_cast<int64_t>(kTile) * a.K_dim;
