@@ -410,6 +410,36 @@ def test_captured_graphs_replay_with_new_inputs(F):
                 assert all(torch.equal(x, y) for x, y in zip(xs, want[k])), k
 
 
+@pytest.mark.parametrize("M,Np", [(1, 20600), (20, 700)])
+def test_prefix_in_parts_on_streams_and_in_graphs(F, M, Np):
+    """The form of three launches that overlap, for single tokens and for more."""
+    Q, K, V, n = make(6, 8, 2, M, 70, 64, "bf16", [70, 0, 33, 1, 70, 16], seed=20)
+    _, Kp, Vp, np_ = make(2, 2, 2, 1, Np, 64, "bf16", [Np, 500], seed=21)
+    call = lambda **kw: F.prefix_attn(Q, Kp, Vp, K, V, np_, n, **kw)  # noqa: E731
+    want = call()
+    ref, lse, bound, lse_bound = R.prefix(Q, Kp, Vp, K, V, np_, n, 0.125)
+    R.check("O", want[0], ref, bound)
+    R.check("LSE", want[1], lse, lse_bound)
+    sides = [torch.cuda.Stream() for _ in range(3)]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [call(stream=s, sync=False) for _ in range(8) for s in sides]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for outs in got for x, y in zip(outs, want))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=sides[0]):
+        held = [call(sync=False) for _ in range(3)]
+    for factor in (1.0, 0.5):
+        for t in (Q, K, Vp):
+            t.mul_(factor)
+        want = call()
+        g.replay()
+        other = call(sync=False)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for outs in (*held, other) for x, y in zip(outs, want))
+
+
 def test_refusals_on_the_device(F):
     Q, K, V, n = make(2, 4, 2, 8, 16, 64, "bf16", [16, 3])
     dO, (O, LSE) = torch.ones_like(Q), saved(Q, K, V, n, 0.125)
