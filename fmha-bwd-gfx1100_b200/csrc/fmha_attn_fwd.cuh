@@ -347,6 +347,12 @@ __device__ __forceinline__ void weights_32(const uint32_t* s, float2 sc, float2 
   }
 }
 
+// 16384 rows, 1024 keys, 40 heads of 128, bf16: 315 to 355 us by the GPU's clock
+// (1.0 to 1.1 PFLOP/s). A step of both tiles takes 3.7 K clocks, of which the
+// exponentials take the SFU 2.0 K and the products the tensor core 2.0 K: each
+// tile's softmax waits for the products between its p and its next S. Few steps
+// are bound by latency: 3 to 4 us pass before the first S.
+//
 // kOwn: the keys of an entry's own tokens, behind a prefix: token m reads n - (M
 // - 1 - m) of them. It starts before the launch before it has ended, and waits
 // for that at its end.
@@ -729,6 +735,10 @@ constexpr int kJoinAhead = 4;
 // Joins the parts of split keys: with weights w_i = exp(LSE_i - max LSE),
 // O = sum w_i O_i / sum w_i and LSE = max LSE + log sum w_i, parts in order.
 // D / 4 lanes to a row: they hold the parts' weights, and take 4 columns each.
+// Bound by the latency of two loads in turn, so the first parts' O is asked for
+// before their weights are known; 24 warps an SM matter more than more loads a
+// thread (4 ahead: 18 us, 8 ahead and 16 warps: 20 for 333 x 777 in 3 parts).
+// 19 parts of 2048 rows of 128: 4 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 6)
     attn_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, int parts, int64_t rows,
