@@ -209,7 +209,9 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cas
 // Per packed row: -LSE log2e (0 for a row without keys, -inf where the tile
 // holds no row: P = 0) plus fp16's power of two of P, and -D. A block takes row
 // tiles one by one, D / 8 threads a row, several rows' loads in flight. In fp16
-// also the largest |dO| and valid |V| that the block saw. Bound by memory: 101
+// also the largest |dO| and valid |V| that the block saw. What the other kernels
+// have no items for is zeroed here: dQ of entries without keys, dK and dV behind
+// the last key (a tile's sums there would be NaN where Q or dO is). Bound by memory: 101
 // MB (2 x 24 heads, 4096 rows of 128) take 25 us from DRAM; more blocks with
 // fewer loads each were slower.
 template <typename T, int D>
@@ -233,6 +235,7 @@ __global__ void __launch_bounds__(256)
     // kv heads innermost: with the usual [token][head] layouts, the blocks read neighbouring memory
     const int hk = i % p.Hkv, tile = i / p.Hkv % p.rows.tiles, b = i / p.Hkv / p.rows.tiles;
     const int64_t base = ((static_cast<int64_t>(b) * p.Hkv + hk) * p.rows.tiles + tile) * kTile;
+    const bool empty = valid_rows(p.lens, b, p.N) == 0;
 #pragma unroll 1
     for (int r = r0; r < kTile; r += kBatch * kStep) {
       uint4 x[kBatch], y[kBatch];
@@ -245,6 +248,7 @@ __global__ void __launch_bounds__(256)
         x[i4] = y[i4] = make_uint4(0, 0, 0, 0);
         l[i4] = 0.f;
         if (real[i4]) {
+          if (empty) reinterpret_cast<uint4*>(p.dQ.at(b, hk * p.rows.G + g, m))[chunk] = make_uint4(0, 0, 0, 0);
           x[i4] = __ldg(reinterpret_cast<const uint4*>(dO.at(b, hk * p.rows.G + g, m)) + chunk);
           y[i4] = __ldg(reinterpret_cast<const uint4*>(O.at(b, hk * p.rows.G + g, m)) + chunk);
           l[i4] = __ldg(LSE + (static_cast<int64_t>(b) * p.Hkv * p.rows.G + hk * p.rows.G + g) * p.rows.M + m);
@@ -271,21 +275,29 @@ __global__ void __launch_bounds__(256)
       }
     }
   }
-  if (!Elem<T>::kBF16) {
+  if (!Elem<T>::kBF16 || p.lens) {
     const int nt = (p.N + kTile - 1) / kTile, key_tiles = p.B * p.Hkv * nt;
     for (int i = blockIdx.x; i < key_tiles; i += gridDim.x) {
       const int bh = i / nt, hk = bh % p.Hkv, b = bh / p.Hkv;
       const int n = valid_rows(p.lens, b, p.N);
+      if (Elem<T>::kBF16 && (i % nt + 1) * kTile <= n) continue;
 #pragma unroll 4
       for (int r = r0; r < kTile; r += kStep) {
         const int key = i % nt * kTile + r;
-        if (key < n) {
+        if (key >= n) {
+          if (key < p.N) {
+            reinterpret_cast<uint4*>(p.dK.at(b, hk, key))[chunk] = make_uint4(0, 0, 0, 0);
+            reinterpret_cast<uint4*>(p.dV.at(b, hk, key))[chunk] = make_uint4(0, 0, 0, 0);
+          }
+        } else if (!Elem<T>::kBF16) {
           const uint4 x = __ldg(reinterpret_cast<const uint4*>(V.at(b, hk, key)) + chunk);
           const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
           top_v = widest(top_v, xw);
         }
       }
     }
+  }
+  if (!Elem<T>::kBF16) {
     __shared__ float2 tops[8];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -301,18 +313,6 @@ __global__ void __launch_bounds__(256)
       }
       amax[blockIdx.x] = make_float2(top_do, top_v);
     }
-  }
-}
-
-// Zeroes rows [from, rows) of each head of a tensor, by the given threads.
-template <typename T, int D>
-__device__ __forceinline__ void zero_rows(const View<T>& v, int b, int heads, int from, int rows, int64_t thread,
-                                          int64_t threads) {
-  const int64_t per = static_cast<int64_t>(rows - from) * (D / 8);
-  for (int64_t i = thread; i < per * heads; i += threads) {
-    const int h = static_cast<int>(i / per);
-    const int64_t w = i % per;
-    *(reinterpret_cast<uint4*>(v.at(b, h, from + w / (D / 8))) + w % (D / 8)) = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -513,15 +513,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       __syncwarp();
     } else if (warp == kUnitWarp) {
-      if (lane == 0) {
-        feed_units<T, true>(p, ring, unit_full, unit_empty, ctx, 305);
-      } else if (p.lens) {
-        // the other lanes: entries without keys have dQ = 0
-        for (int b = 0; b < p.B; ++b)
-          if (valid_rows(p.lens, b, p.N) == 0)
-            zero_rows<T, D>(p.dQ, b, p.Hkv * p.rows.G, 0, p.rows.M, static_cast<int64_t>(blockIdx.x) * 31 + lane - 1,
-                            31ll * gridDim.x);
-      }
+      if (lane == 0) feed_units<T, true>(p, ring, unit_full, unit_empty, ctx, 305);
       __syncwarp();
     } else {
       // ---- MMA issuer of tile t: per step dP, dQ, and S of the next step. A
@@ -898,20 +890,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       __syncwarp();
     } else if (warp == kUnitWarp) {
-      if (lane == 0) {
-        feed_units<T, false>(p, ring, unit_full, unit_empty, ctx, 405);
-      } else if (p.lens) {
-        // the other lanes: dK = dV = 0 behind the last key. (The sums of a
-        // tile would do if Q and dO held neither infinities nor NaN.)
-        const int64_t thread = static_cast<int64_t>(blockIdx.x) * 31 + lane - 1, threads = 31ll * gridDim.x;
-        for (int b = 0; b < p.B; ++b) {
-          const int from = valid_rows(p.lens, b, p.N);
-          if (from < p.N) {
-            zero_rows<T, D>(p.dK, b, p.Hkv, from, p.N, thread, threads);
-            zero_rows<T, D>(p.dV, b, p.Hkv, from, p.N, thread, threads);
-          }
-        }
-      }
+      if (lane == 0) feed_units<T, false>(p, ring, unit_full, unit_empty, ctx, 405);
       __syncwarp();
     } else {
       // ---- MMA issuers: the first dV and S^T of the next row tile (TMEM S, P),
