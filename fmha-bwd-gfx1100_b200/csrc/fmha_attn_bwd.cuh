@@ -235,7 +235,14 @@ __global__ void __launch_bounds__(256)
     // kv heads innermost: with the usual [token][head] layouts, the blocks read neighbouring memory
     const int hk = i % p.Hkv, tile = i / p.Hkv % p.rows.tiles, b = i / p.Hkv / p.rows.tiles;
     const int64_t base = ((static_cast<int64_t>(b) * p.Hkv + hk) * p.rows.tiles + tile) * kTile;
-    const bool empty = valid_rows(p.lens, b, p.N) == 0;
+    if (valid_rows(p.lens, b, p.N) == 0) {  // apart from the loads below, which must not wait for it
+#pragma unroll 1
+      for (int r = r0; r < kTile; r += kStep) {
+        int m, g, s;
+        if (p.rows.row(tile, r, m, g, s))
+          reinterpret_cast<uint4*>(p.dQ.at(b, hk * p.rows.G + g, m))[chunk] = make_uint4(0, 0, 0, 0);
+      }
+    }
 #pragma unroll 1
     for (int r = r0; r < kTile; r += kBatch * kStep) {
       uint4 x[kBatch], y[kBatch];
@@ -248,7 +255,6 @@ __global__ void __launch_bounds__(256)
         x[i4] = y[i4] = make_uint4(0, 0, 0, 0);
         l[i4] = 0.f;
         if (real[i4]) {
-          if (empty) reinterpret_cast<uint4*>(p.dQ.at(b, hk * p.rows.G + g, m))[chunk] = make_uint4(0, 0, 0, 0);
           x[i4] = __ldg(reinterpret_cast<const uint4*>(dO.at(b, hk * p.rows.G + g, m)) + chunk);
           y[i4] = __ldg(reinterpret_cast<const uint4*>(O.at(b, hk * p.rows.G + g, m)) + chunk);
           l[i4] = __ldg(LSE + (static_cast<int64_t>(b) * p.Hkv * p.rows.G + hk * p.rows.G + g) * p.rows.M + m);
