@@ -636,6 +636,7 @@ __global__ void __launch_bounds__(32 * StreamCfg<D, R>::kWarps, 1)
         *reinterpret_cast<uint4*>(src + kV + (c >> 3) * Cfg::kBox + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
             make_uint4(0, 0, 0, 0);
       }
+      fence_proxy_async_smem();  // the next copy into this stage comes behind these stores
       __syncwarp();
     }
     // 16 bytes at column 8 `chunk` of a key's row
