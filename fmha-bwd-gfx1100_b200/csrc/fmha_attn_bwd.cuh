@@ -620,10 +620,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         __syncwarp();
         tc_fence_after();
         uint32_t s[64];
-        tmem_load_32_start(tR, s);
-        tmem_load_32_start(tR + 32, s + 32);
-        tmem_load_32_wait(s);
-        tmem_load_32_wait(s + 32);
+        tmem_load_32(tR, s);
+        tmem_load_32(tR + 32, s + 32);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[kBqSRead0 + t]);

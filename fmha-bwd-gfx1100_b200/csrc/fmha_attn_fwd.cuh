@@ -606,17 +606,13 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
           mask_columns(tS, least + min(tok, p.rows.M - 1), least);
         }
         uint32_t s[128];
-        tmem_load_64_start(tS, s);
-        tmem_load_64_wait(s);
-        tmem_load_64_start(tS + 64, s + 64);
+        tmem_load_64(tS, s);
+        tmem_load_64(tS + 64, s + 64);
         float mx[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) mx[x] = __uint_as_float(s[x]);
 #pragma unroll
-        for (int x = 4; x < 64; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
-        tmem_load_64_wait(s + 64);
-#pragma unroll
-        for (int x = 64; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
+        for (int x = 4; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2 - kBias;
         if (j == it.lo) {
           m = top == -INFINITY ? 0.f : top;

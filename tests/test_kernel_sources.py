@@ -37,3 +37,15 @@ def test_zeroes_in_a_landed_tile_come_before_the_next_copy_into_it():
         for m in stores:
             between = text[m.end():m.end() + re.search(copies, text[m.end():]).start()]
             assert "fence_proxy_async_smem();" in between, f"{name}: no proxy fence behind {m.group()!r}"
+
+
+def test_every_tmem_load_waits_in_its_own_statement():
+    """tcgen05.ld writes its registers some time after it was issued: between it
+    and a wait in another statement the compiler may copy or spill them."""
+    text = source("sm100_ptx.cuh")
+    loads = [m.group() for m in re.finditer(r"asm volatile\(.*?\);\n", text, re.S) if "tcgen05.ld." in m.group()]
+    assert len(loads) >= 5
+    for statement in loads:
+        assert "tcgen05.wait::ld.sync.aligned;" in statement, statement[:120]
+    for name in sorted(os.listdir(CSRC)):
+        assert name == "sm100_ptx.cuh" or "tcgen05.ld." not in source(name), name
