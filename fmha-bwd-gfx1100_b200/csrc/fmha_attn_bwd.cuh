@@ -21,9 +21,11 @@
 // them in order.
 //
 // P and dS are rounded to 16 bits for the tensor cores, after dS was formed
-// from the fp32 P. In fp16, P is held times 2^10 and dS times 2^e with e from
-// the largest |dO| and |V|, so that 2 d |dO| |V| 2^e <= 65504: dS cannot
-// overflow, and gradients of any size keep fp16's precision.
+// from the fp32 P. In fp16, P is held times 2^10 and dS times 2^e, with an e for
+// each kv head of an entry from its own largest finite |dO| and |V|, so that 2 d
+// |dO| |V| 2^e <= 2^15: dS cannot overflow, and what the other heads and entries
+// hold takes nothing from its precision. Within a head, dS below 2^-29 of that
+// bound falls to fp16's subnormals.
 #pragma once
 
 #include "fmha_attn_fwd.cuh"
@@ -38,8 +40,8 @@ struct BwdParams {
   View<T> dQ, dK, dV;
   const float* nlse2;   // [B * Hkv * tiles * 128] -LSE log2e (+ 10 in fp16), packed rows
   const float* ndelta;  // the same rows' -D
-  const float2* amax; // [blocks of attn_delta_kernel]: largest |dO|, |V| (fp16 only)
-  int amax_count;
+  const float* top_do;  // [B * Hkv][row tiles], fp16 only: a tile's largest finite |dO|
+  const float* top_v;   // [B * Hkv][key tiles], fp16 only: and |V| of its valid keys
   float* part;        // [2 * grid][2][128][D] partial sums
   float scale;
   KernelStatus* status;
@@ -57,6 +59,7 @@ struct BwdUnit {
   int len;         // its steps in all
   int slot;        // partial-sum slot, or -1 for a whole item
   int n;           // valid keys of the entry
+  int exp;         // the power of two by which dS is held (ds_exponent)
 };
 
 // Steps that a division by steps has to save, as its partial sums cost about
@@ -153,16 +156,40 @@ struct BwdSchedule {
   }
 };
 
-template <typename T, bool kQMajor>
+// The power of two by which a whole warp's fp16 holds dS of a unit's kv head
+// (see the top): -25 to 54; 0 for bf16, and where all gradients are zero.
+constexpr int kExpBias = 64;
+template <typename T, int D>
+__device__ __forceinline__ int ds_exponent(const BwdParams<T>& p, const BwdUnit& u, int lane) {
+  if (Elem<T>::kBF16) return 0;
+  const int64_t bh = static_cast<int64_t>(u.b) * p.Hkv + u.hk;
+  const int key_tiles = (p.N + kTile - 1) / kTile;
+  // no float here has a sign, so their bits compare as they do
+  uint32_t x = 0, y = 0;
+  for (int i = lane; i < p.rows.tiles; i += 32) x = max(x, __float_as_uint(__ldcg(p.top_do + bh * p.rows.tiles + i)));
+  for (int i = lane; i * kTile < u.n; i += 32) y = max(y, __float_as_uint(__ldcg(p.top_v + bh * key_tiles + i)));
+  x = __reduce_max_sync(0xffffffffu, x);
+  y = __reduce_max_sync(0xffffffffu, y);
+  if (x == 0 || y == 0) return 0;
+  // below 2^ex and 2^ey
+  const int ex = static_cast<int>(x >> 23) - 126, ey = static_cast<int>(y >> 23) - 126;
+  return 15 - (D == 128 ? 8 : 7) - ex - ey;  // 2 d 2^ex 2^ey 2^e = 2^15
+}
+
+template <typename T, int D, bool kQMajor>
 __device__ void feed_units(const BwdParams<T>& p, UnitRing* ring, uint64_t* full, uint64_t* empty, const WaitCtx& ctx,
                            int where) {
   BwdSchedule<T, kQMajor> sched(p, gridDim.x, blockIdx.x);
+  const int lane = threadIdx.x & 31;
   BwdUnit u{};
   for (int k = 0;; ++k) {
     const bool more = sched.next(u);
-    if (!put_unit(ring, full, empty, k, make_int4(u.b, u.hk, u.idx, u.slot), make_int4(u.lo, u.hi, u.n, more ? 1 : 0),
-                  ctx, where) || !more)
-      return;
+    const int exp = more ? ds_exponent<T, D>(p, u, lane) : 0;
+    bool ok = true;
+    if (lane == 0)
+      ok = put_unit(ring, full, empty, k, make_int4(u.b, u.hk, u.idx, u.slot),
+                    make_int4(u.lo, u.hi, u.n, more ? kExpBias + exp : 0), ctx, where);
+    if (!__all_sync(0xffffffffu, ok) || !more) return;
   }
 }
 
@@ -178,29 +205,8 @@ __device__ __forceinline__ bool take_unit(const UnitRing* ring, uint64_t* full, 
   u.lo = b.x;
   u.hi = b.y;
   u.n = b.z;
+  u.exp = b.w - kExpBias;
   return true;
-}
-
-// The power of two by which fp16 holds dS (see the top), 0 for bf16.
-template <typename T, int D>
-__device__ __forceinline__ int ds_exponent(const BwdParams<T>& p, int lane) {
-  if (Elem<T>::kBF16) return 0;
-  float2 a = make_float2(0.f, 0.f);
-  for (int i = lane; i < p.amax_count; i += 32) {
-    const float2 v = __ldcg(p.amax + i);
-    a.x = fmaxf(a.x, v.x);
-    a.y = fmaxf(a.y, v.y);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a.x = fmaxf(a.x, __shfl_xor_sync(0xffffffffu, a.x, o));
-    a.y = fmaxf(a.y, __shfl_xor_sync(0xffffffffu, a.y, o));
-  }
-  // exponents e with x < 2^e; a zero, infinity or NaN leaves dS as it is
-  if (!(a.x > 0.f && a.x < INFINITY && a.y > 0.f && a.y < INFINITY)) return 0;
-  const int ex = static_cast<int>(__float_as_uint(a.x) >> 23) - 126, ey = static_cast<int>(__float_as_uint(a.y) >> 23) - 126;
-  const int e = 15 - (D == 128 ? 8 : 7) - ex - ey;  // 2 d 2^ex 2^ey 2^e = 2^15
-  return e < -40 ? -40 : (e > 60 ? 60 : e);
 }
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
@@ -209,7 +215,7 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cas
 // Per packed row: -LSE log2e (0 for a row without keys, -inf where the tile
 // holds no row: P = 0) plus fp16's power of two of P, and -D. A block takes row
 // tiles one by one, D / 8 threads a row, several rows' loads in flight. In fp16
-// also the largest |dO| and valid |V| that the block saw. What the other kernels
+// also a tile's largest finite |dO|, and a key tile's |V|. What the other kernels
 // have no items for is zeroed here: dQ of entries without keys, dK and dV behind
 // the last key (a tile's sums there would be NaN where Q or dO is). Bound by memory: 101
 // MB (2 x 24 heads, 4096 rows of 128) take 25 us from DRAM; more blocks with
@@ -217,19 +223,36 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cas
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
     attn_delta_kernel(View<T> dO, View<T> O, View<T> V, const float* __restrict__ LSE, BwdParams<T> p,
-                      float* __restrict__ nlse2, float* __restrict__ ndelta, float2* __restrict__ amax) {
+                      float* __restrict__ nlse2, float* __restrict__ ndelta, float* __restrict__ top_do,
+                      float* __restrict__ top_v) {
   constexpr int kPer = D / 8, kStep = 256 / kPer, kBatch = 4;  // threads a row, rows a pass, passes at once
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int chunk = threadIdx.x % kPer, r0 = threadIdx.x / kPer;
   const int tiles = p.B * p.Hkv * p.rows.tiles;
-  float top_do = 0.f, top_v = 0.f;
-  auto widest = [](float top, const uint32_t (&w)[4]) {
+  // largest magnitudes, two fp16 a word; infinities and NaN are left out
+  uint32_t top = 0;
+  auto widest = [&](const uint32_t (&w)[4]) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const float2 v = Elem<T>::unpack(w[x]);
-      top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+      const uint32_t a = w[x] & 0x7fff7fffu;
+      top = __vmaxu2(top, a & __vcmpltu2(a, 0x7c007c00u));
     }
-    return top;
+  };
+  // the block's, to `out`; each call's words are the other ones than the last's,
+  // so that one barrier keeps them apart
+  __shared__ uint32_t tops[2][8];
+  int turn = 0;
+  auto leave = [&](float* out) {
+    top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+    if (threadIdx.x % 32 == 0) tops[turn][threadIdx.x / 32] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int w = 1; w < 8; ++w) top = max(top, tops[turn][w]);
+      *out = __half2float(__ushort_as_half(static_cast<unsigned short>(top)));
+    }
+    turn ^= 1;
+    top = 0;
   };
   for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
     // kv heads innermost: with the usual [token][head] layouts, the blocks read neighbouring memory
@@ -270,7 +293,7 @@ __global__ void __launch_bounds__(256)
           acc = fmaf(a.x, c.x, acc);
           acc = fmaf(a.y, c.y, acc);
         }
-        if (!Elem<T>::kBF16) top_do = widest(top_do, xw);
+        if (!Elem<T>::kBF16) widest(xw);
 #pragma unroll
         for (int o = kPer / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o, kPer);
         if (chunk == 0) {
@@ -280,6 +303,7 @@ __global__ void __launch_bounds__(256)
         }
       }
     }
+    if (!Elem<T>::kBF16) leave(top_do + base / kTile);
   }
   if (!Elem<T>::kBF16 || p.lens) {
     const int nt = (p.N + kTile - 1) / kTile, key_tiles = p.B * p.Hkv * nt;
@@ -298,26 +322,10 @@ __global__ void __launch_bounds__(256)
         } else if (!Elem<T>::kBF16) {
           const uint4 x = __ldg(reinterpret_cast<const uint4*>(V.at(b, hk, key)) + chunk);
           const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-          top_v = widest(top_v, xw);
+          widest(xw);
         }
       }
-    }
-  }
-  if (!Elem<T>::kBF16) {
-    __shared__ float2 tops[8];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      top_do = fmaxf(top_do, __shfl_xor_sync(0xffffffffu, top_do, o));
-      top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
-    }
-    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = make_float2(top_do, top_v);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < 8; ++w) {
-        top_do = fmaxf(top_do, tops[w].x);
-        top_v = fmaxf(top_v, tops[w].y);
-      }
-      amax[blockIdx.x] = make_float2(top_do, top_v);
+      if (!Elem<T>::kBF16) leave(top_v + (static_cast<int64_t>(b) * p.Hkv + hk) * nt + i % nt);
     }
   }
 }
@@ -434,7 +442,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   WaitCtx ctx{abort_flag, p.timeout_ns};
-  // nlse2, ndelta and the exponents come from the launch before; the launch after needs only those
+  // nlse2, ndelta and the magnitudes come from the launch before; the launch after needs only those
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int q_tiles = p.rows.tiles;
@@ -519,7 +527,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       __syncwarp();
     } else if (warp == kUnitWarp) {
-      if (lane == 0) feed_units<T, true>(p, ring, unit_full, unit_empty, ctx, 305);
+      feed_units<T, D, true>(p, ring, unit_full, unit_empty, ctx, 305);
       __syncwarp();
     } else {
       // ---- MMA issuer of tile t: per step dP, dQ, and S of the next step. A
@@ -607,13 +615,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int t = warp >> 3, c = warp >> 2 & 1, r = threadIdx.x & 127;
     const uint32_t tR = tmem + 128 * t + 64 * c + (static_cast<uint32_t>(r & 96) << 16);
     const float sl2 = p.scale * kLog2e;
-    const float ds_mul = pow2(ds_exponent<T, D>(p, lane) - kPBias);
     int ns = 0;
     while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 319, ok)) {
       const int tile = 2 * u.idx + t;
       if (tile >= q_tiles) continue;
       const int64_t row = ((static_cast<int64_t>(u.b) * p.Hkv + u.hk) * q_tiles + tile) * kTile + r;
       const float nl = __ldcg(p.nlse2 + row);
+      const float ds_mul = pow2(u.exp - kPBias);
       const float nd = ds_mul * __ldcg(p.ndelta + row);
       for (int j = u.lo; j < u.hi; ++j, ++ns) {
         if (!mbar_wait(&bar[kBqSFull0 + t], ns & 1, ctx, 320)) { ok = false; break; }
@@ -665,7 +673,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     // last K tile behind the last key, for the issuers that wait for it
     regs_lower<kDqOtherRegs>();
     const int r = threadIdx.x & 127;
-    const float out_mul = p.scale * pow2(-ds_exponent<T, D>(p, lane));
     int na0 = 0, na1 = 0, g = 0;
     uint32_t tail_turns = 0;
     while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 329, ok)) {
@@ -696,7 +703,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                        : real      ? reinterpret_cast<uint8_t*>(p.dQ.at(u.b, u.hk * p.rows.G + g, m))
                                    : nullptr;
         store_sums<T, D, 16>(tmem + 256 + D * t + (static_cast<uint32_t>(r & 96) << 16), u.slot >= 0, out,
-                         u.slot >= 0 ? 1.f : out_mul);
+                         u.slot >= 0 ? 1.f : p.scale * pow2(-u.exp));
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[kBqAccEmpty0 + t]);
@@ -894,7 +901,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       __syncwarp();
     } else if (warp == kUnitWarp) {
-      if (lane == 0) feed_units<T, false>(p, ring, unit_full, unit_empty, ctx, 405);
+      feed_units<T, D, false>(p, ring, unit_full, unit_empty, ctx, 405);
       __syncwarp();
     } else {
       // ---- MMA issuers: the first dV and S^T of the next row tile (TMEM S, P),
@@ -965,11 +972,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(r & 96) << 16;
     const uint32_t tS = tmem + Cfg::kColS + 32 * c + lanes, tX = tmem + Cfg::kColX + 32 * c + lanes;
     const float2 sl2 = make_float2(p.scale * kLog2e, p.scale * kLog2e);
-    const float ds_mul = pow2(ds_exponent<T, D>(p, lane) - kPBias);
     int n = 0;
     while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 419, ok)) {
       // a key that does not count gets P = dS = 0, whatever K and V hold
       const bool valid = u.idx * kTile + r < u.n;
+      const float ds_mul = pow2(u.exp - kPBias);
       for (int i = u.lo; i < u.hi; ++i, ++n) {
         const float4* nl = reinterpret_cast<const float4*>(smem + Cfg::kOffL + (n & 1) * 2 * kTile * 4) + 8 * c;
         const float4* nd = nl + kTile / 4;
@@ -1043,7 +1050,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     // ---- dV and dK: thread = key
     const int r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(r & 96) << 16;
-    const float dk_mul = p.scale * pow2(-ds_exponent<T, D>(p, lane)), dv_mul = pow2(-kPBias);
     int nu = 0;
     while (take_unit<true>(ring, unit_full, unit_empty, k, u, ctx, 429, ok)) {
       if (!mbar_wait(&bar[kBkAcc], nu & 1, ctx, 430)) { ok = false; continue; }
@@ -1059,7 +1065,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                        : key < u.n ? reinterpret_cast<uint8_t*>(v.at(u.b, u.hk, key))
                                    : nullptr;
         store_sums<T, D, 32>(tmem + (which == 0 ? Cfg::kColdV : Cfg::kColdK) + lanes, u.slot >= 0, out,
-                         u.slot >= 0 ? 1.f : (which == 0 ? dv_mul : dk_mul));
+                         u.slot >= 0 ? 1.f : (which == 0 ? pow2(-kPBias) : p.scale * pow2(-u.exp)));
       }
       tc_fence_before();
       __syncwarp();
@@ -1123,7 +1129,7 @@ __global__ void __launch_bounds__(256)
   const JoinItem it = shared;
   if (it.slots == 0) return;
   const BwdParams<T>& p = q_major ? q : kv;
-  const int ds_exp = ds_exponent<T, D>(p, threadIdx.x & 31);
+  const int ds_exp = ds_exponent<T, D>(p, it.u, threadIdx.x & 31);
   const float4* part = reinterpret_cast<const float4*>(p.part);
   for (int e = blockIdx.x * 256 + threadIdx.x; e < 2 * kTile * (D / 4); e += kJoinBlocks * 256) {
     const int which = e / (kTile * (D / 4)), row = e / (D / 4) % kTile, col = e % (D / 4);

@@ -371,12 +371,12 @@ inline FwdPlan own_plan(const fmha_attn_t& a) {
 }
 
 // How a backward divides its work, and its workspace: packed LSE and D, the
-// amplitudes (fp16), and two partial-sum slots for each CTA of both kernels.
+// tiles' magnitudes (fp16), and two partial-sum slots for each CTA of both kernels.
 struct BwdPlan {
   RowPack rows;
   int pairs, grid_q, grid_k, delta_blocks;
   bool join;  // some item may fall to several CTAs
-  int64_t packed_rows, slot_floats;
+  int64_t packed_rows, row_tiles, key_tiles, slot_floats;
   uint64_t ws_bytes;
 };
 
@@ -408,10 +408,12 @@ inline BwdPlan plan_bwd(const fmha_attn_t& a) {
   f.join = a.kv_lens ? bwd_by_steps(std::max(whole_q, whole_k), 1, kPlanSms)
                      : bwd_by_steps(whole_q, heads * f.pairs * nt, f.grid_q) ||
                            bwd_by_steps(whole_k, heads * nt * f.rows.tiles, f.grid_k);
-  f.packed_rows = heads * f.rows.tiles * kTile;
+  f.row_tiles = heads * f.rows.tiles;
+  f.key_tiles = heads * nt;
+  f.packed_rows = f.row_tiles * kTile;
   f.delta_blocks = static_cast<int>(std::min<int64_t>(6 * kPlanSms, heads * std::max<int64_t>(f.rows.tiles, nt)));
   f.slot_floats = 2 * static_cast<int64_t>(kTile) * a.K_dim;
-  f.ws_bytes = 4 * static_cast<uint64_t>(2 * f.packed_rows + 2 * ((f.delta_blocks + 1) / 2 * 2) +
+  f.ws_bytes = 4 * static_cast<uint64_t>(2 * f.packed_rows + (f.row_tiles + f.key_tiles + 3) / 4 * 4 +
                                          2 * (f.grid_q + f.grid_k) * f.slot_floats);
   return f;
 }
@@ -431,7 +433,8 @@ int enqueue_bwd(const fmha_attn_t& a, int device, cudaStream_t stream) {
     return set_error(kErrInvalidArgument, "tensor map encoding failed");
   float* nlse2 = static_cast<float*>(a.workspace);
   float* ndelta = nlse2 + f.packed_rows;
-  float2* amax = reinterpret_cast<float2*>(ndelta + f.packed_rows);
+  float* top_do = ndelta + f.packed_rows;
+  float* top_v = top_do + f.row_tiles;
   BwdParams<T> q;
   q.rows = f.rows;
   q.B = a.batch;
@@ -444,9 +447,9 @@ int enqueue_bwd(const fmha_attn_t& a, int device, cudaStream_t stream) {
   q.dV = view_of<T>(a.dV);
   q.nlse2 = nlse2;
   q.ndelta = ndelta;
-  q.amax = amax;
-  q.amax_count = f.delta_blocks;
-  q.part = reinterpret_cast<float*>(amax + (f.delta_blocks + 1) / 2 * 2);
+  q.top_do = top_do;
+  q.top_v = top_v;
+  q.part = top_do + (f.row_tiles + f.key_tiles + 3) / 4 * 4;
   q.scale = a.softmax_scale;
   q.status = st;
   q.timeout_ns = effective_timeout_ns();
@@ -457,7 +460,7 @@ int enqueue_bwd(const fmha_attn_t& a, int device, cudaStream_t stream) {
     allow_smem<attn_dq_kernel<T, D>>(DqCfg2<D>::kSmemBytes, device);
     allow_smem<attn_dkv_kernel<T, D>>(DkvCfg2<D>::kSmemBytes, device);
     attn_delta_kernel<T, D><<<f.delta_blocks, 256, 0, stream>>>(view_of<T>(a.dO), view_of<T>(a.O), view_of<T>(a.V),
-                                                               a.LSE, q, nlse2, ndelta, amax);
+                                                               a.LSE, q, nlse2, ndelta, top_do, top_v);
     cudaError_t e = launch_after(true, attn_dq_kernel<T, D>, dim3(f.grid_q), kBwdThreads, DqCfg2<D>::kSmemBytes, stream, mQ,
                                  mK, mV, mdO, q);
     if (e == cudaSuccess)

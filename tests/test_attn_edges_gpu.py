@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import attn_reference as R
-from test_cross_gpu import DT, F, make  # noqa: F401 (F is a fixture)
+from test_cross_gpu import DT, F, make, saved, tensor  # noqa: F401 (F is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +27,82 @@ def test_many_ends_of_entries_in_one_stream(F, name, d):
     for _ in range(20):
         again = F.cross_attn_fwd(Q, K, V, n)
         assert torch.equal(O, again[0]) and torch.equal(LSE, again[1])
+
+
+# ----------------------------------------------------- gradients of unlike sizes
+def group_gradients(Q, K, V, O, LSE, dO, n, scale):
+    """R.backward's gradients and bounds of one entry's kv head ([G, M, d], [n, d]
+    of its valid keys), with fp16's dS held times the power of two that this
+    head's largest finite |dO| and |V| allow: below 2^e and 2^e' they leave
+    2^(14 - log2 d - e - e') or more, so a half-step of 2^-25 stands for at most
+    2^-25 2^-14 d (2 max|dO|) (2 max|V|) = d 2^-37 max|dO| max|V|."""
+    G, M, d = Q.shape
+    u, sub = R.roundings(Q.dtype)
+    q, k, v, o, do = Q.double(), K[:n].double(), V[:n].double(), O.double(), dO.double()
+    S = scale * q @ k.T
+    err = (d + 4) * R.E * scale * (q.abs() @ k.abs().T) + 4 * R.E * S.abs()
+    lse = LSE.double()[..., None]
+    P = torch.exp(S - lse)
+    rel_p = 1.01 * err + 2.0 ** -21 + 4 * R.E * lse.abs()
+    dP, D = do @ v.T, (do * o).sum(-1, keepdim=True)
+    dS = P * (dP - D)
+    acc = (d + 4) * R.E
+    e_s = P * acc * (do.abs() @ v.abs().T + (do.abs() * o.abs()).sum(-1, keepdim=True)) + (u + rel_p + 4 * R.E) * dS.abs()
+    if Q.dtype == torch.float16:
+        e_s = e_s + d * 2.0 ** -37 * float(do[do.isfinite()].abs().max()) * float(v.abs().max())
+    many = (G * M + 8) * R.E
+    dQ, bQ = scale * dS @ k, scale * (e_s + (n + 8) * R.E * dS.abs()) @ k.abs()
+    dK = (scale * dS.mT @ q).sum(0)
+    bK = (scale * (e_s + many * dS.abs()).mT @ q.abs()).sum(0)
+    dV = (P.mT @ do).sum(0)
+    bV = (((u + rel_p + many) * P + sub * 2.0 ** -10).mT @ do.abs()).sum(0)
+    return (dQ, dK, dV), tuple((1 + u) * b + u * x.abs() + sub for b, x in zip((bQ, bK, bV), (dQ, dK, dV)))
+
+
+# sizes of dO and of V, for each entry and each of its two kv heads
+UNLIKE = {
+    "entries": ([[300, 300], [0.02, 0.02], [300, 300]], [[16, 16], [1, 1], [16, 16]]),
+    "heads": ([[300, 0.02], [0.02, 300], [1e-3, 1]], [[16, 1], [0.05, 16], [1, 1]]),
+    "tiny": ([[1, 1e-4], [1e-4, 1e-4], [1, 1]], [[1, 1], [1, 0.02], [1, 1]]),
+}
+
+
+@pytest.mark.parametrize("M,N", [(40, 77), (300, 777)])
+@pytest.mark.parametrize("sizes", sorted(UNLIKE))
+@pytest.mark.parametrize("name,d", [("fp16", 64), ("fp16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("wild", [None, "entry without keys", "one row"])
+def test_gradients_of_entries_and_heads_of_unlike_sizes(F, M, N, sizes, name, d, wild):
+    """Each head's gradients keep their own precision whatever the others hold:
+    sizes 1e4 and more apart, an entry without keys whose dO is infinite, and one
+    row of dO that is (its own head's dQ is right in the other rows)."""
+    lens = [N, N - 20, 0]
+    Q, K, V, n = make(3, 4, 2, M, N, d, name, lens, seed=41)
+    dO = tensor(torch.Generator(device="cuda").manual_seed(42), 3, 4, M, d, DT[name])
+    of_do, of_v = (torch.tensor(x, device="cuda")[:, :, None, None] for x in UNLIKE[sizes])
+    dO = (dO.float() * of_do.repeat_interleave(2, 1)).to(dO.dtype)
+    V = (V.float() * of_v).to(V.dtype)
+    O, LSE = saved(Q, K, V, n, d ** -0.5)
+    odd = None
+    if wild == "entry without keys":
+        dO[2] = float("inf")
+    if wild == "one row":
+        odd = (1, 2, M // 2)
+        dO[odd] = float("inf")
+    got = F.cross_attn_bwd(Q, K, V, O, LSE, dO, n)
+    for b in range(2):
+        for h in range(2):
+            hs = slice(2 * h, 2 * h + 2)
+            do = dO[b, hs].clone()
+            alone = odd is None or (b, h) != (odd[0], odd[1] // 2)
+            if not alone:  # its row's sums are not finite; the other rows do not know of it
+                do[odd[1] % 2, odd[2]] = 0
+            outs, bounds = group_gradients(Q[b, hs], K[b, h], V[b, h], O[b, hs], LSE[b, hs], do, lens[b], d ** -0.5)
+            x = got[0][b, hs].clone()
+            if not alone:
+                x[odd[1] % 2, odd[2]] = 0
+            R.check(f"dQ of {b}, {h}", x, outs[0], bounds[0])
+            if alone:
+                R.check(f"dK of {b}, {h}", got[1][b, h, :lens[b]], outs[1], bounds[1])
+                R.check(f"dV of {b}, {h}", got[2][b, h, :lens[b]], outs[2], bounds[2])
+            assert not got[1][b, h, lens[b]:].any() and not got[2][b, h, lens[b]:].any()
+    assert not any(x[2].any() for x in got)
