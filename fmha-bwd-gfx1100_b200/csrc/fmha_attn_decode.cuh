@@ -125,8 +125,6 @@ struct DecodeParams {
   uint64_t timeout_ns;
 };
 
-constexpr float kNoMax = -3.0e38f;  // the reference of a row before its first key
-
 // A warp's share of one tile of rows: Q, the sums and what they refer to.
 template <typename T, int D, int R>
 struct DecodeWarp {

@@ -35,6 +35,7 @@
 namespace fmha_sm100 {
 
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNoMax = -3.0e38f;  // the reference of a row before its first weight
 
 // Units of work that one warp of a CTA works out and the others take from a
 // ring in shared memory: the divisions are done once, and the other roles hold
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         for (int x = 4; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2 - kBias;
         if (j == it.lo) {
-          m = top == -INFINITY ? 0.f : top;
+          m = fmaxf(top, kNoMax);  // finite, and below any score to come, where this tile has no weight
         } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
           const bool move = top > m + 8.f;
           const float f = move ? ex2_approx(m - top) : 1.f;

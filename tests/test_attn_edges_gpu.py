@@ -106,3 +106,21 @@ def test_gradients_of_entries_and_heads_of_unlike_sizes(F, M, N, sizes, name, d,
                 R.check(f"dV of {b}, {h}", got[2][b, h, :lens[b]], outs[2], bounds[2])
             assert not got[1][b, h, lens[b]:].any() and not got[2][b, h, lens[b]:].any()
     assert not any(x[2].any() for x in got)
+
+
+# ------------------------------------------------------------ weights at their ends
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("M,N,front", [(40, 300, 128), (40, 300, 130), (300, 4200, 2000), (1, 300, 130)])
+def test_scores_of_minus_infinity_before_small_ones(F, name, M, N, front):
+    """Keys that no weight falls on, whole tiles of them, ahead of others whose
+    scores lie near -100: the same as without them."""
+    Q, K, V, _ = make(2, 2, 1, M, N, 64, name, seed=51)
+    Q[..., 0] = 1
+    Q[..., 1] = 4
+    K[..., 1] = -200
+    K[:, :, :front, 0] = float("-inf")
+    O, LSE = F.cross_attn_fwd(Q, K, V, scale=0.125)
+    ref, lse, bound, lse_bound = R.forward(Q, K[:, :, front:], V[:, :, front:], None, 0.125)
+    assert float(lse.max()) < -80
+    R.check("O", O, ref, bound)
+    R.check("LSE", LSE, lse, lse_bound)
