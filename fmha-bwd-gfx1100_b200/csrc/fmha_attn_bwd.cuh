@@ -770,23 +770,23 @@ static_assert(kNumBkBars * 8 + 8 <= 256, "barrier area");
 // 2^x of two values on the FMA pipe instead of the SFU, whose 16 results a
 // clock would bound the kernel: x = n + f with n the nearest integer (taken
 // from the low mantissa bits of x + 1.5 2^23) and 2^f on [-1/2, 1/2] by the
-// polynomial of degree 5 with the least largest relative error there (found by
-// Remez exchange): 7.5e-8, 2.4e-7 as evaluated in fp32, like ex2.approx. Below
-// 2^-126 the result stays there; NaN comes out as the largest float, which is
-// infinite in 16 bits.
+// polynomial 1 + f q(f) of degree 5 with the least largest relative error there
+// (found by Remez exchange): 9.1e-8, 1.1e-7 with the coefficients in fp32 and
+// 1.6e-7 as evaluated, like ex2.approx. 2^n is exact, with 0 for n = -127 and
+// infinity for 128, so x is held to [-127, 128], NaN staying what it is.
 __device__ __forceinline__ float2 ex2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n\tmin.NaN.f32 %0, %0, 0f43000000;" : "+f"(x.x));
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n\tmin.NaN.f32 %0, %0, 0f43000000;" : "+f"(x.y));
   auto both = [](float c) { return make_float2(c, c); };
   const float2 t = add_f32x2(x, both(12582912.f));
   const float2 f = fma_f32x2(add_f32x2(t, both(-12582912.f)), both(-1.f), x);
-  float2 p = fma_f32x2(both(1.3276472e-3f), f, both(9.675541e-3f));
-  p = fma_f32x2(p, f, both(5.550713e-2f));
-  p = fma_f32x2(p, f, both(0.24022120f));
-  p = fma_f32x2(p, f, both(0.69314694f));
-  p = fma_f32x2(p, f, both(1.0000001f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  float2 p = fma_f32x2(both(1.3264727e-3f), f, both(9.6715130e-3f));
+  p = fma_f32x2(p, f, both(5.5507336e-2f));
+  p = fma_f32x2(p, f, both(0.24022242f));
+  p = fma_f32x2(p, f, both(0.69314700f));
+  p = fma_f32x2(p, f, both(1.f));
+  return mul_f32x2(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                  __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
 }
 
 template <typename T, int D>

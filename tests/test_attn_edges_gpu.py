@@ -3,11 +3,13 @@ kind goes wrong without its ordinary cases showing it. References and bounds as
 in test_cross_gpu.py."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 import attn_reference as R
-from test_cross_gpu import DT, F, make, saved, tensor  # noqa: F401 (F is a fixture)
+from test_cross_gpu import DT, F, NAN, make, saved, tensor  # noqa: F401 (F is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +126,34 @@ def test_scores_of_minus_infinity_before_small_ones(F, name, M, N, front):
     assert float(lse.max()) < -80
     R.check("O", O, ref, bound)
     R.check("LSE", LSE, lse, lse_bound)
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+def test_weights_of_the_backward_over_their_whole_range(F, name):
+    """dV is the weight itself where one row counts, whose LSE the test chooses:
+    in every place of a tile, from weights that vanish to those that overflow
+    (of an LSE that is not the scores'), and NaN."""
+    powers = [-1e30, -200, -128, -127, -126, -125.5, -60.25, -24, -14.5, -3.7, -1, -0.5, -0.25, 0, 0.3, 0.5, 2.5, 5.5]
+    # in fp16 weights are held times 2^10: from 2^6 on they are infinite
+    powers += [6.5, 40, 126.75, 129, 140, 300, 1e30, NAN] if name == "bf16" else [140, 300, 1e30, NAN]
+    M, N, d = 16, 8, 64
+    B = M * len(powers)
+    Q = torch.zeros(B, 1, M, d, dtype=DT[name], device="cuda")
+    K = torch.zeros(B, 1, N, d, dtype=DT[name], device="cuda")
+    dO = torch.ones_like(Q)
+    LSE = torch.full((B, 1, M), float("inf"), device="cuda")
+    want = torch.empty(B, dtype=torch.float64, device="cuda")
+    for i, x in enumerate(powers):
+        for r in range(M):
+            LSE[i * M + r, 0, r] = -x * math.log(2)
+            want[i * M + r] = 2.0 ** x if x < 128 else (float("inf") if x == x else NAN)
+    dV = F.cross_attn_bwd(Q, K, torch.ones_like(K), torch.zeros_like(Q), LSE, dO)[2].double()
+    u, sub = R.roundings(DT[name])
+    # LSE is rounded, and multiplied by log2 e and rounded once more
+    arg = 4 * R.E * torch.tensor(powers, dtype=torch.float64, device="cuda").abs().nan_to_num(0).repeat_interleave(M)
+    bound = (2 * u + 2.0 ** -21 + arg.clamp(max=1)) * want + sub * 2.0 ** -10 + sub + 2.0 ** -126
+    for key in range(N):
+        for col in (0, 7, d - 1):
+            x = dV[:, 0, key, col]
+            assert torch.equal(x.isnan(), want.isnan())
+            R.check("weight", x[~want.isnan()], want[~want.isnan()], bound[~want.isnan()])
