@@ -40,6 +40,10 @@ inline int check_tensor(fmha_tensor_t& t, const char* name, int batch, int heads
       return set_error(kErrMisaligned, "%s: stride %lld is not a multiple of 8 elements", name,
                        static_cast<long long>(s));
   }
+  const double most = static_cast<double>(t.batch) * (batch - 1) + static_cast<double>(t.head) * (heads - 1) +
+                      static_cast<double>(t.row) * (rows - 1);
+  if (most > 140737488355328.0)  // 2^47 elements are all the addresses there are
+    return set_error(kErrInvalidArgument, "%s: strides reach past any memory", name);
   if (rows > 1 && t.row < D)
     return set_error(kErrInvalidArgument, "%s: rows overlap (row stride %lld, K_dim %d)", name,
                      static_cast<long long>(t.row), D);
@@ -60,6 +64,65 @@ inline int check_tensor(fmha_tensor_t& t, const char* name, int batch, int heads
     }
   }
   return kOk;
+}
+
+// The bytes of a strided tensor or an array: `run` consecutive ones at every
+// combination of steps along up to three axes, the longest steps first.
+struct Region {
+  uintptr_t at = 0;
+  int axes = 0;
+  int64_t n[3] = {1, 1, 1}, step[3] = {0, 0, 0};
+  int64_t span[4] = {0, 0, 0, 0};  // bytes from the first to behind the last, of axes i and on
+};
+inline Region region_of(const void* p, int64_t bytes) {
+  Region r;
+  r.at = reinterpret_cast<uintptr_t>(p);
+  r.span[0] = p ? bytes : 0;
+  return r;
+}
+inline Region region_of(const fmha_tensor_t& t, int batch, int heads, int rows, int D) {
+  Region r;
+  r.at = reinterpret_cast<uintptr_t>(t.ptr);
+  int64_t step[3] = {t.batch, t.head, t.row};
+  int n[3] = {batch, heads, rows};
+  for (int i = 0; i < 3; ++i) {
+    int best = -1;
+    for (int j = 0; j < 3; ++j)
+      if (n[j] > 1 && (best < 0 || step[j] > step[best])) best = j;
+    if (best < 0) break;
+    r.n[r.axes] = n[best];
+    r.step[r.axes++] = 2 * step[best];
+    n[best] = 1;
+  }
+  r.span[r.axes] = 2 * D;
+  for (int i = r.axes - 1; i >= 0; --i) r.span[i] = r.span[i + 1] + r.step[i] * (r.n[i] - 1);
+  return r;
+}
+
+// Whether two regions share a byte, `off` from a's first to b's first, of axes
+// ia and ib on. Along the longest step only the places are followed at which
+// what is left of the two can meet, of steps that both have their difference
+// alone, so that tensors interleaved in one buffer take a few calls. Those that
+// take more than `budget` count as meeting.
+inline bool regions_meet(const Region& a, int ia, const Region& b, int ib, int64_t off, int& budget) {
+  if (off >= a.span[ia] || -off >= b.span[ib]) return false;
+  if (ia == a.axes && ib == b.axes) return true;
+  if (--budget < 0) return true;
+  const int64_t sa = ia < a.axes ? a.step[ia] : 0, sb = ib < b.axes ? b.step[ib] : 0, s = std::max(sa, sb);
+  const int na = sa == s ? ia + 1 : ia, nb = sb == s ? ib + 1 : ib;
+  // off + k s for the k with -b.span < off + k s < a.span
+  const int64_t least = sa == s ? 1 - a.n[ia] : 0, most = sb == s ? b.n[ib] - 1 : 0;
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0 ? 1 : 0); };
+  const int64_t lo = std::max(least, floor_div(-b.span[nb] - off, s) + 1);
+  const int64_t hi = std::min(most, floor_div(a.span[na] - off - 1, s));
+  for (int64_t k = lo; k <= hi; ++k)
+    if (regions_meet(a, na, b, nb, off + k * s, budget)) return true;
+  return false;
+}
+inline bool regions_meet(const Region& a, const Region& b) {
+  if (a.span[0] == 0 || b.span[0] == 0) return false;
+  int budget = 1 << 17;
+  return regions_meet(a, 0, b, 0, static_cast<int64_t>(b.at - a.at), budget);
 }
 
 enum class AttnOp : int { kCrossFwd = FMHA_ATTN_CROSS_FWD, kCrossBwd = FMHA_ATTN_CROSS_BWD, kPrefix = FMHA_ATTN_PREFIX };
@@ -93,6 +156,38 @@ inline int check_attn_sizes(const fmha_attn_t& a, AttnOp op) {
   return kOk;
 }
 
+// What a call reads and writes, its workspace apart.
+struct AttnRegions {
+  Region in[9], out[3];
+  int read = 0, written = 0;
+  AttnRegions(const fmha_attn_t& a, AttnOp op) {
+    auto q = [&](const fmha_tensor_t& t) { return region_of(t, a.batch, a.q_heads, a.M, a.K_dim); };
+    auto k = [&](const fmha_tensor_t& t) { return region_of(t, a.batch, a.kv_heads, a.N, a.K_dim); };
+    auto kp = [&](const fmha_tensor_t& t) { return region_of(t, a.prefixes, a.kv_heads, a.N_prefix, a.K_dim); };
+    const Region lse = region_of(a.LSE, static_cast<int64_t>(a.batch) * a.q_heads * a.M * 4);
+    in[read++] = q(a.Q);
+    in[read++] = k(a.K);
+    in[read++] = k(a.V);
+    in[read++] = region_of(a.kv_lens, static_cast<int64_t>(a.batch) * 4);
+    if (op == AttnOp::kCrossBwd) {
+      in[read++] = q(a.O);
+      in[read++] = q(a.dO);
+      in[read++] = lse;
+      out[written++] = q(a.dQ);
+      out[written++] = k(a.dK);
+      out[written++] = k(a.dV);
+    } else {
+      out[written++] = q(a.O);
+      out[written++] = lse;
+    }
+    if (op == AttnOp::kPrefix) {
+      in[read++] = kp(a.Kp);
+      in[read++] = kp(a.Vp);
+      in[read++] = region_of(a.prefix_lens, static_cast<int64_t>(a.prefixes) * 4);
+    }
+  }
+};
+
 // All arguments; strides of single-row axes are normalised in `a`.
 inline int check_attn(fmha_attn_t& a, AttnOp op) {
   int rc = check_attn_sizes(a, op);
@@ -112,21 +207,19 @@ inline int check_attn(fmha_attn_t& a, AttnOp op) {
     if ((reinterpret_cast<uintptr_t>(a.prefix_lens) & 3u) != 0)
       return set_error(kErrMisaligned, "prefix_lens must be 4-byte aligned");
   }
-  const void* read[] = {a.Q.ptr, a.K.ptr, a.V.ptr, bwd ? a.O.ptr : nullptr, bwd ? a.dO.ptr : nullptr,
-                        op == AttnOp::kPrefix ? a.Kp.ptr : nullptr, op == AttnOp::kPrefix ? a.Vp.ptr : nullptr};
-  const void* written[] = {bwd ? a.dQ.ptr : a.O.ptr, bwd ? a.dK.ptr : a.LSE, bwd ? a.dV.ptr : nullptr};
-  for (const void* const& w : written) {
-    for (const void* r : read)
-      if (r && r == w) return set_error(kErrInvalidArgument, "an output lies over an input");
-    for (const void* const& v : written)
-      if (&v != &w && v && v == w) return set_error(kErrInvalidArgument, "an output lies over another");
-  }
   if (!a.LSE) return set_error(kErrInvalidArgument, "null LSE argument");
   if ((reinterpret_cast<uintptr_t>(a.LSE) & 3u) != 0) return set_error(kErrMisaligned, "LSE must be 4-byte aligned");
   if ((reinterpret_cast<uintptr_t>(a.kv_lens) & 3u) != 0)
     return set_error(kErrMisaligned, "kv_lens must be 4-byte aligned");
   if (!(a.softmax_scale > 0.f) || !(a.softmax_scale < 3.0e38f))
     return set_error(kErrInvalidArgument, "softmax_scale must be positive and finite");
+  AttnRegions all(a, op);
+  for (int w = 0; w < all.written; ++w) {
+    for (int r = 0; r < all.read; ++r)
+      if (regions_meet(all.out[w], all.in[r])) return set_error(kErrInvalidArgument, "an output lies over an input");
+    for (int v = 0; v < w; ++v)
+      if (regions_meet(all.out[w], all.out[v])) return set_error(kErrInvalidArgument, "an output lies over another");
+  }
   return kOk;
 }
 

@@ -501,6 +501,13 @@ int run_attn(const fmha_attn_t* args, AttnOp op, cudaStream_t stream) {
                      static_cast<unsigned long long>(a.workspace ? a.workspace_bytes : 0),
                      static_cast<unsigned long long>(need));
   if (need > 0 && !aligned16(a.workspace)) return set_error(kErrMisaligned, "workspace must be 16-byte aligned");
+  if (need > 0) {
+    const AttnRegions all(a, op);
+    const Region ws = region_of(a.workspace, static_cast<int64_t>(need));
+    for (int i = 0; i < all.read + all.written; ++i)
+      if (regions_meet(ws, i < all.read ? all.in[i] : all.out[i - all.read]))
+        return set_error(kErrInvalidArgument, "the workspace lies over a tensor");
+  }
   int device = 0, sms = 0;
   if ((rc = attn_device(device, sms)) != kOk) return rc;
   if (op == AttnOp::kCrossFwd ? is_decode(a) : op == AttnOp::kPrefix && prefix_together(a)) {

@@ -63,7 +63,11 @@ typedef struct {
  * q_heads is a multiple of kv_heads; query head h reads kv head
  * h / (q_heads / kv_heads). Lengths live on the device and are clamped to
  * [0, rows]; a null length array means that every row counts. What K and V
- * hold at or past a length is never used, NaN and infinities included. */
+ * hold at or past a length is never used, NaN and infinities included.
+ *
+ * No byte of an output or of the workspace may be one of an input (LSE and the
+ * lengths among them), of another output or of the same output twice: such a
+ * call is refused. Tensors may interleave, as slices of one buffer do. */
 typedef struct {
   fmha_tensor_t Q, O;           /* [batch][q_heads][M][K_dim] */
   fmha_tensor_t K, V;           /* [batch][kv_heads][N][K_dim] */
