@@ -259,6 +259,24 @@ __device__ __forceinline__ void add_weighted(float4& acc, float w, const float4&
   acc.w = fmaf(w, v.w, acc.w);
 }
 
+// The infinities and NaN that 4 columns of `count` rows of V hold (every weight
+// is above 0), into a row's sums: see hide_odd.
+template <typename T>
+__device__ __forceinline__ void add_odd4(const T* v, int64_t stride, int count, float4& acc) {
+#pragma unroll 1
+  for (int k = 0; k < count; ++k) {
+    const uint2 all = *reinterpret_cast<const uint2*>(v + k * stride);
+    uint2 rest = all;
+    drop_odd<T>(rest.x);
+    drop_odd<T>(rest.y);
+    const float2 a = Elem<T>::unpack(all.x ^ rest.x), b = Elem<T>::unpack(all.y ^ rest.y);
+    acc.x += a.x;
+    acc.y += a.y;
+    acc.z += b.x;
+    acc.w += b.y;
+  }
+}
+
 // 4 columns of O (and, with the first, LSE) of packed row q of a kv head, from
 // their sum at the reference m. A sum of 0 has no key behind it; NaN stays.
 template <typename T>
@@ -291,7 +309,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
   if (p.part_o) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ __align__(16) float sum_o[W][kRows][D];
   __shared__ float warp_m[W][kRows], warp_l[W][kRows], block_m[kRows], block_l[kRows];
-  __shared__ float weight[kMostSplits][kRows], total[kRows], top_of[kRows];
+  __shared__ float weight[kMostSplits][kRows], total[kRows], top_of[kRows], block_odd;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % p.splits;
@@ -344,6 +362,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
     for (int x = 0; x < 2; ++x)
       limit[r][x] = p.causal ? n - (p.M - 1 - (row0 + 8 * r + 2 * t + x) % p.M) : n;
   const float sl2 = p.scale * kLog2e;
+  // own keys that every token reads; what infinities and NaN V holds behind them
+  // is left out, and added to the tokens that do read it at the end
+  const int shown = p.causal ? max(0, n - (p.M - 1)) : n;
+  int odd = 0;
   for (; i < hi; i += W) {
     float s[R][4];
     uint32_t pt[R][2];
@@ -357,6 +379,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
 #pragma unroll
       for (int r = 0; r < R; ++r) all[r][0] = all[r][1] = np;
       w.weights(s, pt, 16 * i, all, sl2);
+    }
+    if (shown < n && 16 * (i - ahead) + 16 > shown) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          if (16 * (i - ahead) + 2 * t + (x & 1) + 8 * (x >> 1) >= shown && drop_odd<T>(vf[x][c])) odd = 1;
     }
     w.values(pt, [&](int x, int c) { return vf[x][c]; });
     if (more) load_v(i + W);
@@ -372,7 +401,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
         warp_m[warp][8 * r + 2 * t + x] = w.m[r][x];
         warp_l[warp][8 * r + 2 * t + x] = w.l[r][x];
       }
-  __syncthreads();
+  odd = __syncthreads_or(odd);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -408,11 +437,12 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
   if (p.splits > 1) {
     for (int e = threadIdx.x; e < real * (D / 4); e += kThreads)
       *reinterpret_cast<float4*>(&sum_o[0][e / (D / 4)][4 * (e % (D / 4))]) = sum4(e / (D / 4), e % (D / 4));
+    if (threadIdx.x == 0) block_odd = odd ? 1.f : 0.f;
     cluster_sync();
     // the blocks' references and sums, each read by a thread of its own
     for (int e = threadIdx.x; e < p.splits * kRows; e += kThreads)
       weight[e / kRows][e % kRows] = load_cluster(&block_m[e % kRows], e / kRows);
-    __syncthreads();
+    odd = __syncthreads_or(shown < n && threadIdx.x < p.splits && load_cluster(&block_odd, threadIdx.x) != 0.f);
     if (threadIdx.x < kRows) {
       float top = kNoMax;
       for (int y = 0; y < p.splits; ++y) top = fmaxf(top, weight[y][threadIdx.x]);
@@ -439,6 +469,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
 #pragma unroll 4
       for (int y = 0; y < p.splits; ++y) add_weighted(acc, weight[y][row], load_cluster4(&sum_o[0][row][4 * c], y));
     }
+    if (odd) add_odd4(p.V.at(b, hk, shown) + 4 * c, p.V.sr, n - (p.M - 1) + q % p.M - shown, acc);
     decode_output(p, b, hk, q, c, p.splits == 1 ? block_m[row] : top_of[row], p.splits == 1 ? block_l[row] : total[row],
                   acc);
   }

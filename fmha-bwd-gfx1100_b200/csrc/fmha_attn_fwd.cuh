@@ -94,6 +94,12 @@ struct RowPack {
     div_mod(t, nm, u, im);
     div_mod(u, ng, is, ig);
   }
+  // the oldest token of tile t
+  __device__ __forceinline__ int oldest(int t) const {
+    int im, ig, is;
+    box(t, im, ig, is);
+    return im * Mt;
+  }
   // token, head within the group and entry of row r of tile t; false if there is no such row
   __device__ __forceinline__ bool row(int t, int r, int& m, int& g, int& s) const {
     int im, ig, is, rm = r, rg = 0, rs = 0;
@@ -135,6 +141,7 @@ struct FwdParams {
   int splits;         // parts of the keys (1: O and LSE are final)
   int pairs;          // tile pairs of one (batch, kv head)
   int items;          // B * Hkv * splits * pairs
+  View<T> V;          // kOwn: the tensor of tm_V
   View<T> O;
   float* LSE;         // [batch][q head][token]
   float* part_o;      // splits > 1 or partial: [split][row][D], normalised
@@ -172,7 +179,7 @@ enum FwdBar : int {
   kFwQEmpty0 = 2,   // + tile: the item's last S of the tile is done
   kFwKVFull0 = 4,   // + slot (up to 8)
   kFwKVEmpty0 = 12, // + slot
-  kFwTail0 = 20,    // + slot: a last V tile has landed, its rows behind the keys not yet cleared
+  kFwTail0 = 20,    // + slot: a V tile has landed that is_checked, and not yet cleared
   kFwSFull0 = 28,   // + tile
   kFwPFull0 = 30,   // + tile: the first 96 columns of p written (4 warps)
   kFwPRest0 = 32,   // + tile: and the others
@@ -183,46 +190,64 @@ enum FwdBar : int {
   kFwUnitFull0 = 42,
   kFwUnitEmpty0 = 46,
   kFwDrain = 50,
-  kNumFwdBars = 51,
+  kFwChecked = 51,  // kOwn: an item's V tiles have gone through hide_odd
+  kFwSeen = 52,     // and the other epilogue warps know what it found (3 warps)
+  kNumFwdBars = 53,
 };
-static_assert(kNumFwdBars * 8 + 8 <= 512, "barrier area");
+static_assert(kNumFwdBars * 8 + 12 <= 512, "barrier area");
 
 // One item: a pair of row tiles of a (batch, kv head), a range of key tiles.
 struct FwdItem {
   int b, hk, split, tile0, n;  // n: valid keys of the batch entry
   int lo, hi;                  // key tiles
   bool two;                    // the second tile exists
+  int first;                   // kOwn: the first key tile that not all rows see whole
 };
 
 __device__ __forceinline__ FwdItem fwd_item(const int4& a, const int4& b) {
-  return FwdItem{a.x, a.y, a.z, a.w, b.z, b.x, b.y, b.w == 2};
+  return FwdItem{a.x, a.y, a.z, a.w, b.z, b.x, b.y, (b.w & 3) == 2, b.w >> 2};
 }
 
 // The items of this CTA. kv heads lie innermost: with the usual [token][head]
-// layouts of Q and O, the CTAs then read and write neighbouring memory.
-template <typename T>
+// layouts of Q and O, the CTAs then read and write neighbouring memory. kOwn: key
+// tiles behind an item's newest token are left out, whatever they hold.
+template <typename T, bool kOwn>
 __device__ __forceinline__ void fwd_unit(const FwdParams<T>& p, int t, int4& a, int4& b) {
   int hk, pair, split, e;
   div_mod(t, p.Hkv, t, hk);
   div_mod(t, p.pairs, t, pair);
   div_mod(t, p.splits, e, split);
-  const int n = valid_rows(p.lens, e, p.N), nt = (n + kTile - 1) / kTile;
+  const bool two = 2 * pair + 1 < p.rows.tiles;
+  const int n = valid_rows(p.lens, e, p.N);
+  int nt = (n + kTile - 1) / kTile, first = 0;
+  if constexpr (kOwn) {
+    int oldest = p.rows.oldest(2 * pair), newest = oldest;  // of both tiles, by their first rows
+    if (two) {
+      const int t = p.rows.oldest(2 * pair + 1);
+      oldest = min(oldest, t);
+      newest = max(newest, t);
+    }
+    newest = min(newest + p.rows.Mt, p.rows.M) - 1;
+    const int all = n - (p.rows.M - 1);  // token m sees m more
+    first = p.rows.M > 1 ? max(0, all + oldest) / kTile : nt;
+    nt = (max(0, all + newest) + kTile - 1) / kTile;
+  }
   int lo, hi, rest;
   // up to 2^23 tiles times 2 * 148 parts: 32 bits without a sign
   div_mod(static_cast<int>(static_cast<uint32_t>(nt) * split), p.splits, lo, rest);
   div_mod(static_cast<int>(static_cast<uint32_t>(nt) * (split + 1)), p.splits, hi, rest);
   a = make_int4(e, hk, split, 2 * pair);
-  b = make_int4(lo, hi, n, 2 * pair + 1 < p.rows.tiles ? 2 : 1);
+  b = make_int4(lo, hi, n, first << 2 | (two ? 2 : 1));
 }
 // a, b: the first of them.
-template <typename T>
+template <typename T, bool kOwn>
 __device__ void feed_fwd(const FwdParams<T>& p, int4 a, int4 b, UnitRing* ring, uint64_t* full, uint64_t* empty,
                          const WaitCtx& ctx) {
   int k = 0;
   for (int t = blockIdx.x; t < p.items; ++k) {
     if (!put_unit(ring, full, empty, k, a, b, ctx, 205)) return;
     t += gridDim.x;
-    if (t < p.items) fwd_unit(p, t, a, b);
+    if (t < p.items) fwd_unit<T, kOwn>(p, t, a, b);
   }
   put_unit(ring, full, empty, k, make_int4(0, 0, 0, 0), make_int4(0, 0, 0, 0), ctx, 205);
 }
@@ -241,6 +266,65 @@ __device__ __forceinline__ void clear_tail(uint8_t* tile, int left, int lane) {
   fence_proxy_async_smem();
 }
 __device__ __forceinline__ bool has_tail(int n, int hi) { return hi * kTile > n && (n & 15) != 0; }
+
+// kOwn: of the keys that some rows of an item see and others do not, an infinity
+// or NaN in V would reach the latter as 0 times it. The landed V tiles that hold
+// such keys are cleared of them (hide_odd) before their products, and the rows
+// that do see them get them where they are stored (add_odd).
+//
+// Whether the epilogue looks at V tile j of an item before its products.
+template <bool kOwn>
+__device__ __forceinline__ bool is_checked(const FwdItem& it, int j) {
+  return (j + 1 == it.hi && has_tail(it.n, it.hi)) || (kOwn && j >= it.first);
+}
+// Zeroes the elements of a word or four whose exponent is all ones.
+template <typename T>
+__device__ __forceinline__ bool drop_odd(uint32_t& w) {
+  constexpr uint32_t kOnes = Elem<T>::kBF16 ? 0x7f807f80u : 0x7c007c00u;
+  const uint32_t odd = __vcmpeq2(w & kOnes, kOnes);
+  w &= ~odd;
+  return odd != 0;
+}
+template <typename T>
+__device__ __forceinline__ bool drop_odd(uint4& v) {
+  bool odd = drop_odd<T>(v.x);
+  odd |= drop_odd<T>(v.y);
+  odd |= drop_odd<T>(v.z);
+  odd |= drop_odd<T>(v.w);
+  return odd;
+}
+// Rows [from, to) of a landed 128-row tile, by a warp; whether this lane found any.
+template <typename T, int D>
+__device__ __forceinline__ bool hide_odd(uint8_t* tile, int from, int to, int lane) {
+  bool found = false;
+#pragma unroll 1
+  for (int i = lane; i < (to - from) * (D / 8); i += 32) {
+    const int row = from + i / (D / 8), c = i % (D / 8);
+    uint4* at = reinterpret_cast<uint4*>(tile + (c >> 3) * kBoxBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+    uint4 v = *at;
+    if (!drop_odd<T>(v)) continue;
+    *at = v;
+    found = true;
+  }
+  if (found) fence_proxy_async_smem();
+  return found;
+}
+// Adds the infinities and NaN of `count` rows of V (every weight is above 0) to a
+// row of D finished sums; those that hide_odd left in place add nothing new.
+template <typename T, int D>
+__device__ __forceinline__ void add_odd(const T* v, int64_t stride, int count, float* out) {
+  constexpr uint32_t kOnes = Elem<T>::kBF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll 1
+  for (int c = 0; c < D; ++c) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < count; ++k) {
+      const uint32_t x = reinterpret_cast<const uint16_t*>(v + k * stride)[c];
+      if ((x & kOnes) == kOnes) sum += Elem<T>::unpack(x).x;
+    }
+    if (sum != 0.f) out[c] += sum;
+  }
+}
 
 // 8 fp32 accumulators times `mul` as eight 16-bit values.
 template <typename T>
@@ -291,9 +375,10 @@ __device__ __forceinline__ void store_sums(uint32_t taddr, bool fp32, uint8_t* r
 
 // O and LSE of row `tok` of head g and entry s of an item's tile, from the
 // sums in TMEM at taddr, their total l and its reference m; or a part of them.
-template <typename T, int D>
+// `odd`: hide_odd has found something, in this item or another.
+template <typename T, int D, bool kOwn>
 __device__ __forceinline__ void store_tile(const FwdParams<T>& p, const FwdItem& it, uint32_t taddr, int tok, int g, int s,
-                                           bool real, float m, float l) {
+                                           bool real, float m, float l, int odd) {
   const bool keys = it.lo < it.hi;
   const int64_t all_rows = static_cast<int64_t>(p.B) * p.rows.S * p.Hkv * p.rows.G * p.rows.M;
   const int b = it.b * p.rows.S + s, h = it.hk * p.rows.G + g;
@@ -308,6 +393,10 @@ __device__ __forceinline__ void store_tile(const FwdParams<T>& p, const FwdItem&
   if (!real) out = nullptr;
   if (keys) {
     store_sums<T, D, 32>(taddr, p.partial, out, inv);
+    if (kOwn && odd && out) {  // behind a prefix sums are always parts
+      const int all = it.n - (p.rows.M - 1), from = max(max(0, all), it.lo * kTile), to = min(all + tok, it.hi * kTile);
+      add_odd<T, D>(p.V.at(it.b, it.hk, from), p.V.sr, to - from, reinterpret_cast<float*>(out));
+    }
   } else if (out) {  // zeros
     const int chunks = D / (p.partial ? 4 : 8);
     for (int x = 0; x < chunks; ++x) reinterpret_cast<uint4*>(out)[x] = make_uint4(0, 0, 0, 0);
@@ -354,9 +443,9 @@ __device__ __forceinline__ void weights_32(const uint32_t* s, float2 sc, float2 
 // tile's softmax waits for the products between its p and its next S. Few steps
 // are bound by latency: 3 to 4 us pass before the first S.
 //
-// kOwn: the keys of an entry's own tokens, behind a prefix: token m reads n - (M
-// - 1 - m) of them. It starts before the launch before it has ended, and waits
-// for that at its end.
+// kOwn: the keys of an entry's own tokens, behind a prefix: token m reads all but
+// the M - 1 - m newest of them. It starts before the launch before it has ended,
+// and waits for that at its end.
 template <typename T, int D, bool kOwn>
 __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_Q, const __grid_constant__ CUtensorMap tm_K,
@@ -376,6 +465,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + kNumFwdBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* odd_flag = abort_flag + 1;  // kOwn: hide_odd has found something in some item
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   int4 ua, ub;
@@ -384,8 +474,12 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     int count = 1;
     if ((i >= kFwPFull0 && i < kFwOFull0) || (i >= kFwOEmpty0 && i < kFwUnitFull0)) count = 4;
     if (i >= kFwUnitEmpty0 && i < kFwDrain) count = Cfg::kReaders;
+    if (i == kFwSeen) count = 3;
     mbar_init(&bar[i], count);
-    if (i == 0) *abort_flag = 0;
+    if (i == 0) {
+      *abort_flag = 0;
+      *odd_flag = 0;
+    }
     fence_mbar_init();
   }
   if (warp == 12 && elect_one()) {
@@ -398,7 +492,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (warp == 14) fwd_unit(p, blockIdx.x, ua, ub);
+  if (warp == 14) fwd_unit<T, kOwn>(p, blockIdx.x, ua, ub);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -452,7 +546,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
           if (it.lo == it.hi) continue;
           ok = load_q(it, 0, nq0) && load_kv(&tm_K, it, it.lo, kFwKVFull0) && (!it.two || load_q(it, 1, nq1));
           for (int j = it.lo; j < it.hi && ok; ++j)
-            ok = load_kv(&tm_V, it, j, j + 1 == it.hi && has_tail(it.n, it.hi) ? kFwTail0 : kFwKVFull0) &&
+            ok = load_kv(&tm_V, it, j, is_checked<kOwn>(it, j) ? kFwTail0 : kFwKVFull0) &&
                  (j + 1 == it.hi || load_kv(&tm_K, it, j + 1, kFwKVFull0));
         }
         if (*abort_flag) {
@@ -468,7 +562,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
       }
       __syncwarp();
     } else if (warp == 14) {
-      if (lane == 0) feed_fwd(p, ua, ub, ring, unit_full, unit_empty, ctx);
+      if (lane == 0) feed_fwd<T, kOwn>(p, ua, ub, ring, unit_full, unit_empty, ctx);
       __syncwarp();
     } else if (warp == 13) {
       // ---- MMA. Per step, for each tile in turn: O += p V_j, then S of the
@@ -651,13 +745,14 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
       if (p.in_turn) {
         if (it.lo < it.hi) {
           if (!mbar_wait(&bar[kFwOFull0 + t], no & 1, ctx, 233)) { ok = false; continue; }
+          if (kOwn && !mbar_wait(&bar[kFwChecked], no & 1, ctx, 234)) { ok = false; continue; }
           ++no;
         }
         __syncwarp();
         tc_fence_after();
         int tok, g, s;
         const bool real = p.rows.row(it.tile0 + t, r, tok, g, s);
-        store_tile<T, D>(p, it, tO, tok, g, s, real, m, (l0.x + l0.y) + (l1.x + l1.y));
+        store_tile<T, D, kOwn>(p, it, tO, tok, g, s, real, m, (l0.x + l0.y) + (l1.x + l1.y), *odd_flag);
         tc_fence_before();
         __syncwarp();
         if (it.lo < it.hi && lane == 0) mbar_arrive(&bar[kFwOEmpty0 + t]);
@@ -670,26 +765,38 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
       if (lane == 0) mbar_arrive(&bar[kFwStFull0 + t]);
     }
   } else {
-    // ---- epilogue: thread = row of each tile in turn. It also clears the
-    // last V tile behind the last key, for the issuers that wait for it.
+    // ---- epilogue: thread = row of each tile in turn. One warp also clears the
+    // V tiles that are checked, for the issuer that waits for them.
     regs_lower<Cfg::kOtherRegs>();
     const int r = threadIdx.x & 127;
-    int nst0 = 0, nst1 = 0, no0 = 0, no1 = 0, g = 0;
+    int nst0 = 0, nst1 = 0, no0 = 0, no1 = 0, g = 0, ni = 0, odd = 0;
     uint32_t tail_turns = 0;  // a bit for each slot
     while (get_unit<true>(ring, unit_full, unit_empty, k, ua, ub, ctx, 240, ok)) {
       const FwdItem it = fwd_item(ua, ub);
       const bool keys = it.lo < it.hi;
       if (keys) {
-        g += 2 * (it.hi - it.lo);
-        if (warp == 8 && has_tail(it.n, it.hi)) {
-          const int slot = (g - 1) % kSlots;
-          if (!mbar_wait(&bar[kFwTail0 + slot], tail_turns >> slot & 1, ctx, 241)) ok = false;
-          tail_turns ^= 1u << slot;
+        if (warp == 8) {
+#pragma unroll 1
+          for (int j = kOwn ? min(max(it.lo, it.first), it.hi - 1) : it.hi - 1; j < it.hi; ++j) {
+            if (!is_checked<kOwn>(it, j)) continue;
+            const int slot = (g + 2 * (j - it.lo) + 1) % kSlots;
+            if (ok && !mbar_wait(&bar[kFwTail0 + slot], tail_turns >> slot & 1, ctx, 241)) ok = false;
+            tail_turns ^= 1u << slot;
+            __syncwarp();
+            uint8_t* tile = smem + Cfg::kOffKV + slot * Cfg::kTileBytes;
+            if (kOwn && ok && j >= it.first &&
+                hide_odd<T, D>(tile, max(0, it.n - (p.rows.M - 1) - j * kTile), min(kTile, it.n - j * kTile), lane))
+              *odd_flag = 1;
+            if (ok && j + 1 == it.hi && has_tail(it.n, it.hi)) clear_tail<D>(tile, it.n - j * kTile, lane);
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&bar[kFwKVFull0 + slot]);
+          }
+          // no further than one item ahead of the others
+          if (kOwn && ok && ni > 0 && !mbar_wait(&bar[kFwSeen], (ni - 1) & 1, ctx, 245)) ok = false;
           __syncwarp();
-          if (ok) clear_tail<D>(smem + Cfg::kOffKV + slot * Cfg::kTileBytes, it.n - (it.hi - 1) * kTile, lane);
-          __syncwarp();
-          if (ok && lane == 0) mbar_arrive(&bar[kFwKVFull0 + slot]);
+          if (kOwn && ok && lane == 0) mbar_arrive(&bar[kFwChecked]);
         }
+        g += 2 * (it.hi - it.lo);
       }
 #pragma unroll 1
       for (int t = 0; t < 2; ++t) {
@@ -703,6 +810,12 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         if (lane == 0) mbar_arrive(&bar[kFwStEmpty0 + t]);
         if (keys) {
           if (!mbar_wait(&bar[kFwOFull0 + t], (t == 0 ? no0 : no1) & 1, ctx, 243)) { ok = false; break; }
+          if (kOwn && t == 0) {
+            if (!mbar_wait(&bar[kFwChecked], ni & 1, ctx, 244)) { ok = false; break; }
+            odd = *odd_flag;
+            __syncwarp();
+            if (warp != 8 && lane == 0) mbar_arrive(&bar[kFwSeen]);
+          }
           if (t == 0) ++no0;
           else ++no1;
         }
@@ -710,11 +823,13 @@ __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 1)
         tc_fence_after();
         int m, g, s;
         const bool real = p.rows.row(it.tile0 + t, r, m, g, s);
-        store_tile<T, D>(p, it, tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16), m, g, s, real, ml.x, ml.y);
+        store_tile<T, D, kOwn>(p, it, tmem + Cfg::kColO + D * t + (static_cast<uint32_t>(r & 96) << 16), m, g, s, real,
+                               ml.x, ml.y, odd);
         tc_fence_before();
         __syncwarp();
         if (keys && lane == 0) mbar_arrive(&bar[kFwOEmpty0 + t]);
       }
+      if (keys) ++ni;
     }
   }
 

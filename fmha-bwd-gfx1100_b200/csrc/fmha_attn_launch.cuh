@@ -140,6 +140,7 @@ int enqueue_fwd(const fmha_attn_t& a, const FwdPlan& f, const fmha_tensor_t& K, 
   p.splits = f.splits;
   p.pairs = f.pairs;
   p.items = f.items;
+  p.V = view_of<T>(V);
   p.O = view_of<T>(a.O);
   p.LSE = a.LSE;
   p.partial = part_o != nullptr;

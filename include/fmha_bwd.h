@@ -192,8 +192,9 @@ int fmha_cross_bwd(const fmha_attn_t* args, fmha_stream_t stream);
  * batch / prefixes consecutive entries share (entry b reads prefix
  * b / (batch / prefixes), its first prefix_lens rows) and to the entry's own
  * cache K, V behind it (its first kv_lens[b] rows, the M newest tokens
- * last: row m reads kv_lens[b] - (M - 1 - m) of them), in one softmax. O and
- * LSE as fmha_cross_fwd. The prefix is read once for all entries. */
+ * last: row m reads kv_lens[b] - (M - 1 - m) of them, and nothing of the
+ * others reaches it, NaN and infinities included), in one softmax. O and LSE
+ * as fmha_cross_fwd. The prefix is read once for all entries. */
 int fmha_prefix_attn(const fmha_attn_t* args, fmha_stream_t stream);
 
 /* Stage hooks (replace the reference's test_* wrappers,

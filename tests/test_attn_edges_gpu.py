@@ -157,3 +157,53 @@ def test_weights_of_the_backward_over_their_whole_range(F, name):
             x = dV[:, 0, key, col]
             assert torch.equal(x.isnan(), want.isnan())
             R.check("weight", x[~want.isnan()], want[~want.isnan()], bound[~want.isnan()])
+
+
+# ------------------------------------------------- what a newer token's row holds
+MASKED = [
+    # P, S, Hq, Hkv, M, N, Np, d, dtype, kv_lens
+    (1, 2, 4, 4, 2, 40, 100, 64, "fp16", [40, 7]),
+    (2, 1, 8, 2, 3, 300, 70, 128, "bf16", [300, 18]),
+    (1, 3, 2, 1, 5, 33, 129, 64, "bf16", [33, 17, 5]),
+    (1, 1, 1, 1, 16, 4000, 30000, 128, "fp16", [3999]),       # few rows, split among blocks
+    (1, 2, 4, 1, 4, 200, 30000, 64, "bf16", [200, 131]),      # few rows, parts and a join
+    (2, 2, 6, 2, 7, 150, 90, 64, "fp16", [150, 130, 7, 129]),  # 21 rows a kv head
+    (1, 2, 2, 2, 130, 400, 64, 128, "bf16", [400, 131]),
+    (1, 1, 3, 1, 300, 700, 200, 64, "fp16", [700]),
+    (1, 4, 8, 8, 257, 1300, 100, 128, "fp16", [1300, 257, 258, 1281]),
+    (2, 40, 32, 4, 3, 300, 200, 128, "bf16", [3 + (61 * b) % 298 for b in range(80)]),  # several items to a block
+    (2, 40, 32, 4, 3, 300, 200, 64, "fp16", [300] * 80),
+]
+
+
+@pytest.mark.parametrize("what", ["V", "K"])
+@pytest.mark.parametrize("P,S,Hq,Hkv,M,N,Np,d,name,lens", MASKED)
+def test_a_newer_token_does_not_reach_older_ones(F, what, P, S, Hq, Hkv, M, N, Np, d, name, lens):
+    """NaN and infinities in the row of one of the newest tokens: the tokens
+    before it do not see them, it and those behind it do, in their columns."""
+    B = P * S
+    Q, K, V, n = make(B, Hq, Hkv, M, N, d, name, lens, seed=61)
+    _, Kp, Vp, _ = make(P, Hkv, Hkv, 1, Np, d, name, None, seed=62)
+    for tok in sorted({1, M // 2, M - 1} - {0}):
+        k, v, clean = K.clone(), V.clone(), V.clone()
+        for b in range(B):
+            key = lens[b] - M + tok
+            if what == "K":
+                k[b, :, key] = NAN
+            else:
+                v[b, :, key, 3], v[b, :, key, d - 1], v[b, :, key, d // 2] = NAN, float("inf"), float("-inf")
+                clean[b, :, key, [3, d - 1, d // 2]] = 0
+        got, lse = F.prefix_attn(Q, Kp, Vp, k, v, None, n)
+        ref, want_lse, bound, lse_bound = R.prefix(Q, Kp, Vp, K, clean if what == "V" else V, None, n, d ** -0.5)
+        if what == "K":
+            R.check("O", got[:, :, :tok], ref[:, :, :tok], bound[:, :, :tok])
+            R.check("LSE", lse[:, :, :tok], want_lse[:, :, :tok], lse_bound[:, :, :tok])
+            assert got[:, :, tok:].isnan().all() and lse[:, :, tok:].isnan().all()
+            continue
+        R.check("LSE", lse, want_lse, lse_bound)
+        assert got[:, :, tok:, 3].isnan().all()
+        assert (got[:, :, tok:, d - 1] == float("inf")).all() and (got[:, :, tok:, d // 2] == float("-inf")).all()
+        got = got.clone()
+        for c in (3, d - 1, d // 2):
+            got[:, :, tok:, c] = ref[:, :, tok:, c].to(got.dtype)
+        R.check("O", got, ref, bound)
