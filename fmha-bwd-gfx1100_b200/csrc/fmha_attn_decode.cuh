@@ -22,7 +22,7 @@
 // same bias in fp16).
 //
 // Two kernels share this:
-//   * attn_decode_kernel: a block to a tile of rows of a kv head; with few of
+//   * attn_decode_kernel: a block to a kv head's rows (16 at most); with few of
 //     those, a cluster of blocks splits the keys and meets in each other's
 //     shared memory. One launch, no workspace; pieces go straight to registers,
 //     one tile ahead. Behind a shared prefix it takes the prefix's keys along
@@ -30,12 +30,12 @@
 //     attn_join_kernel.
 //   * attn_decode_stream_kernel, for long caches: every block takes an equal run
 //     of the keys of the whole batch, counted on the device from the lengths,
-//     its warps side by side in neighbouring heads (and tiles): those lie
-//     together in a [token][head] cache, whose 128-byte rows otherwise come one
-//     to a DRAM page (4.3 instead of 6.1 TB/s). Each warp keeps a ring of
-//     16-key tiles on its way into shared memory by TMA, across the entries
-//     that the run passes. Heads whose keys fall to several blocks leave
-//     fp32 sums for attn_decode_join_kernel.
+//     its warps side by side in neighbouring heads: those lie together in a
+//     [token][head] cache, whose 128-byte rows otherwise come one to a DRAM page
+//     (4.3 instead of 6.1 TB/s). Each warp keeps a ring of 16-key tiles on its
+//     way into shared memory by TMA, across the entries that the run passes.
+//     Heads whose keys fall to several blocks leave fp32 sums for
+//     attn_decode_join_kernel.
 // Both add up in a fixed order: the same bits each time.
 #pragma once
 
@@ -48,12 +48,6 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {
   asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
-  return v;
-}
-
-__device__ __forceinline__ uint4 load_shared_16(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
   return v;
 }
 
@@ -106,8 +100,7 @@ struct DecodeParams {
   float* LSE;
   const int* lens;  // [B] or null
   int B, Hkv, G, M, N;
-  int row_tiles;    // tiles of 8 R query rows of a kv head
-  int splits;       // blocks (a cluster) that share a tile's keys
+  int splits;       // blocks (a cluster) that share a kv head's keys
   int d16;          // D / 16
   bool causal;      // token m reads lens - (M - 1 - m) keys
   float scale;
@@ -117,15 +110,15 @@ struct DecodeParams {
   const int* prefix_lens; // [B / share] or null
   int share, Np;
   int blocks;         // stream: blocks,
-  int side;           // items (tiles of rows of a kv head) that a block has side by side,
+  int side;           // items (kv heads) that a block has side by side,
   int sub;            // warps to an item (side * sub warps a block)
-  float* run_o;       // [2 * blocks][side][rows of a tile][D] and
-  float2* run_ml;     // [2 * blocks][side][rows of a tile] partial sums
+  float* run_o;       // [2 * blocks][side][8 R rows][D] and
+  float2* run_ml;     // [2 * blocks][side][8 R rows] partial sums
   KernelStatus* status;
   uint64_t timeout_ns;
 };
 
-// A warp's share of one tile of rows: Q, the sums and what they refer to.
+// A warp's share of a kv head's rows: Q, the sums and what they refer to.
 template <typename T, int D, int R>
 struct DecodeWarp {
   static constexpr bool kB = Elem<T>::kBF16;
@@ -134,12 +127,12 @@ struct DecodeWarp {
   float o[R][D / 16][4];
   float m[R][2], l[R][2];
 
-  // Q of rows row0 + g (+ 8), in K's order of columns; no sums yet
-  __device__ __forceinline__ void begin(const DecodeParams<T>& p, int b, int hk, int row0) {
+  // Q of rows g (+ 8), in K's order of columns; no sums yet
+  __device__ __forceinline__ void begin(const DecodeParams<T>& p, int b, int hk) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = row0 + 8 * r + g;
+      const int row = 8 * r + g;
       const T* at = p.Q.at(b, hk * p.G + row / p.M, row % p.M) + 8 * t;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c)
@@ -313,11 +306,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % p.splits;
-  int u = blockIdx.x / p.splits;
-  const int tile = u % p.row_tiles;
-  u /= p.row_tiles;
+  const int u = blockIdx.x / p.splits;
   const int hk = u % p.Hkv, b = u / p.Hkv;
-  const int rows = p.G * p.M, row0 = tile * kRows;
+  const int rows = p.G * p.M;
   const int n = valid_rows(p.lens, b, p.N);
   const int bp = kBehind ? b / p.share : 0, np = kBehind ? valid_rows(p.prefix_lens, bp, p.Np) : 0;
   const int ahead = (np + 15) / 16;  // tiles of the prefix
@@ -354,13 +345,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
     load_v(i);
   }
   DecodeWarp<T, D, R> w;
-  w.begin(p, b, hk, row0);
+  w.begin(p, b, hk);
   int limit[R][2];  // keys that rows 2t and 2t + 1 may read
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int x = 0; x < 2; ++x)
-      limit[r][x] = p.causal ? n - (p.M - 1 - (row0 + 8 * r + 2 * t + x) % p.M) : n;
+      limit[r][x] = p.causal ? n - (p.M - 1 - (8 * r + 2 * t + x) % p.M) : n;
   const float sl2 = p.scale * kLog2e;
   // own keys that every token reads; what infinities and NaN V holds behind them
   // is left out, and added to the tokens that do read it at the end
@@ -410,7 +401,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
       float top = warp_m[0][row];
 #pragma unroll
       for (int y = 1; y < W; ++y) top = fmaxf(top, warp_m[y][row]);
-      if (row0 + row < rows) {
+      if (row < rows) {
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
           float4* at = reinterpret_cast<float4*>(&sum_o[warp][row][64 * c + 8 * g]);
@@ -427,7 +418,6 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
     }
   }
   __syncthreads();
-  const int real = min(kRows, rows - row0);
   auto sum4 = [&](int row, int c) {
     float4 a = *reinterpret_cast<float4*>(&sum_o[0][row][4 * c]);
 #pragma unroll
@@ -435,7 +425,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
     return a;
   };
   if (p.splits > 1) {
-    for (int e = threadIdx.x; e < real * (D / 4); e += kThreads)
+    for (int e = threadIdx.x; e < rows * (D / 4); e += kThreads)
       *reinterpret_cast<float4*>(&sum_o[0][e / (D / 4)][4 * (e % (D / 4))]) = sum4(e / (D / 4), e % (D / 4));
     if (threadIdx.x == 0) block_odd = odd ? 1.f : 0.f;
     cluster_sync();
@@ -459,9 +449,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
     __syncthreads();
   }
   // ---- the blocks' sums: each block finishes a share
-  for (int e = threadIdx.x * p.splits + split; e < real * (D / 4); e += p.splits * kThreads) {
+  for (int e = threadIdx.x * p.splits + split; e < rows * (D / 4); e += p.splits * kThreads) {
     const int row = e / (D / 4), c = e % (D / 4);
-    const int q = row0 + row;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.splits == 1) {
       acc = sum4(row, c);
@@ -469,8 +458,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, decode_blocks(D, R) - (kBeh
 #pragma unroll 4
       for (int y = 0; y < p.splits; ++y) add_weighted(acc, weight[y][row], load_cluster4(&sum_o[0][row][4 * c], y));
     }
-    if (odd) add_odd4(p.V.at(b, hk, shown) + 4 * c, p.V.sr, n - (p.M - 1) + q % p.M - shown, acc);
-    decode_output(p, b, hk, q, c, p.splits == 1 ? block_m[row] : top_of[row], p.splits == 1 ? block_l[row] : total[row],
+    if (odd) add_odd4(p.V.at(b, hk, shown) + 4 * c, p.V.sr, n - (p.M - 1) + row % p.M - shown, acc);
+    decode_output(p, b, hk, row, c, p.splits == 1 ? block_m[row] : top_of[row], p.splits == 1 ? block_l[row] : total[row],
                   acc);
   }
   if (p.splits > 1) cluster_sync();  // no block leaves while its sums are read
@@ -491,7 +480,7 @@ struct DecodeLine {
     return ((valid_rows(p.lens, b, p.N) + 15) / 16 + p.sub - 1) / p.sub;
   }
   __device__ DecodeLine(const DecodeParams<T>& params) : p(params) {
-    groups = (p.Hkv * p.row_tiles + p.side - 1) / p.side;
+    groups = (p.Hkv + p.side - 1) / p.side;
     total = before_entry(p.B);
     each = total / p.blocks;
     more = total % p.blocks;
@@ -603,7 +592,7 @@ __global__ void __launch_bounds__(32 * StreamCfg<D, R>::kWarps, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int items = p.Hkv * p.row_tiles, place = warp % p.side, part = warp / p.side;
+  const int place = warp % p.side, part = warp / p.side;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar) + warp * S;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kOffBar + 8 * Cfg::kWarps * S);
   if (threadIdx.x == 0) {
@@ -625,15 +614,15 @@ __global__ void __launch_bounds__(32 * StreamCfg<D, R>::kWarps, 1)
   int loads = 0;
   auto load = [&](int stage) {  // the next step that has a tile for this warp; all lanes walk, one loads
     for (bool found = false; ahead.left > 0 && !found; ahead.step()) {
-      const int item = ahead.group * p.side + place, i = ahead.j * p.sub + part;
-      found = item < items && 16 * i < ahead.n;
+      const int hk = ahead.group * p.side + place, i = ahead.j * p.sub + part;
+      found = hk < p.Hkv && 16 * i < ahead.n;
       if (found && lane == 0) {
         uint8_t* dst = own + stage * Cfg::kStageBytes;
         mbar_arrive_expect_tx(&bar[stage], Cfg::kStageBytes);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
-          tma_load_4d(dst + c * Cfg::kBox, &tm_K, &bar[stage], 64 * c, 16 * i, item / p.row_tiles, ahead.b, policy);
-          tma_load_4d(dst + kV + c * Cfg::kBox, &tm_V, &bar[stage], 64 * c, 16 * i, item / p.row_tiles, ahead.b, policy);
+          tma_load_4d(dst + c * Cfg::kBox, &tm_K, &bar[stage], 64 * c, 16 * i, hk, ahead.b, policy);
+          tma_load_4d(dst + kV + c * Cfg::kBox, &tm_V, &bar[stage], 64 * c, 16 * i, hk, ahead.b, policy);
         }
       }
       if (found) ++loads;
@@ -647,10 +636,9 @@ __global__ void __launch_bounds__(32 * StreamCfg<D, R>::kWarps, 1)
   bool whole = at.j == 0;  // the group's keys from the first on, in this block
   bool fresh = true, ok = true;
   while (at.left > 0) {
-    const int b = at.b, item = at.group * p.side + place, i = at.j * p.sub + part, n = at.n;
-    const int hk = item / p.row_tiles, row0 = item % p.row_tiles * kRows;
-    const bool mine = item < items;
-    if (fresh && mine) w.begin(p, b, hk, row0);
+    const int b = at.b, hk = at.group * p.side + place, i = at.j * p.sub + part, n = at.n;
+    const bool mine = hk < p.Hkv;
+    if (fresh && mine) w.begin(p, b, hk);
     fresh = false;
     const bool last = at.j + 1 == at.steps;
     const bool opens = at.step();
@@ -740,7 +728,7 @@ __global__ void __launch_bounds__(32 * StreamCfg<D, R>::kWarps, 1)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int row = 8 * r + 2 * t + x;
-          if (row0 + row >= p.G * p.M) continue;
+          if (row >= p.G * p.M) continue;
           const float2 ml = make_float2(w.m[r][x], w.l[r][x]);
 #pragma unroll
           for (int c = 0; c < D / 64; ++c) {
@@ -748,8 +736,8 @@ __global__ void __launch_bounds__(32 * StreamCfg<D, R>::kWarps, 1)
             w.columns(r, x, c, 1.f, a, d);
             const int col4 = 16 * c + 2 * g;
             if (whole && last) {
-              decode_output(p, b, hk, row0 + row, col4, ml.x, ml.y, a);
-              decode_output(p, b, hk, row0 + row, col4 + 1, ml.x, ml.y, d);
+              decode_output(p, b, hk, row, col4, ml.x, ml.y, a);
+              decode_output(p, b, hk, row, col4 + 1, ml.x, ml.y, d);
             } else {
               const int64_t to = (static_cast<int64_t>(slot) * p.side + place) * kRows + row;
               reinterpret_cast<float4*>(p.run_o + to * D)[col4] = a;
@@ -782,7 +770,6 @@ __global__ void __launch_bounds__(D) attn_decode_join_kernel(const __grid_consta
   __shared__ float weight[kMost], mass[kMost], reduce[2][D / 32];
   const int rows = p.G * p.M, q = blockIdx.x % rows;
   const int hk = blockIdx.x / rows % p.Hkv, b = blockIdx.x / rows / p.Hkv;
-  const int item = hk * p.row_tiles + q / kRows, row = q % kRows;
   const DecodeLine<T> line(p);
   const int steps = line.steps_of(b);
   const int c = threadIdx.x % (D / 4), quarter = threadIdx.x / (D / 4);
@@ -791,12 +778,12 @@ __global__ void __launch_bounds__(D) attn_decode_join_kernel(const __grid_consta
     asm volatile("griddepcontrol.wait;" ::: "memory");  // never done before the launch before it
     return;
   }
-  const int start = line.before_entry(b) + item / p.side * steps;
+  const int start = line.before_entry(b) + hk / p.side * steps;
   const int c0 = line.block_of(start), c1 = line.block_of(start + steps - 1);
   const int count = c1 - c0 + 1;
   const int skip = line.mark(c0) < start ? 1 : 0;  // a block that begins in the group has it in its first slot
   auto at = [&](int k) {  // the sum of block c0 + k
-    return ((2ll * (c0 + k) + (k == 0 ? skip : 0)) * p.side + item % p.side) * kRows + row;
+    return ((2ll * (c0 + k) + (k == 0 ? skip : 0)) * p.side + hk % p.side) * kRows + q;
   };
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (count == 1) return;

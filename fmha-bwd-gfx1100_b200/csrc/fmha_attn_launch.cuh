@@ -185,28 +185,25 @@ int enqueue_join(const fmha_attn_t& a, const float* part_o, const float* part_ls
 // cluster of `splits` blocks to a kv head's keys or, `blocks` > 0, that many
 // blocks to equal runs of the whole batch (see DecodeParams).
 struct DecodePlan {
-  int R, row_tiles, splits, blocks, side, sub;
+  int R, splits, blocks, side, sub;
   int64_t tasks;
   uint64_t ws_bytes;
 };
 
 // Stream: evens out lengths and reads at 6.1 TB/s, but costs a second launch
-// and some 15 us in all to fill, drain and join. A block to a tile of rows
-// needs enough of them: 512 (64 entries of 8 heads of 128, up to 512 keys) take
+// and some 15 us in all to fill, drain and join. A block to a kv head needs
+// enough of them: 512 (64 entries of 8 heads of 128, up to 512 keys) take
 // 19 us, 34 streamed; 1024 of 1500 keys of 64 columns 72 and 79 us. With fewer
 // than the GPU holds at a time, clusters divide the keys (some 9 ns a block for
 // the launch): 16 x 4000 keys of 8 heads of 128 take 63 us that way, 51
-// streamed. So streamed are calls of kStreamBytes of keys and values whose
-// tiles of rows do not fill the GPU, or whose lengths can differ much
-// (kStreamKeys). `part`: the output goes to a join anyway, behind a prefix.
+// streamed. So streamed are calls of kStreamBytes of keys and values whose kv
+// heads do not fill the GPU, or whose lengths can differ much (kStreamKeys). `part`: the output goes to a join anyway, behind a prefix.
 constexpr int kStreamKeys = 8192;
 constexpr int64_t kStreamBytes = 96ll << 20;
 inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N, int D, bool part) {
   DecodePlan d;
-  const int64_t rows = static_cast<int64_t>(G) * M;
-  d.R = rows <= 8 ? 1 : 2;
-  d.row_tiles = static_cast<int>((rows + 8 * d.R - 1) / (8 * d.R));
-  d.tasks = static_cast<int64_t>(B) * Hkv * d.row_tiles;
+  d.R = static_cast<int64_t>(G) * M <= 8 ? 1 : 2;
+  d.tasks = static_cast<int64_t>(B) * Hkv;
   d.splits = d.side = d.sub = 1;
   d.blocks = 0;
   d.ws_bytes = 0;
@@ -215,14 +212,13 @@ inline DecodePlan plan_decode(int M, int G, int B, int Hkv, int N, int D, bool p
   if (!part && d.tasks * N * D * 4 >= kStreamBytes && (d.tasks < slots || N >= kStreamKeys) && d.tasks * tiles < (1ll << 30)) {
     const int warps = D == 128 ? (d.R == 1 ? StreamCfg<128, 1>::kWarps : StreamCfg<128, 2>::kWarps)
                                : (d.R == 1 ? StreamCfg<64, 1>::kWarps : StreamCfg<64, 2>::kWarps);
-    // as many items side by side as leave the fewest warps without one
-    const int items = Hkv * d.row_tiles;
+    // as many heads side by side as leave the fewest warps without one
     int best = warps;
     for (int side = warps; side >= 1; --side) {
       if (warps % side != 0) continue;
-      const int idle = (items + side - 1) / side * side - items;
-      const int64_t spent = static_cast<int64_t>(items + idle) * ((tiles + warps / side - 1) / (warps / side)) * (warps / side);
-      const int64_t least = static_cast<int64_t>((items + best - 1) / best * best) *
+      const int64_t spent = static_cast<int64_t>((Hkv + side - 1) / side * side) *
+                            ((tiles + warps / side - 1) / (warps / side)) * (warps / side);
+      const int64_t least = static_cast<int64_t>((Hkv + best - 1) / best * best) *
                             ((tiles + warps / best - 1) / (warps / best)) * (warps / best);
       if (spent < least) best = side;
     }
@@ -281,7 +277,6 @@ int enqueue_decode(const fmha_attn_t& a, AttnOp op, float* part_o, float* part_l
   p.G = G;
   p.M = a.M;
   p.N = a.N;
-  p.row_tiles = d.row_tiles;
   p.splits = d.splits;
   p.causal = op == AttnOp::kPrefix;
   p.d16 = a.K_dim / 16;
