@@ -218,7 +218,7 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cas
 // also a tile's largest finite |dO|, and a key tile's |V|. What the other kernels
 // have no items for is zeroed here: dQ of entries without keys, dK and dV behind
 // the last key (a tile's sums there would be NaN where Q or dO is). Bound by memory: 101
-// MB (2 x 24 heads, 4096 rows of 128) take 25 us from DRAM; more blocks with
+// MB (2 x 24 heads, 4096 rows of 128) take 25 to 31 us from DRAM; more blocks with
 // fewer loads each were slower.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(256)
 //
 // Shared memory (D = 128): Q, dO of both tiles 128 KB, K x2, V x1 = 224 KB.
 // TMEM: R_t [128 t, +128), dQ_t [256 + D t, +D).
-// 2 x 24 heads, 4096 rows, 128 and 512 keys of 128: 66 us, 0.73 PFLOP/s, the
-// tensor pipe 35 % busy; bound by a tile's chain S, P, dP, dS, product, of which
+// 2 x 24 heads, 4096 rows, 128 and 512 keys of 128: 66 to 70 us, 0.7 PFLOP/s,
+// the tensor pipe 33 to 35 % busy; bound by a tile's chain S, P, dP, dS, product, of which
 // the two tiles overlap about half.
 // Both kernels: warpgroups 0 to 3 form P and dS, 4 stores the sums, 5 holds the
 // TMA producer (warp 20), two MMA issuers (21, 23) and the scheduler (22). The
@@ -727,8 +727,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 //   dV += P^T dO;  dP^T = V dO^T -> TMEM;  dS^T, 16-bit, over dP^T;  dK += dS^T Q
 // The warps form dS^T during dV and S^T of the next tile, and its P^T during
 // dK and the next dP^T.
-// 2 x 24 heads, 4096 rows, 128 and 512 keys of 128: 81 us,
-// 0.80 PFLOP/s, the tensor pipe 38 % busy, bound by the same chain.
+// 2 x 24 heads, 4096 rows, 128 and 512 keys of 128: 74 to 81 us, 0.80 to 0.87 PFLOP/s,
+// the tensor pipe 38 to 42 % busy, bound by the same chain.
 //
 // Shared memory (D = 128): K, V 64 KB, Q x3, dO x2 160 KB, nlse2 and ndelta.
 // (With two Q slots, S^T waited some 700 cycles a step for its Q: the slot is

@@ -291,7 +291,7 @@ constexpr int kMostSplits = 16, kDecodeWarps = 4;
 // Blocks that an SM holds at a time.
 __host__ __device__ constexpr int decode_blocks(int D, int R) { return D == 128 ? (R == 1 ? 3 : 2) : (R == 1 ? 5 : 4); }
 
-// 64 x 16 heads, 1500 keys of 64: 72 us, 5.5 TB/s; 8 kv heads of 4096 keys of
+// 64 x 16 heads, 1500 keys of 64: 72 to 75 us, 5.2 to 5.5 TB/s; 8 kv heads of 4096 keys of
 // 128 in clusters of 16: 12 us, bound by latency (lengths, first keys, Q, the
 // exchange).
 // kBehind: over a shared prefix's keys and an entry's own in one go.
@@ -576,8 +576,8 @@ struct StreamCfg {
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
-// 4 entries of 8 kv heads, 4096 to 32768 keys of 128: 48 us without the join,
-// 5.9 TB/s; blocks of equal work end 38 to 48 us after the start.
+// 4 entries of 8 kv heads, 4096 to 32768 keys of 128: 48 to 53 us without the
+// join, 5.4 to 5.9 TB/s; blocks of equal work end 38 to 48 us after the start.
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(32 * StreamCfg<D, R>::kWarps, 1)
     attn_decode_stream_kernel(const __grid_constant__ CUtensorMap tm_K, const __grid_constant__ CUtensorMap tm_V,

@@ -437,8 +437,8 @@ __device__ __forceinline__ void weights_32(const uint32_t* s, float2 sc, float2 
   }
 }
 
-// 16384 rows, 1024 keys, 40 heads of 128, bf16: 315 to 355 us by the GPU's clock
-// (1.0 to 1.1 PFLOP/s). A step of both tiles takes 3.7 K clocks, of which the
+// 16384 rows, 1024 keys, 40 heads of 128, bf16: 343 to 366 us by the GPU's clock
+// (0.94 to 1.0 PFLOP/s). A step of both tiles takes 3.7 K clocks, of which the
 // exponentials take the SFU 2.0 K and the products the tensor core 2.0 K: each
 // tile's softmax waits for the products between its p and its next S. Few steps
 // are bound by latency: 3 to 4 us pass before the first S.

@@ -369,9 +369,9 @@ def cross_attn_fwd(Q, K, V, kv_lens=None, scale=None, *, out=None, stream=None, 
     the fp32 row log-sum-exp that fmha_bwd_lse and cross_attn_bwd take.
 
     Q: [B, Hq, M, d]; K, V: [B, Hkv, N, d], Hq a multiple of Hkv (query head h
-    reads kv head h // (Hq // Hkv)). Any strides that are multiples of 8
-    elements with unit stride along d, so the transposed views of [B, rows, H,
-    d] projections need no copy. ``kv_lens``: int32 [B] on the device, the
+    reads kv head h // (Hq // Hkv)). Any strides above 0 that are multiples of
+    8 elements, with unit stride along d, so the transposed views of [B, rows,
+    H, d] projections need no copy (broadcast views, with stride 0, do). ``kv_lens``: int32 [B] on the device, the
     valid rows of K and V (None: all); what lies behind them is never used. A
     row without valid keys gets O = 0 and LSE = -inf. ``scale`` defaults to
     1/sqrt(d). M = 1 is the form for single tokens: each K and V is then read
@@ -428,8 +428,9 @@ def prefix_attn(Q, Kp, Vp, K, V, prefix_lens=None, kv_lens=None, scale=None, *, 
     b // (B // P)), of which prefix_lens[p] rows count. K, V: [B, Hkv, N, d],
     each entry's own cache behind the prefix, of which kv_lens[b] rows count,
     the M newest tokens' own rows last: row m sees all but the M - 1 - m
-    newest. The softmax runs over both. The prefix is read once for all of
-    its entries. Strides, ``out``, ``stream`` and ``sync`` as cross_attn_fwd."""
+    newest, and nothing of those reaches it. The softmax runs over both. The
+    prefix is read once for all of its entries, or once for each where that is
+    little. Strides, ``out``, ``stream`` and ``sync`` as cross_attn_fwd."""
     shape = B, Hq, M, d = Q.shape
     kshape, dev = _check_qkv(Q, shape, K, V)
     pshape, _ = _check_qkv(Q, shape, Kp, Vp, ("Kp", "Vp"))

@@ -177,7 +177,8 @@ int fmha_bwd_full_noalloc(fmha_bf16_t* dQ, fmha_bf16_t* dK, fmha_bf16_t* dV,
  *   LSE = log sum_n exp(S),   O = sum_n exp(S - LSE) V.
  * A row without valid keys gets O = 0 and LSE = -inf. M = 1 is the form for
  * single tokens. No counterpart in the reference, which starts from P.
- * Stream-ordered; allocates nothing; returns 0 or an error code. */
+ * Stream-ordered; allocates nothing but, with the first call on a device, one
+ * pinned status word; returns 0 or an error code. */
 int fmha_cross_fwd(const fmha_attn_t* args, fmha_stream_t stream);
 
 /* Its backward, from O and LSE as the forward left them and dO:
@@ -194,7 +195,9 @@ int fmha_cross_bwd(const fmha_attn_t* args, fmha_stream_t stream);
  * cache K, V behind it (its first kv_lens[b] rows, the M newest tokens
  * last: row m reads kv_lens[b] - (M - 1 - m) of them, and nothing of the
  * others reaches it, NaN and infinities included), in one softmax. O and LSE
- * as fmha_cross_fwd. The prefix is read once for all entries. */
+ * as fmha_cross_fwd. The prefix is read once for all entries, or, where the
+ * whole call reads 48 MB so at most or each entry has a prefix of its own, once
+ * for each. */
 int fmha_prefix_attn(const fmha_attn_t* args, fmha_stream_t stream);
 
 /* Stage hooks (replace the reference's test_* wrappers,
